@@ -4,6 +4,9 @@
  *   1. exact_int8 linear layer: fixed-point digitization + exact two-digit integer GEMM with fused epilogue;
  *   2. batch-invariant paged decode attention.
  *
+ * and the attention operators around a served cache: an 8-bit paged cache (write, read back, decode over it), the
+ * verification of drafted tokens over a cache, and causal attention of packed prompts.
+ *
  * Conventions (all entry points):
  *   - every pointer is caller-owned device memory; nothing here allocates device memory;
  *   - every call is asynchronous and stream-ordered on `stream` (a cudaStream_t; NULL = legacy default stream);
@@ -259,6 +262,90 @@ int ex_paged_decode_leading(const void* q, int64_t sq_t, int64_t sq_h, const voi
                             const int32_t* query_start_loc, int n, int H, int KV, int D, int BS, float scale,
                             int max_len, int split, void* out, int64_t so_t, int64_t so_h, int out_dtype,
                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Codes of an 8-bit cache. A row (one token, one KV head) of D numbers x is held as codes c and one float32 scale
+ * s = max|x| / Q, with c = x / s rounded to nearest even and Q = 127 (int8) or 448 (e4m3, 1 sign, 4 exponent and 3
+ * mantissa bits); it stands for c * s. A row with an infinity or a NaN is held so that it reads back as NaN. */
+enum { EX_CODE_NONE = -1 /* not quantised: bf16 or fp16 */, EX_CODE_INT8 = 0, EX_CODE_E4M3 = 1 };
+
+/*
+ * Quantises the keys and values of `tokens` tokens into an 8-bit paged cache. No counterpart in the reference, whose
+ * caches are bf16.
+ *   key, value  tokens x KV x D, bf16 or fp16 (dtype), strides (s*_t, s*_h, 1)
+ *   k_cache, v_cache  codes, num_blocks x BS x KV x D bytes with strides (s_block, s_page, s_head, 1), each a multiple
+ *               of 16; D = 64, 128 or 256
+ *   k_scale, v_scale  float32, num_blocks x KV x BS with strides (ss_block, ss_head, 1)
+ *   slots       int64: token t goes to block slots[t] / BS, place slots[t] % BS; a token whose slot is negative or not
+ *               in the cache is not written. The slots of one call must differ from each other.
+ *   key_out, value_out  both NULL, or arrays like key and value that get the numbers which the written rows stand for
+ *               (of every token, written or not): what attention over the cache will see.
+ */
+int ex_cache_write_q8(const void* key, int64_t sk_t, int64_t sk_h, const void* value, int64_t sv_t, int64_t sv_h,
+                      int dtype, int code, void* k_cache, void* v_cache, int64_t s_block, int64_t s_page, int64_t s_head,
+                      float* k_scale, float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks, int BS,
+                      const int64_t* slots, int64_t tokens, int KV, int D, void* key_out, int64_t sko_t, int64_t sko_h,
+                      void* value_out, int64_t svo_t, int64_t svo_h, void* stream);
+
+/*
+ * Reads the first cu_seqlens[b + 1] - cu_seqlens[b] tokens of every sequence b < n back from an 8-bit cache into rows
+ * cu_seqlens[b] .. of key_out and value_out (rows x KV x D, bf16 or fp16). Rows outside the sequences, behind the
+ * block table (n x width) or on a page that is not in [0, num_blocks) are left as they were.
+ */
+int ex_cache_read_q8(const void* k_cache, const void* v_cache, int code, int64_t s_block, int64_t s_page, int64_t s_head,
+                     const float* k_scale, const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                     int BS, const int32_t* block_table, int64_t sbt, int width, const int32_t* cu_seqlens, int n,
+                     int64_t rows, int KV, int D, int dtype, void* key_out, int64_t sko_t, int64_t sko_h, void* value_out,
+                     int64_t svo_t, int64_t svo_h, void* stream);
+
+/* Bytes of (uninitialised) workspace that ex_paged_decode_q8 (tokens = n) and ex_tree_attention need; max_len as in
+ * the call, or larger. */
+size_t ex_paged_rows_workspace_bytes(int64_t tokens, int H, int D, int64_t max_len);
+
+/*
+ * ex_paged_decode over an 8-bit cache (as ex_cache_write_q8 makes it): one query token per request, softmax(scale *
+ * q.K^T) V over its first seq_lens[b] tokens, out in q's type (bf16 or fp16). D = 64, 128 or 256, H / KV <= 16, BS a
+ * multiple of 8. Keys are processed in segments fixed by the request's own length and merged in order, so a request's
+ * bits do not depend on n, on the other requests or on where its pages are.
+ *   - a request of length 0 gives zeros
+ *   - tokens behind max_len or behind the block table (n x width), and tokens on pages outside [0, num_blocks), are
+ *     not seen
+ *   - scales must start on 16 bytes, their strides be multiples of 4
+ */
+int ex_paged_decode_q8(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
+                       int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,
+                       const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                       const int32_t* block_table, int64_t sbt, int width, const int32_t* seq_lens, int n, int H, int KV,
+                       int D, int BS, float scale, int64_t max_len, void* out, int64_t so_t, int64_t so_h,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of drafted tokens over a paged cache, 16-bit (code = EX_CODE_NONE, element type q_dtype) or 8-bit. Request
+ * b has the query rows query_start_loc[b] .. query_start_loc[b + 1] (T_b <= max_tokens <= 64 of them); its last T_b
+ * cached tokens of seq_lens[b] are those drafted tokens themselves. Every row sees the seq_lens[b] - T_b tokens of the
+ * context, and of the drafted tokens those of its bits: row r sees drafted token j if bit j of tree_mask[r] is set
+ * (tree_mask NULL: those up to itself, a chain). A row that sees nothing gives zeros. A request with more than
+ * max_tokens rows, or with rows that q (tokens rows) does not have, is left untouched, as are rows of no request.
+ * Other conventions as ex_paged_decode_q8; a row's bits depend on its own request alone.
+ */
+int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
+                      int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,
+                      const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                      const int32_t* block_table, int64_t sbt, int width, const int32_t* seq_lens,
+                      const int32_t* query_start_loc, const int64_t* tree_mask, int n, int64_t tokens, int max_tokens,
+                      int H, int KV, int D, int BS, float scale, int64_t max_len, void* out, int64_t so_t, int64_t so_h,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention of packed prompts: sequence b < n has query rows cu_q[b] .. cu_q[b + 1] of q (tokens x H x D) and
+ * key rows cu_k[b] .. cu_k[b + 1] of k and v (keys x KV x D), all bf16 or all fp16; its last query is its last key's
+ * token, so query i sees keys j <= i + Lk - Lq (the keys may start before the queries: a continued conversation). A
+ * query that sees no key gives zeros. Rows of no sequence are left untouched; a sequence whose offsets leave the
+ * arrays is skipped. A row's bits depend on its own sequence alone.
+ */
+int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                        const void* v, int64_t sv_t, int64_t sv_h, int dtype, const int32_t* cu_q, const int32_t* cu_k,
+                        int n, int64_t tokens, int64_t keys, int H, int KV, int D, float scale, void* out, int64_t so_t,
+                        int64_t so_h, void* stream);
 
 #ifdef __cplusplus
 }

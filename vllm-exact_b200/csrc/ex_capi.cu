@@ -14,6 +14,9 @@
 #include "ex_gemm_tc.cuh"
 #include "ex_paged_decode.cuh"
 #include "ex_paged_decode_tma.cuh"
+#include "ex_cache_q8.cuh"
+#include "ex_paged_rows.cuh"
+#include "ex_prompt_attn.cuh"
 
 // Split-K scratch of ex_linear_noalloc: a file-scope device array, so that entry point never allocates. Host code
 // must not hand this symbol to a kernel (on the host it is only a stand-in); the device address is looked up once per
@@ -248,6 +251,194 @@ size_t linear_ws(int64_t M, int64_t N, int64_t K, int split_k, int algo) {
   const size_t b = ex::tc_plan(M, N, K, split_k, num_sms(), ex::tc_cluster_cap()).ws_bytes;
   if (algo == EX_ALGO_TC_I8) return b;
   return std::max(a, b);  // automatic choice: enough for either algorithm
+}
+
+// 4-D tensor map over a paged K or V cache of any element type for k_paged_rows: boxes of `box_rows` tokens of one
+// page and head, `pitch` bytes of the head dimension wide.
+bool encode_rows_map(CUtensorMap* map, const void* base, int esz, int D, int KV, int BS, int64_t num_blocks,
+                     int64_t s_head, int64_t s_page, int64_t s_block, int pitch, int box_rows) {
+  ex::PFN_encodeTiled enc = ex::get_encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)KV, (cuuint64_t)BS, (cuuint64_t)num_blocks};
+  cuuint64_t strides[3] = {(cuuint64_t)s_head * esz, (cuuint64_t)s_page * esz, (cuuint64_t)s_block * esz};
+  cuuint32_t box[4] = {(cuuint32_t)(pitch / esz), 1, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, esz == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base),
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             pitch == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The stride of a dimension of one element says nothing (callers pass whatever their array type reports): D instead.
+void one_element(int64_t size, int D, int64_t& stride) {
+  if (size == 1) stride = D;
+}
+bool misaligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+bool half_dtype(int d) { return d == EX_DTYPE_BF16 || d == EX_DTYPE_F16; }
+bool head_size_ok(int D) { return D == 64 || D == 128 || D == 256; }
+
+template <int D, int CODE, bool F16, int NT>
+cudaError_t launch_rows_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
+                          cudaStream_t st) {
+  using C = ex::PrCfg<D, CODE, NT>;
+  static bool done[128] = {};  // the attribute is per device and kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 128 || !done[dev]) {
+    e = cudaFuncSetAttribute(ex::k_paged_rows<D, CODE, F16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev < 128) done[dev] = true;
+  }
+  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
+  return ex_launch_pdl(ex::k_paged_rows<D, CODE, F16, NT>, dim3(grid), dim3(ex::PR_THREADS), C::SMEM, st, mk, mv, a);
+}
+
+template <int D, int CODE, bool F16>
+cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t per_tile,
+                           cudaStream_t st) {
+  if (rows <= 8) return launch_rows_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
+  if (rows <= 16) return launch_rows_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
+  if (rows <= 32 || D == 256) return launch_rows_t<D, CODE, F16, 4>(mk, mv, a, per_tile * cdiv(rows, 32), st);
+  if constexpr (D != 256) return launch_rows_t<D, CODE, F16, 8>(mk, mv, a, per_tile * cdiv(rows, 64), st);
+  return cudaErrorInvalidValue;
+}
+
+template <int D>
+cudaError_t launch_rows_d(int code, int q_dtype, int rows, const CUtensorMap& mk, const CUtensorMap& mv,
+                          const ex::PrArgs& a, int64_t per_tile, cudaStream_t st) {
+  cudaError_t e;
+  if (code == ex::CODE_INT8) e = launch_rows_nt<D, ex::CODE_INT8, true>(rows, mk, mv, a, per_tile, st);
+  else if (code == ex::CODE_E4M3) e = launch_rows_nt<D, ex::CODE_E4M3, true>(rows, mk, mv, a, per_tile, st);
+  else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, a, per_tile, st);
+  else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, a, per_tile, st);
+  if (e != cudaSuccess || a.NS == 1) return e;
+  const dim3 grid((unsigned)cdiv(a.tokens * a.H, 8)), block(256);
+  if (q_dtype == EX_DTYPE_F16) return ex_launch_pdl(ex::k_paged_rows_merge<D, true>, grid, block, 0, st, a);
+  return ex_launch_pdl(ex::k_paged_rows_merge<D, false>, grid, block, 0, st, a);
+}
+
+// ex_paged_decode_q8 and ex_tree_attention: checks, tensor maps, launches.
+int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache, int code,
+               int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale, const float* v_scale,
+               int64_t ss_block, int64_t ss_head, int64_t num_blocks, const int32_t* block_table, int64_t sbt, int width,
+               const int32_t* seq_lens, const int32_t* qsl, const int64_t* mask, int n, int64_t tokens, int max_tokens,
+               int H, int KV, int D, int BS, float scale, int64_t max_len, void* out, int64_t so_t, int64_t so_h,
+               void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  if (n < 0 || tokens < 0 || tokens > INT32_MAX || H <= 0 || KV <= 0 || H % KV != 0 || BS <= 0 || width < 0 || max_len < 0)
+    return EX_ERR_ARG;
+  if (code < ex::CODE_NONE || code > ex::CODE_E4M3 || max_tokens < 1) return EX_ERR_ARG;
+  if (!half_dtype(q_dtype)) return EX_ERR_DTYPE;
+  const int G = H / KV;
+  if (G > 16 || !head_size_ok(D) || BS % 8 != 0 || max_tokens > ex::PR_MAX_TOKENS) return EX_ERR_UNSUPPORTED;
+  if (n == 0 || tokens == 0) return EX_OK;
+  if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !out || num_blocks <= 0) return EX_ERR_ARG;
+  if (code != ex::CODE_NONE && (!k_scale || !v_scale)) return EX_ERR_ARG;
+  for (int64_t* s : {&sq_t, &so_t}) one_element(tokens, D, *s);
+  for (int64_t* s : {&sq_h, &so_h}) one_element(H, D, *s);
+  for (int64_t* s : {&s_head, &ss_head}) one_element(KV, D, *s);
+  for (int64_t* s : {&s_block, &ss_block}) one_element(num_blocks, D, *s);
+  const int esz = code == ex::CODE_NONE ? 2 : 1, vec = 16 / esz;
+  if (misaligned(q, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(out, 4) || sq_t % 8 != 0 ||
+      sq_h % 8 != 0 || s_block % vec != 0 || s_page % vec != 0 || s_head % vec != 0 || so_t % 2 != 0 || so_h % 2 != 0)
+    return EX_ERR_ALIGN;
+  if (code != ex::CODE_NONE && (misaligned(k_scale, 16) || misaligned(v_scale, 16) || ss_block % 4 != 0 || ss_head % 4 != 0))
+    return EX_ERR_ALIGN;
+  max_len = std::min<int64_t>(max_len, std::min<int64_t>((int64_t)width * BS, INT32_MAX - 4096));
+  const int NS = ex::pr_max_segments(max_len);
+  const int64_t rows = tokens * H * NS;
+  const size_t need = ex_paged_rows_workspace_bytes(tokens, H, D, max_len);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return EX_ERR_WORKSPACE;
+  if (need > 0 && misaligned(workspace, 256)) return EX_ERR_ALIGN;
+  const int per_tile_rows = max_tokens * G;
+  const int64_t per_tile = (int64_t)n * NS * KV;
+  if (per_tile * cdiv(per_tile_rows, 8) > INT32_MAX) return EX_ERR_UNSUPPORTED;  // items are numbered in 32 bits
+  if (!ex::device_is_sm100()) return EX_ERR_UNSUPPORTED;
+  ex::PrArgs a = {};
+  a.q = q; a.sq_t = sq_t; a.sq_h = sq_h; a.q_is_f16 = q_dtype == EX_DTYPE_F16;
+  a.bt = block_table; a.sbt = sbt; a.seq_lens = seq_lens; a.qsl = qsl;
+  a.mask = reinterpret_cast<const uint64_t*>(mask);
+  a.n = n; a.H = H; a.G = G; a.KV = KV; a.BS = BS; a.group_log2 = BS % 16 == 0 ? 4 : 3; a.max_tokens = max_tokens;
+  a.max_keys = (int)max_len; a.blocks = num_blocks; a.tokens = tokens; a.scale_log2 = scale * ex::PR_LOG2E;
+  a.k_scale = k_scale; a.v_scale = v_scale; a.ss_block = ss_block; a.ss_head = ss_head; a.NS = NS;
+  if (need > 0) {
+    char* w = reinterpret_cast<char*>(workspace);
+    a.ws_m = reinterpret_cast<float*>(w);
+    a.ws_l = reinterpret_cast<float*>(w + align_up((size_t)rows * 4, 256));
+    a.ws_acc = reinterpret_cast<float*>(w + 2 * align_up((size_t)rows * 4, 256));
+  }
+  a.out = out; a.so_t = so_t; a.so_h = so_h;
+  const int pitch = std::min(128, D * esz), box = 1 << a.group_log2;
+  CUtensorMap mk, mv;
+  if (!encode_rows_map(&mk, k_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box) ||
+      !encode_rows_map(&mv, v_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box))
+    return EX_ERR_UNSUPPORTED;
+  cudaError_t e;
+  if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  return cuda_status(e);
+}
+
+template <int D, bool F16>
+cudaError_t launch_prompt(const ex::PaArgs& a, cudaStream_t st) {
+  const int smem = 3 * 64 * D * 2;
+  cudaError_t e = cudaFuncSetAttribute(ex::k_prompt_attn<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (a.tokens + ex::PS_ROWS - 1) / ex::PS_ROWS + a.n;  // at least as many as there are
+  return ex_launch_pdl(ex::k_prompt_attn<D, F16>, dim3((unsigned)(tiles * a.H)), dim3(128), smem, st, a);
+}
+
+template <int D, int CODE>
+cudaError_t launch_cache_write(const void* key, const void* value, int f16, int64_t sk_t, int64_t sk_h, int64_t sv_t,
+                               int64_t sv_h, const ex::CacheView& c, const int64_t* slots, int64_t tokens, int KV,
+                               void* ko, void* vo, int64_t sko_t, int64_t sko_h, int64_t svo_t, int64_t svo_h,
+                               cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv(tokens * 2 * KV * (D / 8), ex::CQ_THREADS)), block(ex::CQ_THREADS);
+  if (f16)
+    return ex_launch_pdl(ex::k_cache_write<D, CODE, __half>, grid, block, 0, st, (const __half*)key, (const __half*)value,
+                         sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, (__half*)ko, (__half*)vo, sko_t, sko_h, svo_t, svo_h);
+  return ex_launch_pdl(ex::k_cache_write<D, CODE, __nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16*)key,
+                       (const __nv_bfloat16*)value, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, (__nv_bfloat16*)ko,
+                       (__nv_bfloat16*)vo, sko_t, sko_h, svo_t, svo_h);
+}
+
+template <int D, int CODE>
+cudaError_t launch_cache_read(const ex::CacheView& c, const int32_t* bt, int64_t sbt, int width, const int32_t* cu, int n,
+                              int64_t rows, int KV, int f16, void* ko, void* vo, int64_t sko_t, int64_t sko_h,
+                              int64_t svo_t, int64_t svo_h, cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv(rows, ex::CQ_THREADS / 32)), block(ex::CQ_THREADS);
+  if (f16)
+    return ex_launch_pdl(ex::k_cache_read<D, CODE, __half>, grid, block, 0, st, c, bt, sbt, width, cu, n, rows, KV,
+                         (__half*)ko, (__half*)vo, sko_t, sko_h, svo_t, svo_h);
+  return ex_launch_pdl(ex::k_cache_read<D, CODE, __nv_bfloat16>, grid, block, 0, st, c, bt, sbt, width, cu, n, rows, KV,
+                       (__nv_bfloat16*)ko, (__nv_bfloat16*)vo, sko_t, sko_h, svo_t, svo_h);
+}
+
+// Shared checks of the two cache entry points.
+int check_cache(int dtype, int code, const void* k_cache, const void* v_cache, int64_t& s_block, int64_t& s_page,
+                int64_t& s_head, const float* k_scale, const float* v_scale, int64_t num_blocks, int BS, int KV, int D) {
+  if (KV <= 0 || BS <= 0 || num_blocks <= 0 || code < ex::CODE_INT8 || code > ex::CODE_E4M3) return EX_ERR_ARG;
+  if (!half_dtype(dtype)) return EX_ERR_DTYPE;
+  if (!head_size_ok(D)) return EX_ERR_UNSUPPORTED;
+  if (!k_cache || !v_cache || !k_scale || !v_scale) return EX_ERR_ARG;
+  one_element(KV, D, s_head);
+  one_element(BS, D, s_page);
+  one_element(num_blocks, D, s_block);
+  if (misaligned(k_cache, 16) || misaligned(v_cache, 16) || s_block % 16 != 0 || s_page % 16 != 0 || s_head % 16 != 0 ||
+      misaligned(k_scale, 4) || misaligned(v_scale, 4))
+    return EX_ERR_ALIGN;
+  return EX_OK;
+}
+
+ex::CacheView cache_view(const void* k, const void* v, int64_t s_block, int64_t s_page, int64_t s_head, const float* ks,
+                         const float* vs, int64_t ss_block, int64_t ss_head, int64_t blocks, int BS) {
+  ex::CacheView c;
+  c.key = (uint8_t*)const_cast<void*>(k); c.value = (uint8_t*)const_cast<void*>(v);
+  c.s_block = s_block; c.s_page = s_page; c.s_head = s_head;
+  c.key_scale = const_cast<float*>(ks); c.value_scale = const_cast<float*>(vs);
+  c.ss_block = ss_block; c.ss_head = ss_head; c.blocks = blocks; c.page = BS;
+  return c;
 }
 
 }  // namespace
@@ -591,6 +782,136 @@ int ex_paged_decode_leading(const void* q, int64_t sq_t, int64_t sq_h, const voi
   if ((e = cudaGetLastError()) != cudaSuccess) return cuda_status(e);
   return launch_merge(ws_m, ws_l, ws_acc, out, so_t, so_h, n, H, NS, D, out_dtype, seq_lens, split,
                         query_start_loc, st);
+}
+
+size_t ex_paged_rows_workspace_bytes(int64_t tokens, int H, int D, int64_t max_len) {
+  if (tokens <= 0 || H <= 0 || D <= 0 || max_len < 0) return 0;
+  const int64_t NS = ex::pr_max_segments(std::min<int64_t>(max_len, INT32_MAX - 4096));
+  if (NS == 1) return 0;
+  const size_t rows = (size_t)tokens * H * NS;
+  return align_up(rows * 4, 256) * 2 + rows * D * 4;
+}
+
+int ex_paged_decode_q8(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
+                       int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,
+                       const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                       const int32_t* block_table, int64_t sbt, int width, const int32_t* seq_lens, int n, int H, int KV,
+                       int D, int BS, float scale, int64_t max_len, void* out, int64_t so_t, int64_t so_h,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  if (code == EX_CODE_NONE) return EX_ERR_ARG;
+  return paged_rows(q, sq_t, sq_h, q_dtype, k_cache, v_cache, code, s_block, s_page, s_head, k_scale, v_scale, ss_block,
+                    ss_head, num_blocks, block_table, sbt, width, seq_lens, nullptr, nullptr, n, n, 1, H, KV, D, BS,
+                    scale, max_len, out, so_t, so_h, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
+                      int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,
+                      const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                      const int32_t* block_table, int64_t sbt, int width, const int32_t* seq_lens,
+                      const int32_t* query_start_loc, const int64_t* tree_mask, int n, int64_t tokens, int max_tokens,
+                      int H, int KV, int D, int BS, float scale, int64_t max_len, void* out, int64_t so_t, int64_t so_h,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (n > 0 && !query_start_loc) return EX_ERR_ARG;
+  return paged_rows(q, sq_t, sq_h, q_dtype, k_cache, v_cache, code, s_block, s_page, s_head, k_scale, v_scale, ss_block,
+                    ss_head, num_blocks, block_table, sbt, width, seq_lens, query_start_loc, tree_mask, n, tokens,
+                    max_tokens, H, KV, D, BS, scale, max_len, out, so_t, so_h, workspace, workspace_bytes,
+                    (cudaStream_t)stream);
+}
+
+int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                        const void* v, int64_t sv_t, int64_t sv_h, int dtype, const int32_t* cu_q, const int32_t* cu_k,
+                        int n, int64_t tokens, int64_t keys, int H, int KV, int D, float scale, void* out, int64_t so_t,
+                        int64_t so_h, void* stream) {
+  if (n < 0 || tokens < 0 || keys < 0 || tokens > INT32_MAX / 2 || keys > INT32_MAX / 2 || H <= 0 || KV <= 0 || H % KV != 0)
+    return EX_ERR_ARG;
+  if (!half_dtype(dtype)) return EX_ERR_DTYPE;
+  if (!head_size_ok(D)) return EX_ERR_UNSUPPORTED;
+  if (n == 0 || tokens == 0) return EX_OK;
+  if (!q || !cu_q || !cu_k || !out || (keys > 0 && (!k || !v))) return EX_ERR_ARG;
+  for (int64_t* s : {&sq_t, &so_t}) one_element(tokens, D, *s);
+  for (int64_t* s : {&sk_t, &sv_t}) one_element(keys, D, *s);
+  for (int64_t* s : {&sq_h, &so_h}) one_element(H, D, *s);
+  for (int64_t* s : {&sk_h, &sv_h}) one_element(KV, D, *s);
+  if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(out, 16) || sq_t % 8 != 0 ||
+      sq_h % 8 != 0 || sk_t % 8 != 0 || sk_h % 8 != 0 || sv_t % 8 != 0 || sv_h % 8 != 0 || so_t % 8 != 0 || so_h % 8 != 0)
+    return EX_ERR_ALIGN;
+  if ((cdiv(tokens, ex::PS_ROWS) + n) * H > INT32_MAX) return EX_ERR_UNSUPPORTED;
+  if (!ex::device_is_sm100()) return EX_ERR_UNSUPPORTED;
+  ex::PaArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.sq_t = sq_t; a.sq_h = sq_h; a.sk_t = sk_t; a.sk_h = sk_h; a.sv_t = sv_t; a.sv_h = sv_h;
+  a.cu_q = cu_q; a.cu_k = cu_k; a.n = n; a.H = H; a.G = H / KV; a.tokens = tokens; a.keys = keys;
+  a.scale_log2 = scale * ex::PR_LOG2E; a.out = out; a.so_t = so_t; a.so_h = so_h;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = dtype == EX_DTYPE_F16;
+  if (D == 64) return cuda_status(f16 ? launch_prompt<64, true>(a, st) : launch_prompt<64, false>(a, st));
+  if (D == 128) return cuda_status(f16 ? launch_prompt<128, true>(a, st) : launch_prompt<128, false>(a, st));
+  return cuda_status(f16 ? launch_prompt<256, true>(a, st) : launch_prompt<256, false>(a, st));
+}
+
+int ex_cache_write_q8(const void* key, int64_t sk_t, int64_t sk_h, const void* value, int64_t sv_t, int64_t sv_h,
+                      int dtype, int code, void* k_cache, void* v_cache, int64_t s_block, int64_t s_page, int64_t s_head,
+                      float* k_scale, float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks, int BS,
+                      const int64_t* slots, int64_t tokens, int KV, int D, void* key_out, int64_t sko_t, int64_t sko_h,
+                      void* value_out, int64_t svo_t, int64_t svo_h, void* stream) {
+  if (tokens < 0) return EX_ERR_ARG;
+  const int rc = check_cache(dtype, code, k_cache, v_cache, s_block, s_page, s_head, k_scale, v_scale, num_blocks, BS, KV, D);
+  if (rc != EX_OK || tokens == 0) return rc;
+  if (!key || !value || !slots || (!key_out) != (!value_out)) return EX_ERR_ARG;
+  for (int64_t* s : {&sk_t, &sv_t, &sko_t, &svo_t}) one_element(tokens, D, *s);
+  for (int64_t* s : {&sk_h, &sv_h, &sko_h, &svo_h}) one_element(KV, D, *s);
+  if (misaligned(key, 16) || misaligned(value, 16) || misaligned(slots, 8) || sk_t % 8 != 0 || sk_h % 8 != 0 ||
+      sv_t % 8 != 0 || sv_h % 8 != 0)
+    return EX_ERR_ALIGN;
+  if (key_out && (misaligned(key_out, 16) || misaligned(value_out, 16) || sko_t % 8 != 0 || sko_h % 8 != 0 ||
+                  svo_t % 8 != 0 || svo_h % 8 != 0))
+    return EX_ERR_ALIGN;
+  if (tokens > INT32_MAX / 4 / KV) return EX_ERR_UNSUPPORTED;
+  const ex::CacheView c = cache_view(k_cache, v_cache, s_block, s_page, s_head, k_scale, v_scale, ss_block, ss_head, num_blocks, BS);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int f16 = dtype == EX_DTYPE_F16;
+#define EX_CW(DD, CC)                                                                                              \
+  if (D == DD && code == CC)                                                                                       \
+    return cuda_status(launch_cache_write<DD, CC>(key, value, f16, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV,   \
+                                                  key_out, value_out, sko_t, sko_h, svo_t, svo_h, st));
+  EX_CW(64, ex::CODE_INT8)
+  EX_CW(128, ex::CODE_INT8)
+  EX_CW(256, ex::CODE_INT8)
+  EX_CW(64, ex::CODE_E4M3)
+  EX_CW(128, ex::CODE_E4M3)
+  EX_CW(256, ex::CODE_E4M3)
+#undef EX_CW
+  return EX_ERR_UNSUPPORTED;
+}
+
+int ex_cache_read_q8(const void* k_cache, const void* v_cache, int code, int64_t s_block, int64_t s_page, int64_t s_head,
+                     const float* k_scale, const float* v_scale, int64_t ss_block, int64_t ss_head, int64_t num_blocks,
+                     int BS, const int32_t* block_table, int64_t sbt, int width, const int32_t* cu_seqlens, int n,
+                     int64_t rows, int KV, int D, int dtype, void* key_out, int64_t sko_t, int64_t sko_h, void* value_out,
+                     int64_t svo_t, int64_t svo_h, void* stream) {
+  if (rows < 0 || n < 0 || width < 0) return EX_ERR_ARG;
+  const int rc = check_cache(dtype, code, k_cache, v_cache, s_block, s_page, s_head, k_scale, v_scale, num_blocks, BS, KV, D);
+  if (rc != EX_OK || rows == 0 || n == 0) return rc;
+  if (!block_table || !cu_seqlens || !key_out || !value_out) return EX_ERR_ARG;
+  for (int64_t* s : {&sko_t, &svo_t}) one_element(rows, D, *s);
+  for (int64_t* s : {&sko_h, &svo_h}) one_element(KV, D, *s);
+  if (misaligned(key_out, 16) || misaligned(value_out, 16) || sko_t % 8 != 0 || sko_h % 8 != 0 || svo_t % 8 != 0 || svo_h % 8 != 0)
+    return EX_ERR_ALIGN;
+  if (rows > INT32_MAX) return EX_ERR_UNSUPPORTED;
+  const ex::CacheView c = cache_view(k_cache, v_cache, s_block, s_page, s_head, k_scale, v_scale, ss_block, ss_head, num_blocks, BS);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int f16 = dtype == EX_DTYPE_F16;
+#define EX_CR(DD, CC)                                                                                                  \
+  if (D == DD && code == CC)                                                                                           \
+    return cuda_status(launch_cache_read<DD, CC>(c, block_table, sbt, width, cu_seqlens, n, rows, KV, f16, key_out,    \
+                                                 value_out, sko_t, sko_h, svo_t, svo_h, st));
+  EX_CR(64, ex::CODE_INT8)
+  EX_CR(128, ex::CODE_INT8)
+  EX_CR(256, ex::CODE_INT8)
+  EX_CR(64, ex::CODE_E4M3)
+  EX_CR(128, ex::CODE_E4M3)
+  EX_CR(256, ex::CODE_E4M3)
+#undef EX_CR
+  return EX_ERR_UNSUPPORTED;
 }
 
 }  // extern "C"

@@ -11,6 +11,7 @@ LIB_PATH = Path(os.environ.get("VLLM_EXACT_B200_LIB", Path(__file__).with_name("
 
 EX_OK, EX_ERR_ARG, EX_ERR_ALIGN, EX_ERR_WORKSPACE, EX_ERR_DTYPE, EX_ERR_UNSUPPORTED, EX_ERR_CUDA, EX_ERR_DEVICE = range(8)
 EX_DTYPE_F32, EX_DTYPE_BF16, EX_DTYPE_F16 = 0, 1, 2
+EX_CODE_NONE, EX_CODE_INT8, EX_CODE_E4M3 = -1, 0, 1
 EX_IPC_HANDLE_BYTES = 64
 EX_TP_MAX_WORLD, EX_TP_MAX_BLOCKS = 16, 256
 
@@ -57,6 +58,21 @@ SIGNATURES = {
     "ex_paged_decode_leading": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp,
                                         c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32, c_i32, c_vp, c_i64, c_i64,
                                         c_i32, c_vp, c_sz, c_vp]),
+    "ex_cache_write_q8": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                  c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_i64,
+                                  c_vp, c_i64, c_i64, c_vp]),
+    "ex_cache_read_q8": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp,
+                                 c_i64, c_i32, c_vp, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp, c_i64, c_i64, c_vp, c_i64,
+                                 c_i64, c_vp]),
+    "ex_paged_rows_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32, c_i64]),
+    "ex_paged_decode_q8": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64,
+                                   c_i64, c_i64, c_vp, c_i64, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32,
+                                   c_i64, c_vp, c_i64, c_i64, c_vp, c_sz, c_vp]),
+    "ex_tree_attention": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64,
+                                  c_i64, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_i32,
+                                  c_i32, c_i32, c_f32, c_i64, c_vp, c_i64, c_i64, c_vp, c_sz, c_vp]),
+    "ex_prompt_attention": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32,
+                                    c_i64, c_i64, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_i64, c_vp]),
 }
 
 _LIB = None

@@ -10,12 +10,16 @@ Mirrors the reference's src/vllm_exact/paged_attn.py:
 Kernel parameters are module constants that never depend on the batch (reference paged_attn.py:21-28): SPLIT keys
 per segment and the number of segments ceil(MAX_LEN / SPLIT) fix the floating-point reduction order of every
 request, so a request's output bits are the same alone, in any batch, and under any placement of its pages.
+
+Beside them, without a counterpart in the reference: ``paged_decode_q8``, the same over an 8-bit cache (kv_cache.py), and
+``tree_attention``, up to 64 drafted tokens per request over a 16-bit or 8-bit cache under an ancestor mask. Their
+segments depend on the request's own length, not on MAX_LEN, with the same invariance.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, kv_cache
 from ._lib import check, lib
 
 SPLIT = 4096       # keys per segment (fixed per deployment: it sets the reduction order)
@@ -78,6 +82,133 @@ def paged_decode(query, key_cache, value_cache, block_table, seq_lens, scale, ou
             None if query_start_loc is None else query_start_loc.data_ptr(), n, H, KV, D, BS, float(scale),
             MAX_LEN, split, out.data_ptr(), out.stride(0), out.stride(1), _DT[out.dtype], workspace.data_ptr(),
             nbytes, torch.cuda.current_stream(query.device).cuda_stream))
+    return out
+
+
+_DT16 = {torch.bfloat16: _lib.EX_DTYPE_BF16, torch.float16: _lib.EX_DTYPE_F16}
+MAX_DRAFT = 64  # drafted tokens of a request (the bits of a mask word)
+
+
+def rows_workspace_bytes(tokens: int, H: int, D: int, max_len: int) -> int:
+    """Bytes of workspace of paged_decode_q8 (tokens = n) and tree_attention for requests of at most max_len keys."""
+    return lib().ex_paged_rows_workspace_bytes(tokens, H, D, max_len)
+
+
+def _rows_operands(name, query, key_cache, value_cache, block_table, seq_lens, out, n, others):
+    """Checks shared by paged_decode_q8 and tree_attention."""
+    dev = query.device
+    if not query.is_cuda or any(t.device != dev for t in (key_cache, value_cache, block_table, seq_lens, out, *others)):
+        raise ValueError(f"{name} needs CUDA tensors of one device (there is no CPU fallback)")
+    if query.dtype not in _DT16 or out.dtype != query.dtype:
+        raise TypeError(f"{name} expects a bf16 or fp16 query, and out of the same type")
+    if query.dim() != 3 or out.dim() != 3 or key_cache.dim() != 4 or query.shape[2] != key_cache.shape[3]:
+        raise ValueError("query and out must be (tokens, H, D), caches (num_blocks, block_size, KV, D)")
+    if out.shape[0] < query.shape[0] or out.shape[1:] != query.shape[1:]:
+        raise ValueError("out must have a row for every row of query")
+    if query.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("block_table and seq_lens must be int32")
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] < n or seq_lens.shape[0] < n:
+        raise ValueError("block_table (n, pages) and seq_lens (n) need a row for every request")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block table rows must be contiguous")
+
+
+def _rows_scratch(tokens, H, D, max_len, workspace, dev):
+    nbytes = rows_workspace_bytes(tokens, H, D, max_len)
+    if nbytes and (workspace is None or workspace.numel() * workspace.element_size() < nbytes):
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    elif workspace is not None and workspace.device != dev:
+        raise ValueError("the workspace must be on the query's device")
+    return nbytes, workspace
+
+
+def paged_decode_q8(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, scale, out, n,
+                    max_seq_len=None, workspace=None):
+    """paged_decode over an 8-bit cache (kv_cache.py: codes int8 or float8_e4m3fn, one float32 scale per token and KV
+    head). query (>=n, H, D) bf16 or fp16, D = 64, 128 or 256, at most 16 query heads per KV head; block_size a multiple
+    of 8; out (>=n, H, D) in query's type. Computes the first n requests only and returns out.
+
+    max_seq_len: no request is longer (a bound for the workspace; default: what the block table holds). Tokens behind
+    it, and tokens on pages that the cache does not have, are not seen. A request of length 0 gives zeros. workspace: as
+    in paged_decode (rows_workspace_bytes), not to be shared by calls that may run at the same time."""
+    if n <= 0:
+        return out
+    if query.shape[0] < n or out.shape[0] < n:
+        raise ValueError("query and out need a row for every request")
+    _rows_operands("paged_decode_q8", query[:n], key_cache, value_cache, block_table, seq_lens, out, n, ())
+    dev = query.device
+    code = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+    seq_lens = seq_lens.contiguous()
+    H, D = query.shape[1:]
+    nb, BS, KV, _ = key_cache.shape
+    width = block_table.shape[1]
+    max_len = width * BS if max_seq_len is None else min(max(0, int(max_seq_len)), width * BS)
+    nbytes, workspace = _rows_scratch(n, H, D, max_len, workspace, dev)
+    sq, sc, ss, so = query.stride(), key_cache.stride(), key_scale.stride(), out.stride()
+    with torch.cuda.device(dev):
+        check("ex_paged_decode_q8", lib().ex_paged_decode_q8(
+            query.data_ptr(), sq[0], sq[1], _DT16[query.dtype], key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0],
+            sc[1], sc[2], key_scale.data_ptr(), value_scale.data_ptr(), ss[0], ss[1], nb, block_table.data_ptr(),
+            block_table.stride(0), width, seq_lens.data_ptr(), n, H, KV, D, BS, float(scale), max_len, out.data_ptr(),
+            so[0], so[1], workspace.data_ptr() if nbytes else None, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+    return out
+
+
+def tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, out, max_query_len,
+                   tree_mask=None, key_scale=None, value_scale=None, max_seq_len=None, workspace=None):
+    """Attention of drafted tokens over a paged cache that already holds them. query (tokens, H, D) bf16 or fp16; request
+    b has the rows query_start_loc[b] .. query_start_loc[b + 1] (int32, n + 1 entries; at most max_query_len <= 64 rows,
+    which are the last tokens of its seq_lens[b] cached ones). Every row sees its request's context (the tokens before
+    the drafted ones); of the drafted tokens row r sees number j if bit j of tree_mask[r] (int64, one word per row of
+    query) is set, its own bit included if it is to see itself. tree_mask None: a chain, each row sees the drafted tokens
+    up to itself. A row that sees nothing gives zeros.
+
+    The cache is 16-bit in query's type, any strides as in paged_decode, or 8-bit with key_scale and value_scale
+    (kv_cache.py); block_size a multiple of 8. A request with more rows than max_query_len is left untouched, as are rows
+    of out that belong to no request. max_seq_len and workspace as in paged_decode_q8. Returns out."""
+    tokens = query.shape[0]
+    n = query_start_loc.shape[0] - 1
+    if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or n < 0:
+        raise TypeError("query_start_loc must be a 1-D int32 tensor with n + 1 entries")
+    if not 1 <= max_query_len <= MAX_DRAFT:
+        raise ValueError(f"max_query_len must be 1 to {MAX_DRAFT}")
+    others = (query_start_loc,)
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 1 or tree_mask.shape[0] < tokens:
+            raise TypeError("tree_mask must be a 1-D int64 tensor with a word for every row of query")
+        tree_mask = tree_mask.contiguous()
+        others += (tree_mask,)
+    _rows_operands("tree_attention", query, key_cache, value_cache, block_table, seq_lens, out, n, others)
+    dev = query.device
+    if key_cache.dtype == query.dtype:
+        if value_cache.dtype != key_cache.dtype or key_scale is not None or value_scale is not None:
+            raise TypeError("a 16-bit cache has query's type and no scales")
+        if value_cache.shape != key_cache.shape or value_cache.stride() != key_cache.stride() or key_cache.stride(3) != 1:
+            raise ValueError("key and value caches must share shape and strides, with a contiguous head dimension")
+        code, ks, vs, ss = _lib.EX_CODE_NONE, None, None, (0, 0)
+    else:
+        if key_scale is None or value_scale is None:
+            raise TypeError("the cache must be in query's type, or 8-bit with key_scale and value_scale")
+        code = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+        ks, vs, ss = key_scale.data_ptr(), value_scale.data_ptr(), key_scale.stride()
+    if n == 0 or tokens == 0:
+        return out
+    seq_lens, query_start_loc = seq_lens.contiguous(), query_start_loc.contiguous()
+    H, D = query.shape[1:]
+    nb, BS, KV, _ = key_cache.shape
+    width = block_table.shape[1]
+    max_len = width * BS if max_seq_len is None else min(max(0, int(max_seq_len)), width * BS)
+    nbytes, workspace = _rows_scratch(tokens, H, D, max_len, workspace, dev)
+    sq, sc, so = query.stride(), key_cache.stride(), out.stride()
+    with torch.cuda.device(dev):
+        check("ex_tree_attention", lib().ex_tree_attention(
+            query.data_ptr(), sq[0], sq[1], _DT16[query.dtype], key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0],
+            sc[1], sc[2], ks, vs, ss[0], ss[1], nb, block_table.data_ptr(), block_table.stride(0), width,
+            seq_lens.data_ptr(), query_start_loc.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), n,
+            tokens, max_query_len, H, KV, D, BS, float(scale), max_len, out.data_ptr(), so[0], so[1],
+            workspace.data_ptr() if nbytes else None, nbytes, torch.cuda.current_stream(dev).cuda_stream))
     return out
 
 
