@@ -340,7 +340,7 @@ int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, co
  * key rows cu_k[b] .. cu_k[b + 1] of k and v (keys x KV x D), all bf16 or all fp16; its last query is its last key's
  * token, so query i sees keys j <= i + Lk - Lq (the keys may start before the queries: a continued conversation). A
  * query that sees no key gives zeros. Rows of no sequence are left untouched; a sequence whose offsets leave the
- * arrays is skipped. A row's bits depend on its own sequence alone.
+ * arrays is skipped. scale must be positive. A row's bits depend on its own sequence alone.
  */
 int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
                         const void* v, int64_t sv_t, int64_t sv_h, int dtype, const int32_t* cu_q, const int32_t* cu_k,

@@ -539,6 +539,32 @@ def test_prompt_attention_neighbours_that_are_not_finite(D):
     assert torch.equal(got[70:270], clean[70:270]) and bool(torch.isnan(got[:70]).all())
 
 
+@pytest.mark.parametrize("real", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_attention_hidden_values_that_are_not_finite(D, real):
+    """Infinities and NaN in a key and value reach the queries behind it and none before it, element by element."""
+    H, KV, L, before = 4, 2, 400, 70
+    g = gen(7)
+    q = torch.randn(L - before, H, D, generator=g).to(real).to(DEV)
+    k, v = (torch.randn(L, KV, D, generator=g).to(real).to(DEV) for _ in range(2))
+    clean = prompt(q, k, v, [L - before], [L], 0.1)
+    v2 = v.clone()
+    v2[100, 0, 3], v2[301, 1, D - 1], v2[301, 1, 0] = float("inf"), float("nan"), float("-inf")
+    k2 = k.clone()
+    k2[350, 0, 2] = float("nan")
+    got = prompt(q, k2, v2, [L - before], [L], 0.1)
+    i = torch.arange(before, L)
+    bad = torch.zeros(L - before, H, D, dtype=torch.bool)
+    bad[i >= 100, :2, 3] = True
+    bad[i >= 301, 2:, 0] = True
+    bad[i >= 301, 2:, D - 1] = True
+    bad[i >= 350, :2] = True
+    bad = bad.to(DEV)
+    assert torch.equal(got[~bad], clean[~bad])
+    assert not bool(torch.isfinite(got[bad]).any())
+    assert bool((got[31:280, :2, 3] == float("inf")).all()) and bool(torch.isnan(got[280:, :2]).all())
+
+
 def test_prompt_attention_graph():
     H, KV, D = 4, 2, 128
     g0 = gen(6)

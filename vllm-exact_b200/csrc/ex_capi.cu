@@ -380,13 +380,39 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   return cuda_status(e);
 }
 
+// 3-D tensor map over packed rows (D, heads, rows): boxes of 128 rows of one head, 64 dims wide.
+bool encode_packed_map(CUtensorMap* map, const void* base, int D, int heads, int64_t rows, int64_t s_h, int64_t s_t) {
+  ex::PFN_encodeTiled enc = ex::get_encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)s_h * 2, (cuuint64_t)s_t * 2};
+  cuuint32_t box[3] = {64, 1, 128};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool F16>
-cudaError_t launch_prompt(const ex::PaArgs& a, cudaStream_t st) {
-  const int smem = 3 * 64 * D * 2;
-  cudaError_t e = cudaFuncSetAttribute(ex::k_prompt_attn<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  const int64_t tiles = (a.tokens + ex::PS_ROWS - 1) / ex::PS_ROWS + a.n;  // at least as many as there are
-  return ex_launch_pdl(ex::k_prompt_attn<D, F16>, dim3((unsigned)(tiles * a.H)), dim3(128), smem, st, a);
+int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, ex::PaArgs a, cudaStream_t st) {
+  using C = ex::PaCfg<D>;
+  static int ready[128] = {};  // per device: 1 = the kernel can run as planned, -1 = it cannot
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  if (dev >= 128) return EX_ERR_UNSUPPORTED;
+  if (ready[dev] == 0) {
+    e = cudaFuncSetAttribute(ex::k_prompt_attn<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, ex::k_prompt_attn<D, F16>)) != cudaSuccess) return cuda_status(e);
+    ready[dev] = fa.numRegs == ex::PA_REGS_LAUNCH ? 1 : -1;  // the warps share out the registers of the launch
+  }
+  if (ready[dev] < 0) return EX_ERR_UNSUPPORTED;
+  a.tiles = (int)(cdiv(a.tokens, C::ROWS) + a.n);  // at least as many as there are
+  if ((int64_t)a.tiles * a.H > INT32_MAX) return EX_ERR_UNSUPPORTED;
+  return cuda_status(ex_launch_pdl(ex::k_prompt_attn<D, F16>, dim3((unsigned)(a.tiles * a.H)), dim3(ex::PA_THREADS),
+                                   C::SMEM, st, mq, mk, mv, a));
 }
 
 template <int D, int CODE>
@@ -835,17 +861,28 @@ int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k
   if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(out, 16) || sq_t % 8 != 0 ||
       sq_h % 8 != 0 || sk_t % 8 != 0 || sk_h % 8 != 0 || sv_t % 8 != 0 || sv_h % 8 != 0 || so_t % 8 != 0 || so_h % 8 != 0)
     return EX_ERR_ALIGN;
-  if ((cdiv(tokens, ex::PS_ROWS) + n) * H > INT32_MAX) return EX_ERR_UNSUPPORTED;
+  if (!(scale > 0.0f && scale < INFINITY)) return EX_ERR_ARG;
   if (!ex::device_is_sm100()) return EX_ERR_UNSUPPORTED;
+  if (keys == 0) {  // nothing to map: any rows do, none of them is read
+    k = v = q;
+    sk_t = sv_t = sq_t;
+    sk_h = sv_h = sq_h;
+    KV = H;
+  }
+  CUtensorMap mq, mk, mv;
+  if (!encode_packed_map(&mq, q, D, H, tokens, sq_h, sq_t) ||
+      !encode_packed_map(&mk, k, D, KV, keys > 0 ? keys : tokens, sk_h, sk_t) ||
+      !encode_packed_map(&mv, v, D, KV, keys > 0 ? keys : tokens, sv_h, sv_t))
+    return EX_ERR_UNSUPPORTED;
   ex::PaArgs a = {};
-  a.q = q; a.k = k; a.v = v; a.sq_t = sq_t; a.sq_h = sq_h; a.sk_t = sk_t; a.sk_h = sk_h; a.sv_t = sv_t; a.sv_h = sv_h;
+  a.v = v; a.sv_t = sv_t; a.sv_h = sv_h;
   a.cu_q = cu_q; a.cu_k = cu_k; a.n = n; a.H = H; a.G = H / KV; a.tokens = tokens; a.keys = keys;
   a.scale_log2 = scale * ex::PR_LOG2E; a.out = out; a.so_t = so_t; a.so_h = so_h;
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = dtype == EX_DTYPE_F16;
-  if (D == 64) return cuda_status(f16 ? launch_prompt<64, true>(a, st) : launch_prompt<64, false>(a, st));
-  if (D == 128) return cuda_status(f16 ? launch_prompt<128, true>(a, st) : launch_prompt<128, false>(a, st));
-  return cuda_status(f16 ? launch_prompt<256, true>(a, st) : launch_prompt<256, false>(a, st));
+  if (D == 64) return f16 ? launch_prompt<64, true>(mq, mk, mv, a, st) : launch_prompt<64, false>(mq, mk, mv, a, st);
+  if (D == 128) return f16 ? launch_prompt<128, true>(mq, mk, mv, a, st) : launch_prompt<128, false>(mq, mk, mv, a, st);
+  return f16 ? launch_prompt<256, true>(mq, mk, mv, a, st) : launch_prompt<256, false>(mq, mk, mv, a, st);
 }
 
 int ex_cache_write_q8(const void* key, int64_t sk_t, int64_t sk_h, const void* value, int64_t sv_t, int64_t sv_h,

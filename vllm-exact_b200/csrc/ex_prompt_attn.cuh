@@ -1,23 +1,114 @@
 // Causal attention of packed prompts with grouped heads: sequence b has queries cu_q[b] .. cu_q[b + 1] and keys
 // cu_k[b] .. cu_k[b + 1] of the packed arrays; its last query is its last key's token, so query i sees the keys
 // j <= i + Lk - Lq. A query that sees none (Lk < Lq) gives zeros.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - m) scale log2 e),  s_j = q . k_j
+//
+// m is a row's largest score so far, taken up only when it has grown by more than a factor 2^8 (p stays below 2^8, far
+// inside float16 and bf16, whose relative precision does not depend on it): O is rescaled a few times per row, not once
+// per block. All of it depends on the row alone.
+//
+// One CTA takes 256 queries of one head (128 where D = 256) and walks their keys in blocks of 128. tcgen05 products:
+// S = Q K^T with both operands in shared memory, O += P V with P in tensor memory, over the S it came from.
+//   warps 0-3, 4-7  softmax of query tiles 0 and 1, one row a thread; the S row is read to registers, P written back
+//   warp 8          issues the products; while one tile's softmax runs, the other tile's products do
+//   warp 9          TMA producer: Q once, then K and V of every block through one ring of slots
+//   warps 10, 11    edge blocks (those not visible to every row): values behind the sequence's end, which belong to
+//                   another sequence or to nobody, are zeroed, since 0 * NaN would reach O; values that are not finite
+//                   are zeroed and noted, and the rows that see such a key get it added at the end.
+// D = 256: one query tile and two S buffers (tensor memory holds no more), S of the next block issued before P V.
 #pragma once
 #include "ex_paged_rows.cuh"
 
 namespace ex {
 
 struct PaArgs {
-  const void *q, *k, *v;
-  int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;
+  const void* v;  // as the tensor map reads it, for values that are not finite
+  int64_t sv_t, sv_h;
   const int32_t *cu_q, *cu_k;
   int n, H, G;
   int64_t tokens, keys;  // rows of q and of k, v
+  int tiles;             // at least as many query tiles as there are
   float scale_log2;
   void* out;
   int64_t so_t, so_h;
 };
 
-constexpr int PS_ROWS = 64, PS_KEYS = 64;
+constexpr int PA_THREADS = 384;
+constexpr int PA_KEYS = 128;
+constexpr int PA_EDGES = 4;  // 256 rows reach over at most 3 blocks that are not visible to all of them
+constexpr int PA_REGS_LAUNCH = 168, PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
+static_assert(256 * PA_REGS_SOFTMAX + 128 * PA_REGS_OTHER <= PA_THREADS * PA_REGS_LAUNCH, "register shares");
+
+template <int D>
+struct PaCfg {
+  static constexpr int NQ = D == 256 ? 1 : 2;      // query tiles of 128 rows
+  static constexpr int ROWS = 128 * NQ;
+  static constexpr int SW = D < 128 ? D : 128;     // dims of a ring slot
+  static constexpr int PARTS = D / SW;             // slots of one block's K or V
+  static constexpr int SUB = 128 * 128;            // bytes of 128 rows x 64 dims, one swizzled column
+  static constexpr int SLOT = SW / 64 * SUB;
+  static constexpr int Q_BYTES = NQ * (D / 64) * SUB;
+  static constexpr int SLOTS = D == 64 ? 8 : 5;
+  static constexpr int SMEM = Q_BYTES + SLOTS * SLOT + 1024 + 512;
+  static constexpr int TM_S = 0, TM_O = 256;       // columns: two S buffers of 128, then O (NQ x D)
+};
+
+// Instruction descriptor of tcgen05.mma kind::f16 with float32 accumulation: D format in bits [4,6) (1 = f32), A and B
+// formats in [7,10) and [10,13) (0 = f16, 1 = bf16), B's major dimension in bit 16 (0 = K, 1 = N), N >> 3 in [17,23),
+// M >> 4 in [24,29).
+__host__ __device__ constexpr uint32_t make_idesc_16(int M, int N, bool f16, bool b_n_major) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+
+// Descriptor of an N-major operand in 128-byte swizzled columns of 64 elements: 8 rows of K are 1024 bytes, the next
+// 64 elements of N lie `column` bytes on.
+__device__ __forceinline__ uint64_t make_sw128_desc_n(uint32_t smem_addr, uint32_t column) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFF) | ((uint64_t)(column >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void tc_mma_16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+#define EX_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+#define EX_I8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : EX_R8(r, 0), EX_R8(r, 8), EX_R8(r, 16), EX_R8(r, 24)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::EX_I8(r, 0),
+      EX_I8(r, 8), EX_I8(r, 16), EX_I8(r, 24), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          ex_smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(ex_smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 
 // The tile'th tile of `rows` queries over all sequences: its sequence and first query in it; false if there is none.
 __device__ __forceinline__ bool pa_find_tile(const int32_t* __restrict__ cu, int n, int rows, int tile, int& b, int& row0) {
@@ -53,115 +144,398 @@ __device__ __forceinline__ void pa_sequence(const PaArgs& a, int b, int& q0, int
   Lk = k0 >= 0 && k1 <= a.keys ? (int)max((int64_t)0, k1 - k0) : 0;
 }
 
+template <bool F16>
+__device__ __forceinline__ bool finite_word(uint32_t w) {  // both halves
+  const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+  return (w & e) != e && ((w >> 16) & e) != e;
+}
+
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) k_prompt_attn(const __grid_constant__ PaArgs a) {
-  extern __shared__ __align__(1024) uint8_t ps_smem[];
+__global__ void __launch_bounds__(PA_THREADS, 1)
+    k_prompt_attn(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PaArgs a) {
+  using C = PaCfg<D>;
+  extern __shared__ uint8_t pa_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + C::Q_BYTES;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(ring + C::SLOTS * C::SLOT);
+  uint64_t* full_bar = bar;            // [8] ring slots
+  uint64_t* empty_bar = bar + 8;       // [8]
+  uint64_t* q_bar = bar + 16;
+  uint64_t* s_bar = bar + 17;          // [2] S of a tile (D = 256: of a buffer) is there
+  uint64_t* p_bar = bar + 19;          // [2] P of a tile (buffer) is there
+  uint64_t* o_bar = bar + 21;          // D = 256: P V of a block is done
+  uint64_t* end_bar = bar + 22;        // every product is done
+  uint64_t* ask_bar = bar + 23;        // [PA_EDGES] loads of an edge block's values have been issued
+  uint64_t* fix_bar = ask_bar + PA_EDGES;  // [PA_EDGES] they have been looked at
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix_bar + PA_EDGES);
+  uint32_t* poison = tmem_slot + 1;    // [16] edge keys with a value that is not finite
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int b, row0;
-  if (!pa_find_tile(a.cu_q, a.n, PS_ROWS, blockIdx.x / a.H, b, row0)) return;
+  // the last tiles have the most keys: they start first
+  if (!pa_find_tile(a.cu_q, a.n, C::ROWS, a.tiles - 1 - (int)(blockIdx.x / a.H), b, row0)) return;
   const int h = blockIdx.x % a.H, g = h / a.G;
   int q0, Lq, k0, Lk;
   pa_sequence(a, b, q0, Lq, k0, Lk);
-  const int off = Lk - Lq;  // query i sees keys j <= i + off
-  const int last = min(Lk, min(row0 + PS_ROWS, Lq) + off);  // keys that some row of the tile sees
-  const uint32_t s0 = ex_smem_u32(ps_smem);
-  constexpr int CH = D / 8;
-  auto load = [&](uint32_t dst, const uint16_t* base, int64_t st, int r0, int rmax) {
-    for (int c = tid; c < 64 * CH; c += 128) {
-      const int r = c / CH, ch = c % CH;
-      const bool ok = r0 + r < rmax;
-      cp_async16(dst + pd_swz(r, ch, D), ok ? base + (int64_t)(r0 + r) * st + ch * 8 : base, ok);
-    }
-    cp_async_commit();
-  };
-  const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)q0 * a.sq_t + (int64_t)h * a.sq_h;
-  const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k) + (int64_t)k0 * a.sk_t + (int64_t)g * a.sk_h;
-  const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)k0 * a.sv_t + (int64_t)g * a.sv_h;
-  const uint32_t sQ = s0, sK = s0 + 64 * D * 2, sV = sK + 64 * D * 2;
-  load(sQ, qp, a.sq_t, row0, Lq);
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[D / 8][4];
+  if (row0 >= Lq) return;
+  const int off = Lk - Lq;  // row i sees the keys j <= i + off
+  int nblk[2];              // blocks of each tile
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  for (int kb = 0; kb < last; kb += PS_KEYS) {
-    __syncthreads();
-    load(sK, kp, a.sk_t, kb, Lk);
-    load(sV, vp, a.sv_t, kb, Lk);
-    cp_async_wait<0>();
-    __syncthreads();
-    float sc[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < D / 16; ++kt) {
-      uint32_t af[4];
-      ldsm_x4(sQ + pd_swz(warp * 16 + (lane & 15), kt * 2 + (lane >> 4), D), af);
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        uint32_t bf[4];
-        ldsm_x4(sK + pd_swz(j * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1), D), bf);
-        mma_16816<F16>(sc[j], af, bf[0], bf[1]);
-        mma_16816<F16>(sc[j + 1], af, bf[2], bf[3]);
-      }
-    }
-    uint32_t pa[8][2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {  // rows lane/4 and lane/4 + 8
-      const int row = row0 + warp * 16 + (lane >> 2) + 8 * e;
-      float mx = m[e];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const int key = kb + j * 8 + (lane & 3) * 2 + f;
-          float& x = sc[j][2 * e + f];
-          x = key < Lk && key <= row + off ? x * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, x);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float sub = mx == -INFINITY ? 0.0f : mx;
-      const float al = ex2(m[e] - sub);
-      m[e] = mx;
-      l[e] *= al;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float p0 = ex2(sc[j][2 * e] - sub), p1 = ex2(sc[j][2 * e + 1] - sub);
-        l[e] += p0 + p1;
-        pa[j][e] = F16 ? pack2<__half>(p0, p1) : pack_bf16(p0, p1);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][2 * e] *= al;
-        o[i][2 * e + 1] *= al;
-      }
-    }
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      const uint32_t af[4] = {pa[2 * kt][0], pa[2 * kt][1], pa[2 * kt + 1][0], pa[2 * kt + 1][1]};
-#pragma unroll
-      for (int i = 0; i < D / 8; i += 2) {
-        uint32_t bf[4];
-        ldsm_x4_t(sV + pd_swz(kt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), i + (lane >> 4), D), bf);
-        mma_16816<F16>(o[i], af, bf[0], bf[1]);
-        mma_16816<F16>(o[i + 1], af, bf[2], bf[3]);
-      }
-    }
+  for (int i = 0; i < 2; ++i) {
+    const int first = row0 + 128 * i, last = min(first + 127, Lq - 1);
+    nblk[i] = (i < C::NQ && first < Lq) ? max(0, (min(Lk, last + off + 1) + PA_KEYS - 1) / PA_KEYS) : 0;
   }
-  cp_async_wait<0>();
+  const int nmax = max(nblk[0], nblk[1]);
+  const int edge = max(0, min(Lk, row0 + off + 1)) / PA_KEYS;  // blocks before it are seen by every row
+
+  if (tid == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(full_bar + i, 1);
+      mbar_init(empty_bar + i, 1);
+    }
+    mbar_init(q_bar, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_bar + i, 1);
+      mbar_init(p_bar + i, 128);
+    }
+    mbar_init(o_bar, 1);
+    mbar_init(end_bar, 1);
+    for (int i = 0; i < PA_EDGES; ++i) {
+      mbar_init(ask_bar + i, 1);
+      mbar_init(fix_bar + i, 64);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = 0; i < 16; ++i) poison[i] = 0;
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
+    if (warp == 9) {
+      // -------------------------------------------------------------------------------------------- TMA producer
+      if (lane == 0 && nmax > 0) {
+        mbar_arrive_expect_tx(q_bar, C::Q_BYTES);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    const int row = row0 + warp * 16 + (lane >> 2) + 8 * e;
-    if (row >= Lq) continue;
-    const float inv = l[e] > 0.0f ? 1.0f / l[e] : (l[e] == 0.0f ? 0.0f : l[e]);
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(q0 + row) * a.so_t + (int64_t)h * a.so_h + (lane & 3) * 2;
+        for (int i = 0; i < C::NQ * (D / 64); ++i)
+          tma_load_3d(smem + i * C::SUB, &tm_q, q_bar, (i % (D / 64)) * 64, h, q0 + row0 + (i / (D / 64)) * 128);
+        int slot = 0, made = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        auto load = [&](const CUtensorMap* m, int j) {
+          for (int p = 0; p < C::PARTS && ok; ++p) {
+            ok = mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
+            if (!ok) return;
+            mbar_arrive_expect_tx(full_bar + slot, C::SLOT);
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-      *reinterpret_cast<uint32_t*>(dst + i * 8) = F16 ? pack2<__half>(o[i][2 * e] * inv, o[i][2 * e + 1] * inv)
-                                                     : pack_bf16(o[i][2 * e] * inv, o[i][2 * e + 1] * inv);
+            for (int s = 0; s < C::SW / 64; ++s)
+              tma_load_3d(ring + slot * C::SLOT + s * C::SUB, m, full_bar + slot, p * C::SW + s * 64, g, k0 + j * PA_KEYS);
+            ++made;
+            if (++slot == C::SLOTS) slot = 0, ph ^= 1;
+          }
+        };
+        // in the order of use: S of a block is issued one block ahead of P V
+        load(&tm_k, 0);
+        if (C::NQ == 1 && nmax > 1) load(&tm_k, 1);
+        for (int j = 0; j < nmax && ok; ++j) {
+          load(&tm_v, j);
+          if (j >= edge && ok) mbar_arrive(ask_bar + (j - edge));
+          const int k = j + (C::NQ == 1 ? 2 : 1);
+          if (k < nmax) load(&tm_k, k);
+        }
+        mbar_wait(q_bar, 0, EX_DEVERR_WAIT_TMA);  // every load has landed before the CTA ends
+        for (int i = max(0, made - C::SLOTS); i < made; ++i)
+          mbar_wait(full_bar + i % C::SLOTS, (uint32_t)(i / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
+      }
+    } else if (warp == 8) {
+      // -------------------------------------------------------------------------------------------- products
+      if (lane == 0 && nmax > 0) {
+        constexpr uint32_t id_s = make_idesc_16(128, 128, F16, false), id_o = make_idesc_16(128, C::SW, F16, true);
+        const uint32_t sq = ex_smem_u32(smem), sr = ex_smem_u32(ring);
+        int slot = 0;  // next slot to be used
+        uint32_t ph = 0;
+        bool ok = mbar_wait(q_bar, 0, EX_DEVERR_WAIT_TMA);
+        auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1; };
+        auto full = [&]() { if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA); };
+        // S (buffer) = Q (tile) K^T over the dims of one slot
+        auto issue_s = [&](int tile, int buf, int part) {
+#pragma unroll
+          for (int s = 0; s < C::SW / 64; ++s) {
+            const uint64_t da = make_sw128_desc(sq + (tile * (D / 64) + part * (C::SW / 64) + s) * C::SUB);
+            const uint64_t db = make_sw128_desc(sr + slot * C::SLOT + s * C::SUB);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_16(tmem + C::TM_S + buf * 128, da + 2 * k, db + 2 * k, id_s, (part | s | k) != 0);
+          }
+        };
+        auto issue_o = [&](int tile, int buf, int part, int j) {
+          const uint64_t db = make_sw128_desc_n(sr + slot * C::SLOT, C::SUB);
+#pragma unroll
+          for (int k = 0; k < PA_KEYS / 16; ++k)
+            tc_mma_16_ta(tmem + C::TM_O + tile * D + part * C::SW, tmem + C::TM_S + buf * 128 + k * 8, db + k * (2048 >> 4),
+                         id_o, (j | k) != 0);
+        };
+        if constexpr (C::NQ == 2) {
+          full();
+          tc_fence_after();
+          for (int i = 0; i < 2 && ok; ++i)
+            if (nblk[i] > 0) {
+              issue_s(i, i, 0);
+              tc_commit(s_bar + i);
+            }
+          if (ok) tc_commit(empty_bar + slot);
+          advance();
+          for (int j = 0; j < nmax && ok; ++j) {
+            const int vslot = slot;
+            bool have_v = false, have_k = false;
+            for (int i = 0; i < 2 && ok; ++i) {
+              if (j >= nblk[i]) continue;
+              if (!have_v) {
+                full();
+                if (ok && j >= edge) ok = mbar_wait(fix_bar + (j - edge), 0, EX_DEVERR_WAIT_MMA);
+                have_v = true;
+              }
+              if (ok) ok = mbar_wait(p_bar + i, (uint32_t)j & 1u, EX_DEVERR_WAIT_TMEM);
+              if (!ok) break;
+              tc_fence_after();
+              issue_o(i, i, 0, j);
+              if (j + 1 < nblk[i]) {
+                advance();  // to K of the next block
+                if (!have_k) full();
+                have_k = true;
+                if (ok) {
+                  tc_fence_after();
+                  issue_s(i, i, 0);
+                  tc_commit(s_bar + i);
+                }
+                if (--slot < 0) slot = C::SLOTS - 1, ph ^= 1;  // back to V
+              }
+            }
+            if (!ok) break;
+            tc_commit(empty_bar + vslot);
+            advance();
+            if (j + 1 < nmax) {
+              tc_commit(empty_bar + slot);
+              advance();
+            }
+          }
+        } else {
+          auto s_of = [&](int j) {
+            for (int p = 0; p < C::PARTS && ok; ++p) {
+              full();
+              if (!ok) return;
+              tc_fence_after();
+              issue_s(0, j & 1, p);
+              tc_commit(empty_bar + slot);
+              advance();
+            }
+            if (ok) tc_commit(s_bar + (j & 1));
+          };
+          s_of(0);
+          if (nmax > 1) s_of(1);
+          for (int j = 0; j < nmax && ok; ++j) {
+            if (ok && j >= edge) ok = mbar_wait(fix_bar + (j - edge), 0, EX_DEVERR_WAIT_MMA);
+            if (ok) ok = mbar_wait(p_bar + (j & 1), (uint32_t)(j >> 1) & 1u, EX_DEVERR_WAIT_TMEM);
+            for (int p = 0; p < C::PARTS && ok; ++p) {
+              full();
+              if (!ok) break;
+              tc_fence_after();
+              issue_o(0, j & 1, p, j);
+              tc_commit(empty_bar + slot);
+              advance();
+            }
+            if (ok) tc_commit(o_bar);
+            if (j + 2 < nmax && ok) s_of(j + 2);
+          }
+        }
+        tc_commit(end_bar);
+        mbar_wait(end_bar, 0, EX_DEVERR_WAIT_MMA);
+      }
+    } else {
+      // -------------------------------------------------------------------------------------------- edge values
+      const int t = tid - 320;  // 64 threads
+      bool ok = true;
+      for (int j = edge; j < nmax && ok; ++j) {
+        // the producer may be any number of blocks behind: its word that the slots are this block's comes first
+        ok = mbar_wait(ask_bar + (j - edge), 0, EX_DEVERR_WAIT_SLOT);
+        for (int p = 0; p < C::PARTS && ok; ++p) {
+          // number of the slot in the order of loading: K of min(j + 2, nmax) or j + 1 blocks and V of j came before
+          const int at = C::NQ == 1 ? (min(j + 2, nmax) + j) * C::PARTS + p : 2 * j + 1;
+          uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
+          ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
+          for (int r = t; r < PA_KEYS && ok; r += 64) {
+            const int key = j * PA_KEYS + r;
+            bool bad = false;
+            for (int c = 0; c < C::SW / 8; ++c) {
+              uint4* x = reinterpret_cast<uint4*>(vs + (c >> 3) * C::SUB + r * 128 + (c & 7) * 16);
+              if (key >= Lk) {
+                *x = make_uint4(0, 0, 0, 0);
+              } else {
+                uint4 w = *x;
+                if (!(finite_word<F16>(w.x) && finite_word<F16>(w.y) && finite_word<F16>(w.z) && finite_word<F16>(w.w))) {
+                  bad = true;
+                  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
+                    if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
+                  }
+                  *x = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+              }
+            }
+            const int k = key - edge * PA_KEYS;
+            if (bad && k < 512) atomicOr(poison + (k >> 5), 1u << (k & 31));
+          }
+        }
+        fence_proxy_async_shared();  // the products read shared memory through the async proxy
+        if (ok) mbar_arrive(fix_bar + (j - edge));
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
+    const int tile = warp >> 2;
+    const int nb = nblk[tile & 1];
+    const int row = row0 + tile * 128 + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + lanes + C::TM_O + tile * D;
+    const float sc = a.scale_log2;
+    const float grow = 8.0f / sc;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      const int buf = C::NQ == 2 ? tile : (j & 1);
+      const uint32_t s_addr = tmem + lanes + C::TM_S + buf * 128;
+      ok = mbar_wait(s_bar + buf, (uint32_t)(C::NQ == 2 ? j : j >> 1) & 1u, EX_DEVERR_WAIT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+      tmem_ld_wait();
+      if (j >= edge) {
+        const int limit = min(Lk - 1, row + off) - j * PA_KEYS;  // columns behind it are not seen
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+      const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool take = mb > m + grow || m == -INFINITY;
+      if (j == 0) {
+        m = mb;
+      } else if (__any_sync(0xffffffffu, take)) {
+        // the next product on O waits for P, the last one is done: it was issued before this S (D = 256: after it)
+        if (C::NQ == 1) {
+          ok = mbar_wait(o_bar, (uint32_t)(j - 1) & 1u, EX_DEVERR_WAIT_MMA);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        const float mn = take ? fmaxf(m, mb) : m;
+        const float al = m == -INFINITY ? (mn == -INFINITY ? 1.0f : 0.0f) : ex2((m - mn) * sc);
+        m = mn;
+        l *= al;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+          tmem_st32(o_addr + c, o);
+        }
+      }
+      const float sub = m == -INFINITY ? 0.0f : m * sc;
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float x = ex2(__fmaf_rn(s[c * 64 + 2 * i], sc, -sub)), y = ex2(__fmaf_rn(s[c * 64 + 2 * i + 1], sc, -sub));
+          sum[0] += x;
+          sum[1] += y;
+          p[i] = F16 ? pack2<__half>(x, y) : pack_bf16(x, y);
+        }
+        tmem_st32(s_addr + c * 32, p);
+      }
+      l += sum[0] + sum[1];
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_bar + buf);
+    }
+    if (tile < C::NQ) {
+      if (nmax > 0) {
+        if (ok) ok = mbar_wait(end_bar, 0, EX_DEVERR_WAIT_MMA);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (ok) {
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // nothing seen: zeros; NaN stays NaN
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(q0 + row) * a.so_t + (int64_t)h * a.so_h;
+        bool any = false;
+        for (int i = 0; i < 16; ++i) any |= poison[i] != 0;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          if (nb > 0) {
+            tmem_ld32(o_addr + c, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
+            const int seen = min(Lk, row + off + 1);
+#pragma unroll 1
+            for (int key = edge * PA_KEYS; key < seen; ++key) {
+              const int k = key - edge * PA_KEYS;
+              if (k >= 512 || !((poison[k >> 5] >> (k & 31)) & 1u)) continue;
+              const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)(k0 + key) * a.sv_t + (int64_t)g * a.sv_h + c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float x = F16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
+                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+              }
+            }
+          }
+          if (row < Lq) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
+                w[k] = F16 ? pack2<__half>(x, y) : pack_bf16(x, y);
+              }
+              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
