@@ -277,28 +277,50 @@ bool misaligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t
 bool half_dtype(int d) { return d == EX_DTYPE_BF16 || d == EX_DTYPE_F16; }
 bool head_size_ok(int D) { return D == 64 || D == 128 || D == 256; }
 
-template <int D, int CODE, bool F16, int NT>
-cudaError_t launch_rows_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
-                          cudaStream_t st) {
-  using C = ex::PrCfg<D, CODE, NT>;
-  static bool done[128] = {};  // the attribute is per device and kernel
+// One launch of a kernel that takes dynamic shared memory, the attribute set once per device.
+template <typename K, typename... Args>
+cudaError_t launch_smem(K kernel, bool (&done)[128], int grid, int threads, int smem, cudaStream_t st, const Args&... args) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 128 || !done[dev]) {
-    e = cudaFuncSetAttribute(ex::k_paged_rows<D, CODE, F16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev < 128) done[dev] = true;
   }
-  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
-  return ex_launch_pdl(ex::k_paged_rows<D, CODE, F16, NT>, dim3(grid), dim3(ex::PR_THREADS), C::SMEM, st, mk, mv, a);
+  return ex_launch_pdl(kernel, dim3(grid), dim3(threads), smem, st, args...);
 }
 
+template <int D, int CODE, bool F16, int NT>
+cudaError_t launch_rows_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
+                          cudaStream_t st) {
+  using C = ex::PrCfg<D, CODE, NT>;
+  static bool done[128] = {};
+  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
+  return launch_smem(ex::k_paged_rows<D, CODE, F16, NT>, done, grid, ex::PR_THREADS, C::SMEM, st, mk, mv, a);
+}
+
+template <int D, int CODE, bool F16, int NT>
+cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
+                         cudaStream_t st) {
+  using C = ex::PfCfg<D, CODE, NT>;
+  static bool done[128] = {};
+  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
+  return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, done, grid, ex::PR_THREADS, C::SMEM, st, mk, mv, a);
+}
+
+// Requests of at most 16 rows a KV head go to k_paged_few, the others to k_paged_rows: by their own number of rows, so
+// that a request's bits do not depend on the longest one of the batch.
 template <int D, int CODE, bool F16>
-cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t per_tile,
+cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, ex::PrArgs a, int64_t per_tile,
                            cudaStream_t st) {
-  if (rows <= 8) return launch_rows_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
-  if (rows <= 16) return launch_rows_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
+  a.rows_lo = 0;
+  a.rows_hi = 16;
+  if (rows <= 8) return launch_few_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
+  cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
+  if (rows <= 16 || e != cudaSuccess) return e;
+  a.rows_lo = 16;
+  a.rows_hi = INT32_MAX;
   if (rows <= 32 || D == 256) return launch_rows_t<D, CODE, F16, 4>(mk, mv, a, per_tile * cdiv(rows, 32), st);
   if constexpr (D != 256) return launch_rows_t<D, CODE, F16, 8>(mk, mv, a, per_tile * cdiv(rows, 64), st);
   return cudaErrorInvalidValue;

@@ -80,6 +80,7 @@ struct PrArgs {
   const float* v_scale;
   int64_t ss_block, ss_head;
   int NS;
+  int rows_lo, rows_hi;      // requests with rows_lo < T G <= rows_hi are this kernel's
   float* ws_m;
   float* ws_l;
   float* ws_acc;
@@ -113,7 +114,8 @@ struct PrWalk {
       const int r = base + lane;
       if (r < a.n) {
         pr_request(a, r, first, T, L);
-        if (T > 0) cnt = pr_segments(pr_keys(a, L)) * a.KV * ((T * a.G + rows_per_tile - 1) / rows_per_tile);
+        if (T > 0 && T * a.G > a.rows_lo && T * a.G <= a.rows_hi)
+          cnt = pr_segments(pr_keys(a, L)) * a.KV * ((T * a.G + rows_per_tile - 1) / rows_per_tile);
       }
       incl = cnt;
 #pragma unroll
@@ -188,6 +190,92 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 #define PR_BAR() asm volatile("bar.sync 1, 128;" ::: "memory")
 
+// The producer warp: every block of the CTA's items through the ring, running ahead of the consumers.
+template <int D, int CODE, int NT, int STAGES>
+__device__ __forceinline__ void pr_produce(const PrArgs& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* smem,
+                                           uint64_t* full_bar, uint64_t* empty_bar, uint32_t* sgood) {
+  using C = PrCfg<D, CODE, NT>;
+  constexpr bool Q8 = CODE != CODE_NONE;
+  const int lane = threadIdx.x & 31;
+  PrWalk walk;
+  uint32_t blkno = 0;
+  const int group = 1 << a.group_log2, per = PR_BLK >> a.group_log2;  // at most 8 groups a block
+  bool ok = true;
+  for (int it = blockIdx.x; ok; it += gridDim.x) {
+    int b, first, T, L, rem;
+    if (!walk.find(a, 8 * NT, it, b, first, T, L, rem)) break;
+    const int tiles = (T * a.G + 8 * NT - 1) / (8 * NT);
+    const int g = (rem / tiles) % a.KV, s = rem / (tiles * a.KV);
+    const int keys = pr_keys(a, L), seg = pr_segment(keys);
+    const int start = s * seg, end = min(keys, start + seg);
+    const int32_t* btr = a.bt + (int64_t)b * a.sbt;
+    for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
+      const int st = blkno % STAGES;
+      if (lane == 0) ok = mbar_wait(empty_bar + st, ((blkno / STAGES) & 1u) ^ 1u, EX_DEVERR_WAIT_SLOT);
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (!ok) break;
+      const int key0 = kb + lane * group;
+      int page = -1, off = 0;
+      if (lane < per && key0 < end) {
+        page = btr[key0 / a.BS];
+        off = key0 % a.BS;
+      }
+      const unsigned good = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
+      uint8_t* ks = smem + st * C::STAGE;
+      if (lane == 0) {
+        sgood[st] = good;
+        mbar_arrive_expect_tx(full_bar + st, (uint32_t)(__popc(good) * group * (2 * C::ROW + (Q8 ? 8 : 0))));
+      }
+      __syncwarp();
+      if ((good >> lane) & 1) {
+        uint8_t* vs = ks + C::TILE;
+#pragma unroll
+        for (int h = 0; h < C::NH; ++h) {
+          tma_load_4d(ks + h * C::HALF + lane * group * C::PITCH, tm_k, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
+          tma_load_4d(vs + h * C::HALF + lane * group * C::PITCH, tm_v, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
+        }
+        if constexpr (Q8) {
+          float* ss = reinterpret_cast<float*>(ks + 2 * C::TILE);
+          const int64_t so = (int64_t)page * a.ss_block + g * a.ss_head + off;
+          bulk_load(ss + lane * group, a.k_scale + so, (uint32_t)group * 4, full_bar + st);
+          bulk_load(ss + PR_BLK + lane * group, a.v_scale + so, (uint32_t)group * 4, full_bar + st);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  // every load has landed before the CTA ends (also after a wait that ran out)
+  if (lane == 0) {
+    for (uint32_t i = blkno > (uint32_t)STAGES ? blkno - STAGES : 0; i < blkno; ++i)
+      mbar_wait(full_bar + i % STAGES, (i / STAGES) & 1u, EX_DEVERR_WAIT_TMA);
+  }
+  __syncwarp();
+}
+
+// 1 / f and f = 2^e with m in [f, 2f): what a row with largest element m is divided by on its way to float16. Exponents
+// are kept where both are normal numbers.
+__device__ __forceinline__ float pr_query_scale(float m, float& f) {
+  int e = (int)((__float_as_uint(m) >> 23) & 255u);
+  e = e == 255 ? 127 : min(max(e, 2), 252);
+  f = __uint_as_float((uint32_t)e << 23);
+  return __uint_as_float((uint32_t)(254 - e) << 23);
+}
+
+// a word of the transposing load: dims 2x, 2x + 1 of two keys, as the two keys' dim 2x and their dim 2x + 1
+template <int CODE>
+__device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
+  if constexpr (CODE == CODE_E4M3) {
+    codes_to_f16<CODE>(__byte_perm(w, 0, 0x3120), even, odd);
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    even = __byte_perm(u, 0x64646464u, 0x4240);
+    odd = __byte_perm(u, 0x64646464u, 0x4341);
+    const __half2 off = __half2half2(__ushort_as_half(0xe480));  // -1152
+    *reinterpret_cast<__half2*>(&even) = __hadd2(*reinterpret_cast<__half2*>(&even), off);
+    *reinterpret_cast<__half2*>(&odd) = __hadd2(*reinterpret_cast<__half2*>(&odd), off);
+  }
+}
+
 template <int D, int CODE, bool F16, int NT>
 __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
     k_paged_rows(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -222,63 +310,12 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
   __syncthreads();
   pdl_wait();
 
-  PrWalk walk;
-  uint32_t blkno = 0;  // blocks through the ring so far
   if (warp == 4) {
-    // ------------------------------------------------------------------------------------------------ producer
-    const int group = 1 << a.group_log2, per = PR_BLK >> a.group_log2;  // at most 8 groups a block
-    bool ok = true;
-    for (int it = blockIdx.x; ok; it += gridDim.x) {
-      int b, first, T, L, rem;
-      if (!walk.find(a, ROWS, it, b, first, T, L, rem)) break;
-      const int tiles = (T * a.G + ROWS - 1) / ROWS;
-      const int g = (rem / tiles) % a.KV, s = rem / (tiles * a.KV);
-      const int keys = pr_keys(a, L), seg = pr_segment(keys);
-      const int start = s * seg, end = min(keys, start + seg);
-      const int32_t* btr = a.bt + (int64_t)b * a.sbt;
-      for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
-        const int st = blkno % C::STAGES;
-        if (lane == 0) ok = mbar_wait(empty_bar + st, ((blkno / C::STAGES) & 1u) ^ 1u, EX_DEVERR_WAIT_SLOT);
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok) break;
-        const int key0 = kb + lane * group;
-        int page = -1, off = 0;
-        if (lane < per && key0 < end) {
-          page = btr[key0 / a.BS];
-          off = key0 % a.BS;
-        }
-        const unsigned good = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
-        uint8_t* ks = smem + st * C::STAGE;
-        if (lane == 0) {
-          sgood[st] = good;
-          mbar_arrive_expect_tx(full_bar + st, (uint32_t)(__popc(good) * group * (2 * C::ROW + (Q8 ? 8 : 0))));
-        }
-        __syncwarp();
-        if ((good >> lane) & 1) {
-          uint8_t* vs = ks + C::TILE;
-#pragma unroll
-          for (int h = 0; h < C::NH; ++h) {
-            tma_load_4d(ks + h * C::HALF + lane * group * C::PITCH, &tm_k, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
-            tma_load_4d(vs + h * C::HALF + lane * group * C::PITCH, &tm_v, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
-          }
-          if constexpr (Q8) {
-            float* ss = reinterpret_cast<float*>(ks + 2 * C::TILE);
-            const int64_t so = (int64_t)page * a.ss_block + g * a.ss_head + off;
-            bulk_load(ss + lane * group, a.k_scale + so, (uint32_t)group * 4, full_bar + st);
-            bulk_load(ss + PR_BLK + lane * group, a.v_scale + so, (uint32_t)group * 4, full_bar + st);
-          }
-        }
-        __syncwarp();
-      }
-    }
-    // every load has landed before the CTA ends (also after a wait that ran out)
-    if (lane == 0) {
-      for (uint32_t i = blkno > (uint32_t)C::STAGES ? blkno - C::STAGES : 0; i < blkno; ++i)
-        mbar_wait(full_bar + i % C::STAGES, (i / C::STAGES) & 1u, EX_DEVERR_WAIT_TMA);
-    }
-    __syncwarp();
+    pr_produce<D, CODE, NT, C::STAGES>(a, &tm_k, &tm_v, smem, full_bar, empty_bar, sgood);
     return;
   }
+  PrWalk walk;
+  uint32_t blkno = 0;  // blocks through the ring so far
   // -------------------------------------------------------------------------------------------------- consumers
   const int qr = lane >> 2, qc = (lane & 3) * 2;
   const uint32_t sq0 = ex_smem_u32(sq), sp0 = ex_smem_u32(sp);
@@ -321,11 +358,7 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
             for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
 #pragma unroll
             for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            // f = 2^e with the row's largest element in [f, 2f); exponents are kept where both f and 1/f are normal
-            int e = (int)((__float_as_uint(m) >> 23) & 255u);
-            e = e == 255 ? 127 : min(max(e, 2), 252);
-            f = __uint_as_float((uint32_t)e << 23);
-            const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+            const float inv = pr_query_scale(m, f);
             v.x = pack2<__half>(x[0] * inv, x[1] * inv);
             v.y = pack2<__half>(x[2] * inv, x[3] * inv);
             v.z = pack2<__half>(x[4] * inv, x[5] * inv);
@@ -594,8 +627,8 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
             uint32_t w0, w1;
             const uint32_t ad = vs0 + pr_at<C::PITCH, C::HALF>(kt * 16 + (mi & 1) * 8 + (lane & 7), warp);
             asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w0), "=r"(w1) : "r"(ad));
-            codes_to_f16<CODE>(__byte_perm(w0, 0, 0x3120), va[0][0], va[0][1]);
-            codes_to_f16<CODE>(__byte_perm(w1, 0, 0x3120), va[0][2], va[0][3]);
+            transposed_to_f16<CODE>(w0, va[0][0], va[0][1]);
+            transposed_to_f16<CODE>(w1, va[0][2], va[0][3]);
           } else {
 #pragma unroll
             for (int i = 0; i < MT; i += 2) {
@@ -603,8 +636,8 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
               ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(kt * 16 + (mi & 1) * 8 + (lane & 7), warp * MT + i + (mi >> 1)), w);
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                codes_to_f16<CODE>(__byte_perm(w[2 * u], 0, 0x3120), va[i + u][0], va[i + u][1]);
-                codes_to_f16<CODE>(__byte_perm(w[2 * u + 1], 0, 0x3120), va[i + u][2], va[i + u][3]);
+                transposed_to_f16<CODE>(w[2 * u], va[i + u][0], va[i + u][1]);
+                transposed_to_f16<CODE>(w[2 * u + 1], va[i + u][2], va[i + u][3]);
               }
             }
           }
@@ -693,6 +726,451 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
         }
       }
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// At most 16 rows of a KV head: a decode step, or a few drafted tokens.
+//
+// Every warp is on its own: warp w of 4 takes the keys 16w .. 16w + 15 of each block with its own m, l and O (all of D), so
+// nothing waits inside the key loop but for data. m is taken up only when a score passes it by more than 6 (a factor of 64;
+// p stays small enough for float16), and the reference of the value scales when one is 64 times it: the common path
+// has two votes and no shuffles. Both are decided for every row alone. The warps are added up in order at the end.
+// ------------------------------------------------------------------------------------------------------------------
+template <int D, int CODE, int NT>
+struct PfCfg {
+  using R = PrCfg<D, CODE, NT>;
+  static constexpr int MERGE = 2 * 8 * NT * D * 4;     // two buffers of O
+  static constexpr int FIXED = MERGE + 4 * 8 * NT * 8 + 1024 + 512;
+  static constexpr int PER_SM = D == 256 && (NT == 2 || CODE == CODE_NONE) ? 1 : (NT == 2 || D == 256 || CODE == CODE_NONE) ? 2 : 3;
+  static constexpr int ROOM = 226 * 1024 / PER_SM - 1024 - FIXED;
+  static constexpr int STAGES = ROOM / R::STAGE < 8 ? ROOM / R::STAGE : 8;
+  static constexpr int SMEM = FIXED + STAGES * R::STAGE;
+  static constexpr bool Q_REGS = D * NT <= 256;        // query fragments in registers, else read again for every block
+  static_assert(STAGES >= 2, "ring");
+};
+
+template <int D, int CODE, bool F16, int NT>
+__global__ void __launch_bounds__(PR_THREADS, PfCfg<D, CODE, NT>::PER_SM)
+    k_paged_few(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                const __grid_constant__ PrArgs a) {
+  using C = PrCfg<D, CODE, NT>;
+  using F = PfCfg<D, CODE, NT>;
+  constexpr bool Q8 = CODE != CODE_NONE;
+  constexpr bool MF16 = Q8 || F16;
+  constexpr int ROWS = 8 * NT;
+  constexpr int KT = D / 16;
+  extern __shared__ uint8_t pr_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
+  float* so = reinterpret_cast<float*>(smem + F::STAGES * C::STAGE);  // [2][ROWS][D]
+  float* sm = so + 2 * ROWS * D;                                      // [4][ROWS]
+  float* sl = sm + 4 * ROWS;                                          // [4][ROWS]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sl + 4 * ROWS);
+  uint64_t* empty_bar = full_bar + 8;
+  uint32_t* sgood = reinterpret_cast<uint32_t*>(empty_bar + 8);
+  volatile int* sfail = reinterpret_cast<int*>(sgood + 8);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+  if (tid == 0) {
+    *sfail = 0;
+    for (int i = 0; i < F::STAGES; ++i) {
+      mbar_init(full_bar + i, 1);
+      mbar_init(empty_bar + i, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_wait();
+  if (warp == 4) {
+    pr_produce<D, CODE, NT, F::STAGES>(a, &tm_k, &tm_v, smem, full_bar, empty_bar, sgood);
+    return;
+  }
+  PrWalk walk;
+  uint32_t blkno = 0;
+  const int qr = lane >> 2, qc = (lane & 3) * 2;
+  const int per = PR_BLK >> a.group_log2;
+  bool alive = true;
+  for (int it = blockIdx.x; alive; it += gridDim.x) {
+    int b, first, T, L, rem;
+    if (!walk.find(a, ROWS, it, b, first, T, L, rem)) break;
+    const int R = T * a.G;  // one tile: at most ROWS
+    const int g = rem % a.KV, s = rem / a.KV;
+    const int keys = pr_keys(a, L), seg = pr_segment(keys);
+    const int start = s * seg, end = min(keys, start + seg);
+    const int ctx = L - T;
+
+    // query fragments of the MMA's second operand: row qr of each 8, dims 16 kt + 2 (lane % 4) + {0, 1, 8, 9} for a 16-bit
+    // cache; for codes the four dims 16 kt + 4 (lane % 4) .., since a word of four codes takes those slots
+    uint32_t qf[NT][KT][2];
+    float qs[NT];  // what a row was divided by
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int r = j * 8 + qr;
+      const bool have = r < R;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + (have ? r / a.G : 0)) * a.sq_t +
+                           (int64_t)(g * a.G + (have ? r % a.G : 0)) * a.sq_h;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        if constexpr (Q8) {
+          const uint2 v = *reinterpret_cast<const uint2*>(qp + kt * 16 + 2 * qc);
+          qf[j][kt][0] = have ? v.x : 0u;
+          qf[j][kt][1] = have ? v.y : 0u;
+        } else {
+          const uint32_t v0 = *reinterpret_cast<const uint32_t*>(qp + kt * 16 + qc);
+          const uint32_t v1 = *reinterpret_cast<const uint32_t*>(qp + kt * 16 + qc + 8);
+          qf[j][kt][0] = have ? v0 : 0u;
+          qf[j][kt][1] = have ? v1 : 0u;
+        }
+      }
+      qs[j] = 1.0f;
+      if (Q8 && !a.q_is_f16) {
+        float m = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x, y;
+            unpack2<__nv_bfloat16>(qf[j][kt][i], x, y);
+            m = fmaxf(m, fmaxf(fabsf(x), fabsf(y)));
+          }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float inv = pr_query_scale(m, qs[j]);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x, y;
+            unpack2<__nv_bfloat16>(qf[j][kt][i], x, y);
+            qf[j][kt][i] = pack2<__half>(x * inv, y * inv);
+          }
+      }
+    }
+    float fac[2 * NT];  // score factors of columns qc, qc + 1 of each 8
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i)
+      fac[i] = Q8 ? __shfl_sync(0xffffffffu, qs[i >> 1], (qc + (i & 1)) * 4) * a.scale_log2 : a.scale_log2;
+
+    float m[2 * NT], l[2 * NT], o[KT][NT][4];
+    float vref = 0.0f, vinv = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+
+    for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
+      const int st = blkno % F::STAGES;
+      if (!mbar_wait(full_bar + st, (blkno / F::STAGES) & 1u, EX_DEVERR_WAIT_TMA)) {
+        *sfail = 1;
+        break;
+      }
+      uint8_t* ks = smem + st * C::STAGE;
+      uint8_t* vs = ks + C::TILE;
+      const uint32_t ks0 = ex_smem_u32(ks), vs0 = ex_smem_u32(vs);
+      const int k0 = warp * 16;  // this warp's keys of the block
+      const uint32_t good = sgood[st];
+      const bool whole = kb + PR_BLK <= min(end, ctx) && good == (1u << per) - 1u;
+      if (kb + k0 < end) {
+        float sc[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; kt += (Q8 ? 2 : 1)) {
+          uint32_t af[2][4];
+          if constexpr (Q8) {
+            uint32_t w[4];
+            ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, kt + (lane >> 4)), w);
+            codes_to_f16<CODE>(w[0], af[0][0], af[0][2]);
+            codes_to_f16<CODE>(w[1], af[0][1], af[0][3]);
+            codes_to_f16<CODE>(w[2], af[1][0], af[1][2]);
+            codes_to_f16<CODE>(w[3], af[1][1], af[1][3]);
+          } else {
+            ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(k0 + (lane & 15), kt * 2 + (lane >> 4)), af[0]);
+          }
+#pragma unroll
+          for (int u = 0; u < (Q8 ? 2 : 1); ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_16816<MF16>(sc[j], af[u], qf[j][kt + u][0], qf[j][kt + u][1]);
+        }
+        float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
+        if constexpr (Q8) {
+          const float* kscale = reinterpret_cast<const float*>(ks + 2 * C::TILE) + k0 + qr;
+          ksc[0] = kscale[0];
+          ksc[1] = kscale[8];
+          vsc[0] = kscale[PR_BLK];
+          vsc[1] = kscale[PR_BLK + 8];
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] *= Q8 ? fac[2 * j + (e & 1)] * ksc[e >> 1] : fac[2 * j + (e & 1)];
+        bool slow = false;  // 16-bit: a value that is not finite and that some row may not see
+        uint32_t bits = 0xffffffffu;
+        if (!whole) {
+          bits = 0;
+          const int kk = k0 + qr;
+          bool readable[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            readable[e] = kb + kk + 8 * e < end && ((good >> ((kk + 8 * e) >> a.group_log2)) & 1u);
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i) {
+            const int r = (i >> 1) * 8 + qc + (i & 1);
+            const int t = r / a.G;
+            uint64_t w = 0;
+            if (r < R) w = a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = kb + kk + 8 * e - ctx;
+              if (r < R && readable[e] && (d < 0 || ((w >> d) & 1ull))) bits |= 1u << (2 * i + e);
+            }
+          }
+          if constexpr (Q8) {
+            if (!readable[0]) vsc[0] = 0.0f;
+            if (!readable[1]) vsc[1] = 0.0f;
+          }
+          int bad = 0;
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {
+            const bool none = kb + k0 + i >= end || !((good >> ((k0 + i) >> a.group_log2)) & 1u);
+            for (int c = lane; c < C::ROW / 16; c += 32) {
+              uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(k0 + i, c));
+              if (none) {
+                *x = make_uint4(0, 0, 0, 0);  // values that may not be read: 0 * NaN would reach O
+              } else if constexpr (!Q8) {
+                const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+                const uint32_t w[4] = {x->x, x->y, x->z, x->w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
+              }
+            }
+          }
+          fence_proxy_async_shared();  // the ring slot is written by TMA next
+          if constexpr (!Q8) slow = __any_sync(0xffffffffu, bad);
+          else __syncwarp();
+        }
+        // references: taken up for the rows that need it
+        float top[2 * NT];
+        bool need = false;
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+          float& s0 = sc[i >> 1][i & 1];
+          float& s1 = sc[i >> 1][2 + (i & 1)];
+          if (!((bits >> (2 * i)) & 1u)) s0 = -INFINITY;
+          if (!((bits >> (2 * i + 1)) & 1u)) s1 = -INFINITY;
+          top[i] = fmaxf(s0, s1);
+          need |= top[i] > m[i] + 6.0f;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i) {
+            float v = top[i];
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            if (v > m[i] + 6.0f) {  // (for m = -inf as well)
+              const float al = ex2(m[i] - v);
+              m[i] = v;
+              l[i] *= al;
+#pragma unroll
+              for (int mt = 0; mt < KT; ++mt) {
+                o[mt][i >> 1][i & 1] *= al;
+                o[mt][i >> 1][2 + (i & 1)] *= al;
+              }
+            }
+          }
+        }
+        if constexpr (Q8) {
+          const float v0 = vsc[0] < INFINITY ? vsc[0] : 0.0f, v1 = vsc[1] < INFINITY ? vsc[1] : 0.0f;  // (NaN: 0)
+          float v = fmaxf(v0, v1);
+          if (__any_sync(0xffffffffu, v > 64.0f * vref)) {
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            const bool tiny = v < 1.2e-38f;  // such values are zero next to any output type's smallest step
+            const float be = tiny ? 1.0f : __fdividef(vref, v);
+            vinv = tiny ? 0.0f : __frcp_rn(v);
+            vref = v;
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][j][e] *= be;
+          }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 2 * j + (e & 1);
+            p[e] = ex2(sc[j][e] - (m[i] == -INFINITY ? 0.0f : m[i]));
+          }
+          l[2 * j] += p[0] + p[2];
+          l[2 * j + 1] += p[1] + p[3];
+          if constexpr (Q8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // a key that is not seen has a scale that may be anything
+              p[e] *= vsc[e >> 1] * vinv;
+              if (!((bits >> (2 * (2 * j + (e & 1)) + (e >> 1))) & 1u)) p[e] = 0.0f;
+            }
+          }
+          pb[j][0] = movmatrix_t(MF16 ? pack2<__half>(p[0], p[1]) : pack_bf16(p[0], p[1]));
+          pb[j][1] = movmatrix_t(MF16 ? pack2<__half>(p[2], p[3]) : pack_bf16(p[2], p[3]));
+        }
+        const int mi = lane >> 3;
+        if (!Q8 && slow) {
+          // one product at a time: a weight of 0 leaves a value out that is not finite
+#pragma unroll 1
+          for (int kk = 0; kk < 16; ++kk) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                // weight of (row 8 j + qc + e, key kk): in pb[j][kk / 8] of lane (qc + e) * 4 + (kk % 8) / 2
+                const uint32_t w = __shfl_sync(0xffffffffu, kk < 8 ? pb[j][0] : pb[j][1], (qc + e) * 4 + ((kk & 7) >> 1));
+                const uint32_t w16 = (kk & 1) ? w >> 16 : w & 0xffffu;
+                const float p = F16 ? __half2float(__ushort_as_half((uint16_t)w16)) : __uint_as_float(w16 << 16);
+#pragma unroll
+                for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+                  for (int u = 0; u < 2; ++u) {
+                    const int d = mt * 16 + qr + 8 * u;
+                    const uint16_t vr = *reinterpret_cast<const uint16_t*>(vs + pr_at<C::PITCH, C::HALF>(k0 + kk, d >> 3) + (d & 7) * 2);
+                    const float v = F16 ? __half2float(__ushort_as_half(vr)) : __uint_as_float((uint32_t)vr << 16);
+                    if (p != 0.0f) o[mt][j][2 * u + e] += p * v;
+                  }
+              }
+          }
+        } else {
+#pragma unroll
+          for (int mt = 0; mt < KT; mt += (Q8 ? 2 : 1)) {
+            uint32_t va[2][4];
+            if constexpr (Q8) {
+              uint32_t w[4];  // keys 0-7 | 8-15 of a 16-byte chunk (16 dims), then of the next
+              ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(k0 + (mi & 1) * 8 + (lane & 7), mt + (mi >> 1)), w);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                transposed_to_f16<CODE>(w[2 * u], va[u][0], va[u][1]);
+                transposed_to_f16<CODE>(w[2 * u + 1], va[u][2], va[u][3]);
+              }
+            } else {
+              ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(k0 + (mi >> 1) * 8 + (lane & 7), mt * 2 + (mi & 1)), va[0]);
+            }
+#pragma unroll
+            for (int u = 0; u < (Q8 ? 2 : 1); ++u)
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma_16816<MF16>(o[mt + u][j], va[u], pb[j][0], pb[j][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar + st);
+    }
+
+    // the four warps, in order: all brought to the largest m, then added up
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      float v = l[i];
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      l[i] = v;
+      if (qr == 0) {
+        sm[warp * ROWS + (i >> 1) * 8 + qc + (i & 1)] = m[i];
+        sl[warp * ROWS + (i >> 1) * 8 + qc + (i & 1)] = v;
+      }
+    }
+    PR_BAR();
+    if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
+    float mall[2 * NT], lall[2 * NT];
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int c = (i >> 1) * 8 + qc + (i & 1);
+      float v = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v = fmaxf(v, sm[w * ROWS + c]);
+      mall[i] = v;
+      const float sub = v == -INFINITY ? 0.0f : v;
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) t += sl[w * ROWS + c] * ex2(sm[w * ROWS + c] - sub);
+      lall[i] = t;
+      const float f = ex2(m[i] - sub) * (Q8 ? vref : 1.0f);
+      const float keep = m[i] == -INFINITY ? 0.0f : f;
+#pragma unroll
+      for (int mt = 0; mt < KT; ++mt) {
+        o[mt][i >> 1][i & 1] *= keep;
+        o[mt][i >> 1][2 + (i & 1)] *= keep;
+      }
+    }
+    float* mine = so + (warp & 1) * ROWS * D;
+#pragma unroll
+    for (int phase = 0; phase < 2; ++phase) {
+      if ((warp >> 1) == phase) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+          const int c = (i >> 1) * 8 + qc + (i & 1);
+          if (c < R) {
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt) {
+              // codes: dims 2 qr, 2 qr + 1 of the 16; 16-bit: qr, qr + 8
+              float* x = mine + c * D + mt * 16 + (Q8 ? 2 * qr : qr);
+              const float u = o[mt][i >> 1][i & 1], v = o[mt][i >> 1][2 + (i & 1)];
+              if (phase == 0) {
+                x[0] = u;
+                x[Q8 ? 1 : 8] = v;
+              } else {
+                x[0] += u;
+                x[Q8 ? 1 : 8] += v;
+              }
+            }
+          }
+        }
+      }
+      PR_BAR();
+    }
+    const bool single = pr_segments(keys) == 1;
+    if (warp == 0 && qr == 0) {  // one thread per column
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i) {
+        const int c = (i >> 1) * 8 + qc + (i & 1);
+        sl[c] = lall[i];  // (every warp has read sm and sl: two barriers ago)
+        if (!single && c < R) {
+          const int64_t pi = ((int64_t)(first + c / a.G) * a.H + g * a.G + c % a.G) * a.NS + s;
+          a.ws_m[pi] = mall[i];
+          a.ws_l[pi] = lall[i];
+        }
+      }
+    }
+    PR_BAR();
+    for (int x = tid; x < R * (D / 4); x += 128) {
+      const int c = x / (D / 4), d = (x % (D / 4)) * 4;
+      const float4 u = *reinterpret_cast<const float4*>(so + c * D + d);
+      const float4 v = *reinterpret_cast<const float4*>(so + (ROWS + c) * D + d);
+      const float4 w = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+      const int t = c / a.G, h = g * a.G + c % a.G;
+      if (single) {
+        const float lx = sl[c];
+        const float inv = lx > 0.0f ? 1.0f / lx : (lx == 0.0f ? 0.0f : lx);  // nothing seen: zeros; NaN stays NaN
+        uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t +
+                                                    (int64_t)h * a.so_h + d);
+        const bool f16 = Q8 ? a.q_is_f16 != 0 : F16;
+        dst[0] = f16 ? pack2<__half>(w.x * inv, w.y * inv) : pack_bf16(w.x * inv, w.y * inv);
+        dst[1] = f16 ? pack2<__half>(w.z * inv, w.w * inv) : pack_bf16(w.z * inv, w.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(a.ws_acc + (((int64_t)(first + t) * a.H + h) * a.NS + s) * D + d) = w;
+      }
+    }
+    PR_BAR();  // before the buffers are written again
   }
 }
 
