@@ -305,8 +305,8 @@ cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex:
                          cudaStream_t st) {
   using C = ex::PfCfg<D, CODE, NT>;
   static bool done[128] = {};
-  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
-  return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, done, grid, ex::PR_THREADS, C::SMEM, st, mk, mv, a);
+  const int grid = (int)std::min<int64_t>(items, num_sms());
+  return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, done, grid, 32 * C::NW, C::SMEM, st, mk, mv, a);
 }
 
 // Requests of at most 16 rows a KV head go to k_paged_few, the others to k_paged_rows: by their own number of rows, so
@@ -335,7 +335,7 @@ cudaError_t launch_rows_d(int code, int q_dtype, int rows, const CUtensorMap& mk
   else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, a, per_tile, st);
   else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, a, per_tile, st);
   if (e != cudaSuccess || a.NS == 1) return e;
-  const dim3 grid((unsigned)cdiv(a.tokens * a.H, 8)), block(256);
+  const dim3 grid((unsigned)cdiv(a.tokens * a.H * (D / 64), 4)), block(128);
   if (q_dtype == EX_DTYPE_F16) return ex_launch_pdl(ex::k_paged_rows_merge<D, true>, grid, block, 0, st, a);
   return ex_launch_pdl(ex::k_paged_rows_merge<D, false>, grid, block, 0, st, a);
 }

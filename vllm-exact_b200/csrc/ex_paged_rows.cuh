@@ -23,6 +23,19 @@
 #include "ex_paged_decode.cuh"
 #include "ex_paged_decode_tma.cuh"
 
+#ifndef XSEG_A
+#define XSEG_A 256
+#define XSEG_B 512
+#endif
+#ifndef XNW
+#define XNW ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 12 : (CODE == CODE_NONE ? 2 : 1) * D <= 256 ? 8 : 4)
+#endif
+#ifndef XMK
+#define XMK ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 2 : 1)
+#endif
+#ifndef XPER
+#define XPER (D == 256 && (NT == 2 || CODE == CODE_NONE) ? 1 : 2)
+#endif
 namespace ex {
 
 constexpr int PR_THREADS = 160;
@@ -31,7 +44,7 @@ constexpr int PR_MAX_TOKENS = 64;  // drafted tokens of a request (bits of a mas
 constexpr float PR_LOG2E = 1.4426950408889634f;
 
 // Keys a segment, by the request's own length.
-__host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? 256 : 1024; }
+__host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? XSEG_A : XSEG_B; }
 __host__ __device__ inline int pr_segments(int64_t L) {
   const int s = pr_segment(L);
   const int n = (int)((L + s - 1) / s);
@@ -43,15 +56,15 @@ __host__ inline int pr_max_segments(int64_t max_len) {
   return a > b ? a : b;
 }
 
-template <int D, int CODE, int NT>
+template <int D, int CODE, int NT, int BLK = PR_BLK>
 struct PrCfg {
   static constexpr int ESZ = CODE == CODE_NONE ? 2 : 1;
   static constexpr int ROW = D * ESZ;                       // bytes of a key
   static constexpr int PITCH = ROW < 128 ? ROW : 128;       // bytes of a row of a TMA box
   static constexpr int NH = ROW / PITCH;                    // boxes across the head dimension
-  static constexpr int HALF = PR_BLK * PITCH;
-  static constexpr int TILE = PR_BLK * ROW;                 // K or V of a block
-  static constexpr int STAGE = 2 * TILE + (CODE == CODE_NONE ? 0 : 1024);  // + scales of 64 keys and 64 values, padded
+  static constexpr int HALF = BLK * PITCH;
+  static constexpr int TILE = BLK * ROW;                 // K or V of a block
+  static constexpr int STAGE = 2 * TILE + (CODE == CODE_NONE ? 0 : 1024);  // + scales of the keys and of the values, padded
   static constexpr int Q_BYTES = 8 * NT * D * 2;
   static constexpr int P_BYTES = 8 * NT * 128;
   static constexpr int MISC = 4 * 8 * NT * 4 /* maxima */ + 8 * NT * 4 /* row factors or sums */ + 512;
@@ -182,66 +195,101 @@ __device__ __forceinline__ uint32_t pr_at(int row, int chunk) {
   }
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ex_smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(ex_smem_u32(bar))
-      : "memory");
-}
 #define PR_BAR() asm volatile("bar.sync 1, 128;" ::: "memory")
 
 // The producer warp: every block of the CTA's items through the ring, running ahead of the consumers.
-template <int D, int CODE, int NT, int STAGES>
+template <int D, int CODE, int NT, int STAGES, int BLK = PR_BLK>
 __device__ __forceinline__ void pr_produce(const PrArgs& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* smem,
                                            uint64_t* full_bar, uint64_t* empty_bar, uint32_t* sgood) {
-  using C = PrCfg<D, CODE, NT>;
+  using C = PrCfg<D, CODE, NT, BLK>;
   constexpr bool Q8 = CODE != CODE_NONE;
   const int lane = threadIdx.x & 31;
   PrWalk walk;
   uint32_t blkno = 0;
-  const int group = 1 << a.group_log2, per = PR_BLK >> a.group_log2;  // at most 8 groups a block
-  bool ok = true;
-  for (int it = blockIdx.x; ok; it += gridDim.x) {
+  const int group = 1 << a.group_log2, per = BLK >> a.group_log2;  // at most 16 groups a block
+  // an item's keys and, a window of 32 groups at a time, where they lie: lane l holds the page of group l (-1: none)
+  int it = blockIdx.x, g = 0, start = 0, end = 0;
+  const int32_t* btr = a.bt;
+  auto next_item = [&]() {
     int b, first, T, L, rem;
-    if (!walk.find(a, 8 * NT, it, b, first, T, L, rem)) break;
+    if (!walk.find(a, 8 * NT, it, b, first, T, L, rem)) return false;
+    it += gridDim.x;
     const int tiles = (T * a.G + 8 * NT - 1) / (8 * NT);
-    const int g = (rem / tiles) % a.KV, s = rem / (tiles * a.KV);
     const int keys = pr_keys(a, L), seg = pr_segment(keys);
-    const int start = s * seg, end = min(keys, start + seg);
-    const int32_t* btr = a.bt + (int64_t)b * a.sbt;
-    for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
-      const int st = blkno % STAGES;
-      if (lane == 0) ok = mbar_wait(empty_bar + st, ((blkno / STAGES) & 1u) ^ 1u, EX_DEVERR_WAIT_SLOT);
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (!ok) break;
-      const int key0 = kb + lane * group;
-      int page = -1, off = 0;
-      if (lane < per && key0 < end) {
-        page = btr[key0 / a.BS];
-        off = key0 % a.BS;
+    g = (rem / tiles) % a.KV;
+    start = rem / (tiles * a.KV) * seg;
+    end = min(keys, start + seg);
+    btr = a.bt + (int64_t)b * a.sbt;
+    return true;
+  };
+  auto window = [&](int key, int last, int& page, int& off) {
+    const int key0 = key + lane * group;
+    page = -1;
+    if (key0 < last) {
+      page = btr[key0 / a.BS];
+      off = key0 % a.BS;
+    }
+  };
+  bool ok = true, have = next_item();
+  int page = -1, off = 0;
+  if (have) window(start, end, page, off);
+  while (have && ok) {
+    const int cg = g, cend = end;
+    int wkey = start;
+    bool more = true;
+    // the window after this one is looked up while this one is loaded: of this item, or the first of the next
+    while (more && ok) {
+      const int after = wkey + 32 * group;
+      int npage = -1, noff = 0;
+      more = after < cend;
+      if (more) {
+        window(after, cend, npage, noff);
+      } else {
+        have = next_item();
+        if (have) window(start, end, npage, noff);
       }
-      const unsigned good = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
-      uint8_t* ks = smem + st * C::STAGE;
-      if (lane == 0) {
-        sgood[st] = good;
-        mbar_arrive_expect_tx(full_bar + st, (uint32_t)(__popc(good) * group * (2 * C::ROW + (Q8 ? 8 : 0))));
-      }
-      __syncwarp();
-      if ((good >> lane) & 1) {
-        uint8_t* vs = ks + C::TILE;
+      const unsigned goods = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
+      for (int base = 0; base < 32; base += per) {
+        if (wkey + base * group >= cend) break;
+        const int st = blkno % STAGES;
+        ok = mbar_wait(empty_bar + st, ((blkno / STAGES) & 1u) ^ 1u, EX_DEVERR_WAIT_SLOT);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const unsigned good = (goods >> base) & ((1u << per) - 1u);
+        if (lane == 0) {
+          sgood[st] = good;
+          mbar_arrive_expect_tx(full_bar + st, (uint32_t)(__popc(good) * group * (2 * C::ROW)));
+        }
+        __syncwarp();
+        const int sub = lane - base;
+        if (sub >= 0 && sub < per && ((good >> sub) & 1u)) {
+          uint8_t* ks = smem + st * C::STAGE;
+          uint8_t* vs = ks + C::TILE;
 #pragma unroll
-        for (int h = 0; h < C::NH; ++h) {
-          tma_load_4d(ks + h * C::HALF + lane * group * C::PITCH, tm_k, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
-          tma_load_4d(vs + h * C::HALF + lane * group * C::PITCH, tm_v, full_bar + st, h * (C::PITCH / C::ESZ), g, off, page);
+          for (int h = 0; h < C::NH; ++h) {
+            tma_load_4d(ks + h * C::HALF + sub * group * C::PITCH, tm_k, full_bar + st, h * (C::PITCH / C::ESZ), cg, off, page);
+            tma_load_4d(vs + h * C::HALF + sub * group * C::PITCH, tm_v, full_bar + st, h * (C::PITCH / C::ESZ), cg, off, page);
+          }
         }
         if constexpr (Q8) {
-          float* ss = reinterpret_cast<float*>(ks + 2 * C::TILE);
-          const int64_t so = (int64_t)page * a.ss_block + g * a.ss_head + off;
-          bulk_load(ss + lane * group, a.k_scale + so, (uint32_t)group * 4, full_bar + st);
-          bulk_load(ss + PR_BLK + lane * group, a.v_scale + so, (uint32_t)group * 4, full_bar + st);
+          // scales: 16 bytes of four tokens a lane. Not by bulk copies: as many of them as of the codes' boxes, 64 bytes
+          // each, would take as much of the TMA unit as the codes.
+          const int from = min(base + ((lane * 4) >> a.group_log2), 31);
+          const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
+          if (lane < BLK / 4 && ((goods >> from) & 1u)) {
+            float* ss = reinterpret_cast<float*>(smem + st * C::STAGE + 2 * C::TILE) + lane * 4;
+            const int64_t so = (int64_t)pg * a.ss_block + cg * a.ss_head + po + ((lane * 4) & (group - 1));
+            cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
+            cp_async16(ex_smem_u32(ss + BLK), a.v_scale + so, true);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(full_bar + st)) : "memory");
         }
+        __syncwarp();
+        ++blkno;
       }
-      __syncwarp();
+      wkey = after;
+      page = npage;
+      off = noff;
     }
   }
   // every load has landed before the CTA ends (also after a wait that ran out)
@@ -286,7 +334,7 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
   constexpr int ROWS = 8 * NT;
   constexpr int MT = D / 64;        // 16-dim tiles of a warp's quarter
   extern __shared__ uint8_t pr_smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = pr_smem_raw + ((0u - ex_smem_u32(pr_smem_raw)) & 1023u);
   uint8_t* sq = smem + C::STAGES * C::STAGE;
   uint8_t* sp = sq + C::Q_BYTES;
   float* smax = reinterpret_cast<float*>(sp + C::P_BYTES);  // [4][ROWS]
@@ -302,7 +350,7 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
   if (tid == 0) {
     *sfail = 0;
     for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(full_bar + i, 1);
+      mbar_init(full_bar + i, Q8 ? 33 : 1);  // codes: and every producer lane's copies of scales
       mbar_init(empty_bar + i, 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -732,66 +780,135 @@ __global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
 // ------------------------------------------------------------------------------------------------------------------
 // At most 16 rows of a KV head: a decode step, or a few drafted tokens.
 //
-// Every warp is on its own: warp w of 4 takes the keys 16w .. 16w + 15 of each block with its own m, l and O (all of D), so
-// nothing waits inside the key loop but for data. m is taken up only when a score passes it by more than 6 (a factor of 64;
-// p stays small enough for float16), and the reference of the value scales when one is 64 times it: the common path
-// has two votes and no shuffles. Both are decided for every row alone. The warps are added up in order at the end.
+// Every warp streams its own items: it loads blocks of 16 MK keys into its own ring, S blocks ahead and on into its next
+// item, and computes S^T = K Q^T, P and O^T += V^T P^T on what has arrived. No thread waits for another warp. m is taken up
+// only when a score passes it by more than 6 (a factor of 64; p stays small enough for float16), and the reference of
+// the value scales when one is 64 times it: the common path has two votes and no shuffles. Both are decided for
+// every row (every key) alone.
 // ------------------------------------------------------------------------------------------------------------------
 template <int D, int CODE, int NT>
 struct PfCfg {
-  using R = PrCfg<D, CODE, NT>;
-  static constexpr int MERGE = 2 * 8 * NT * D * 4;     // two buffers of O
-  static constexpr int FIXED = MERGE + 4 * 8 * NT * 8 + 1024 + 512;
-  static constexpr int PER_SM = D == 256 && (NT == 2 || CODE == CODE_NONE) ? 1 : (NT == 2 || D == 256 || CODE == CODE_NONE) ? 2 : 3;
-  static constexpr int ROOM = 226 * 1024 / PER_SM - 1024 - FIXED;
-  static constexpr int STAGES = ROOM / R::STAGE < 8 ? ROOM / R::STAGE : 8;
-  static constexpr int SMEM = FIXED + STAGES * R::STAGE;
-  static constexpr bool Q_REGS = D * NT <= 256;        // query fragments in registers, else read again for every block
+  static constexpr int MK = XMK;                       // 16-key tiles of a block
+  static constexpr int NW = XNW;                       // warps of a CTA, one CTA per SM
+  static constexpr int BLK = 16 * MK;
+  using R = PrCfg<D, CODE, NT, BLK>;
+  static constexpr int STAGE = 2 * R::TILE;
+  static constexpr int SCALES = CODE == CODE_NONE ? 0 : 8 * BLK;  // bytes of a block's scales, keys' first
+  static constexpr int ROOM = (225 * 1024) / NW;
+  static constexpr int STAGES = ROOM / (STAGE + SCALES) < 8 ? ROOM / (STAGE + SCALES) : 8;
+  static constexpr int SMEM = NW * STAGES * (STAGE + SCALES) + 1024 + NW * 8 * (8 + 4);
   static_assert(STAGES >= 2, "ring");
 };
 
 template <int D, int CODE, bool F16, int NT>
-__global__ void __launch_bounds__(PR_THREADS, PfCfg<D, CODE, NT>::PER_SM)
+__global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
     k_paged_few(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                 const __grid_constant__ PrArgs a) {
-  using C = PrCfg<D, CODE, NT>;
   using F = PfCfg<D, CODE, NT>;
+  using C = typename F::R;
+  constexpr int MK = F::MK, BLK = F::BLK, NW = F::NW, STAGES = F::STAGES;
   constexpr bool Q8 = CODE != CODE_NONE;
   constexpr bool MF16 = Q8 || F16;
   constexpr int ROWS = 8 * NT;
   constexpr int KT = D / 16;
   extern __shared__ uint8_t pr_smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
-  float* so = reinterpret_cast<float*>(smem + F::STAGES * C::STAGE);  // [2][ROWS][D]
-  float* sm = so + 2 * ROWS * D;                                      // [4][ROWS]
-  float* sl = sm + 4 * ROWS;                                          // [4][ROWS]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sl + 4 * ROWS);
-  uint64_t* empty_bar = full_bar + 8;
-  uint32_t* sgood = reinterpret_cast<uint32_t*>(empty_bar + 8);
-  volatile int* sfail = reinterpret_cast<int*>(sgood + 8);
-
+  uint8_t* smem = pr_smem_raw + ((0u - ex_smem_u32(pr_smem_raw)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = smem + warp * STAGES * F::STAGE;
+  uint8_t* behind = smem + NW * STAGES * F::STAGE;
+  float* scales = reinterpret_cast<float*>(behind + warp * STAGES * F::SCALES);
+  behind += NW * STAGES * F::SCALES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(behind) + warp * 8;
+  uint32_t* sgood = reinterpret_cast<uint32_t*>(behind + NW * 64) + warp * 8;  // groups whose page exists
+
   pdl_launch_dependents();
-  if (tid == 0) {
-    *sfail = 0;
-    for (int i = 0; i < F::STAGES; ++i) {
-      mbar_init(full_bar + i, 1);
-      mbar_init(empty_bar + i, 4);
-    }
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(full_bar + i, Q8 ? 33 : 1);  // codes: and every lane's copies of scales
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
+  __syncwarp();
   pdl_wait();
-  if (warp == 4) {
-    pr_produce<D, CODE, NT, F::STAGES>(a, &tm_k, &tm_v, smem, full_bar, empty_bar, sgood);
-    return;
-  }
+
+  const int stride = gridDim.x * NW;
+  const int glog = a.group_log2, group = 1 << glog, per = BLK >> glog;  // groups of a block
+  // ---- what is loaded next: an item's keys and, for groups lane and lane + 32 of it, where they lie
+  PrWalk lwalk;
+  int lit = warp * gridDim.x + blockIdx.x, lg = 0, lkey = 0, lend = 0, lgi = 0, page[2] = {-1, -1}, off[2] = {0, 0};
+  bool lhave = true;
+  int lslot = 0;
+  auto load_item = [&]() {  // the next item that has keys
+    do {
+      int b, first, T, L, rem;
+      lhave = lwalk.find(a, ROWS, lit, b, first, T, L, rem);
+      if (!lhave) return;
+      lit += stride;
+      const int keys = pr_keys(a, L), seg = pr_segment(keys);
+      lg = rem % a.KV;
+      lkey = rem / a.KV * seg;
+      lend = min(keys, lkey + seg);
+      lgi = 0;
+      const int32_t* btr = a.bt + (int64_t)b * a.sbt;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = lkey + (lane + 32 * i) * group;
+        page[i] = -1;
+        if (key < lend) {
+          page[i] = btr[key / a.BS];
+          off[i] = key % a.BS;
+        }
+      }
+    } while (lkey >= lend);
+  };
+  auto load_block = [&]() {
+    if (!lhave) return;
+    const int pg = lgi < 32 ? page[0] : page[1], po = lgi < 32 ? off[0] : off[1];
+    const unsigned goods = __ballot_sync(0xffffffffu, pg >= 0 && pg < a.blocks);
+    const int base = lgi & 31;
+    const unsigned good = (goods >> base) & ((1u << per) - 1u);
+    uint8_t* ks = ring + lslot * F::STAGE;
+    uint64_t* bar = full_bar + lslot;
+    if (lane == 0) {
+      sgood[lslot] = good;
+      mbar_arrive_expect_tx(bar, (uint32_t)(__popc(good) * group * 2 * C::ROW));
+    }
+    __syncwarp();
+    const int sub = lane - base;
+    if (sub >= 0 && sub < per && ((good >> sub) & 1u)) {
+#pragma unroll
+      for (int h = 0; h < C::NH; ++h) {
+        tma_load_4d(ks + h * C::HALF + sub * group * C::PITCH, &tm_k, bar, h * (C::PITCH / C::ESZ), lg, po, pg);
+        tma_load_4d(ks + C::TILE + h * C::HALF + sub * group * C::PITCH, &tm_v, bar, h * (C::PITCH / C::ESZ), lg, po, pg);
+      }
+    }
+    if constexpr (Q8) {
+      // scales: 16 bytes of four tokens a lane. Not by bulk copies: as many of them as of the codes' boxes would take as
+      // much of the TMA unit as the codes.
+      const int tok = (lane * 4) & (BLK - 1);
+      const int from = base + (tok >> glog);
+      const int p2 = __shfl_sync(0xffffffffu, pg, from), o2 = __shfl_sync(0xffffffffu, po, from);
+      if (lane < BLK / 2 && ((goods >> from) & 1u)) {
+        float* ss = scales + lslot * 2 * BLK + lane * 4;
+        const float* src = lane < BLK / 4 ? a.k_scale : a.v_scale;
+        cp_async16(ex_smem_u32(ss), src + (int64_t)p2 * a.ss_block + lg * a.ss_head + o2 + (tok & (group - 1)), true);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(bar)) : "memory");
+    }
+    if (++lslot == STAGES) lslot = 0;
+    lkey += BLK;
+    lgi += per;
+    if (lkey >= lend) load_item();
+  };
+  load_item();
+#pragma unroll 1
+  for (int i = 0; i < STAGES; ++i) load_block();
+
+  // ---- what is computed
   PrWalk walk;
-  uint32_t blkno = 0;
+  int st = 0;  // ring slot of the next block and its phase
+  uint32_t phase = 0;
   const int qr = lane >> 2, qc = (lane & 3) * 2;
-  const int per = PR_BLK >> a.group_log2;
-  bool alive = true;
-  for (int it = blockIdx.x; alive; it += gridDim.x) {
+  bool ok = true;
+  for (int it = warp * gridDim.x + blockIdx.x; ok; it += stride) {
     int b, first, T, L, rem;
     if (!walk.find(a, ROWS, it, b, first, T, L, rem)) break;
     const int R = T * a.G;  // one tile: at most ROWS
@@ -864,324 +981,308 @@ __global__ void __launch_bounds__(PR_THREADS, PfCfg<D, CODE, NT>::PER_SM)
 #pragma unroll
       for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
 
-    for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
-      const int st = blkno % F::STAGES;
-      if (!mbar_wait(full_bar + st, (blkno / F::STAGES) & 1u, EX_DEVERR_WAIT_TMA)) {
-        *sfail = 1;
-        break;
-      }
-      uint8_t* ks = smem + st * C::STAGE;
+    for (int kb = start; kb < end; kb += BLK) {
+      ok = mbar_wait(full_bar + st, phase, EX_DEVERR_WAIT_TMA);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* ks = ring + st * F::STAGE;
       uint8_t* vs = ks + C::TILE;
-      const uint32_t ks0 = ex_smem_u32(ks), vs0 = ex_smem_u32(vs);
-      const int k0 = warp * 16;  // this warp's keys of the block
+      const float* kscale = scales + st * 2 * BLK + qr;  // then those of the values
       const uint32_t good = sgood[st];
-      const bool whole = kb + PR_BLK <= min(end, ctx) && good == (1u << per) - 1u;
-      if (kb + k0 < end) {
-        float sc[NT][4];
+      const bool whole = kb + BLK <= min(end, ctx) && good == (1u << per) - 1u;
+      // S^T, 16 keys a tile: a column's chunk c of the tile's rows lies at (base ^ (c % 8) * 16) + c / 8 * HALF for even c
+      float sc[MK][NT][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+      for (int i = 0; i < MK; ++i)
 #pragma unroll
-        for (int kt = 0; kt < KT; kt += (Q8 ? 2 : 1)) {
+        for (int j = 0; j < NT; ++j) sc[i][j][0] = sc[i][j][1] = sc[i][j][2] = sc[i][j][3] = 0.0f;
+      uint32_t kbase[MK];
+#pragma unroll
+      for (int i = 0; i < MK; ++i)
+        kbase[i] = ex_smem_u32(ks) +
+                   (Q8 ? pr_at<C::PITCH, C::HALF>(16 * i + (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4)
+                       : pr_at<C::PITCH, C::HALF>(16 * i + (lane & 15), lane >> 4));
+#pragma unroll
+      for (int kt = 0; kt < KT; kt += (Q8 ? 2 : 1)) {
+        const int c = Q8 ? kt : 2 * kt;
+#pragma unroll
+        for (int i = 0; i < MK; ++i) {
           uint32_t af[2][4];
+          uint32_t w[4];
+          ldsm_x4((kbase[i] ^ ((c & 7) << 4)) + (c >> 3) * C::HALF, w);
           if constexpr (Q8) {
-            uint32_t w[4];
-            ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, kt + (lane >> 4)), w);
             codes_to_f16<CODE>(w[0], af[0][0], af[0][2]);
             codes_to_f16<CODE>(w[1], af[0][1], af[0][3]);
             codes_to_f16<CODE>(w[2], af[1][0], af[1][2]);
             codes_to_f16<CODE>(w[3], af[1][1], af[1][3]);
           } else {
-            ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(k0 + (lane & 15), kt * 2 + (lane >> 4)), af[0]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) af[0][x] = w[x];
           }
 #pragma unroll
           for (int u = 0; u < (Q8 ? 2 : 1); ++u)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_16816<MF16>(sc[j], af[u], qf[j][kt + u][0], qf[j][kt + u][1]);
+            for (int j = 0; j < NT; ++j) mma_16816<MF16>(sc[i][j], af[u], qf[j][kt + u][0], qf[j][kt + u][1]);
         }
-        float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
-        if constexpr (Q8) {
-          const float* kscale = reinterpret_cast<const float*>(ks + 2 * C::TILE) + k0 + qr;
-          ksc[0] = kscale[0];
-          ksc[1] = kscale[8];
-          vsc[0] = kscale[PR_BLK];
-          vsc[1] = kscale[PR_BLK + 8];
+      }
+      float vsc[MK][2];
+#pragma unroll
+      for (int i = 0; i < MK; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ksc = Q8 ? kscale[16 * i + 8 * e] : 1.0f;
+          vsc[i][e] = Q8 ? kscale[BLK + 16 * i + 8 * e] : 1.0f;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            sc[i][j][2 * e] *= Q8 ? fac[2 * j] * ksc : fac[2 * j];
+            sc[i][j][2 * e + 1] *= Q8 ? fac[2 * j + 1] * ksc : fac[2 * j + 1];
+          }
         }
+      bool slow = false;  // 16-bit: a value that is not finite and that some row may not see
+      uint32_t hidden = 0;  // bit ((i NT + j) 4 + e): the row does not see the key
+      if (!whole) {
+        int bad = 0;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int i = 0; i < MK; ++i) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[j][e] *= Q8 ? fac[2 * j + (e & 1)] * ksc[e >> 1] : fac[2 * j + (e & 1)];
-        bool slow = false;  // 16-bit: a value that is not finite and that some row may not see
-        uint32_t bits = 0xffffffffu;
-        if (!whole) {
-          bits = 0;
-          const int kk = k0 + qr;
-          bool readable[2];
+          for (int e = 0; e < 2; ++e) {
+            const int kk = 16 * i + qr + 8 * e, d = kb + kk - ctx;
+            const bool readable = kb + kk < end && ((good >> (kk >> a.group_log2)) & 1u);
+            if (!readable) vsc[i][e] = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            readable[e] = kb + kk + 8 * e < end && ((good >> ((kk + 8 * e) >> a.group_log2)) & 1u);
-#pragma unroll
-          for (int i = 0; i < 2 * NT; ++i) {
-            const int r = (i >> 1) * 8 + qc + (i & 1);
-            const int t = r / a.G;
-            uint64_t w = 0;
-            if (r < R) w = a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = kb + kk + 8 * e - ctx;
-              if (r < R && readable[e] && (d < 0 || ((w >> d) & 1ull))) bits |= 1u << (2 * i + e);
+            for (int x = 0; x < 2 * NT; ++x) {
+              const int r = (x >> 1) * 8 + qc + (x & 1);
+              bool see = r < R && readable;
+              if (see && d >= 0) {
+                const int t = r / a.G;
+                const uint64_t w = a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull);
+                see = (w >> d) & 1ull;
+              }
+              if (!see) {
+                hidden |= 1u << ((i * NT + (x >> 1)) * 4 + 2 * e + (x & 1));
+                sc[i][x >> 1][2 * e + (x & 1)] = -INFINITY;
+              }
             }
           }
-          if constexpr (Q8) {
-            if (!readable[0]) vsc[0] = 0.0f;
-            if (!readable[1]) vsc[1] = 0.0f;
-          }
-          int bad = 0;
+        }
 #pragma unroll 1
-          for (int i = 0; i < 16; ++i) {
-            const bool none = kb + k0 + i >= end || !((good >> ((k0 + i) >> a.group_log2)) & 1u);
-            for (int c = lane; c < C::ROW / 16; c += 32) {
-              uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(k0 + i, c));
-              if (none) {
-                *x = make_uint4(0, 0, 0, 0);  // values that may not be read: 0 * NaN would reach O
-              } else if constexpr (!Q8) {
-                const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-                const uint32_t w[4] = {x->x, x->y, x->z, x->w};
+        for (int i = 0; i < 16 * MK; ++i) {
+          const bool none = kb + i >= end || !((good >> ((i) >> a.group_log2)) & 1u);
+          for (int c = lane; c < C::ROW / 16; c += 32) {
+            uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(i, c));
+            if (none) {
+              *x = make_uint4(0, 0, 0, 0);  // values that may not be read: 0 * NaN would reach O
+            } else if constexpr (!Q8) {
+              const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+              const uint32_t w[4] = {x->x, x->y, x->z, x->w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
-              }
-            }
-          }
-          fence_proxy_async_shared();  // the ring slot is written by TMA next
-          if constexpr (!Q8) slow = __any_sync(0xffffffffu, bad);
-          else __syncwarp();
-        }
-        // references: taken up for the rows that need it
-        float top[2 * NT];
-        bool need = false;
-#pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-          float& s0 = sc[i >> 1][i & 1];
-          float& s1 = sc[i >> 1][2 + (i & 1)];
-          if (!((bits >> (2 * i)) & 1u)) s0 = -INFINITY;
-          if (!((bits >> (2 * i + 1)) & 1u)) s1 = -INFINITY;
-          top[i] = fmaxf(s0, s1);
-          need |= top[i] > m[i] + 6.0f;
-        }
-        if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-          for (int i = 0; i < 2 * NT; ++i) {
-            float v = top[i];
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            if (v > m[i] + 6.0f) {  // (for m = -inf as well)
-              const float al = ex2(m[i] - v);
-              m[i] = v;
-              l[i] *= al;
-#pragma unroll
-              for (int mt = 0; mt < KT; ++mt) {
-                o[mt][i >> 1][i & 1] *= al;
-                o[mt][i >> 1][2 + (i & 1)] *= al;
-              }
+              for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
             }
           }
         }
-        if constexpr (Q8) {
-          const float v0 = vsc[0] < INFINITY ? vsc[0] : 0.0f, v1 = vsc[1] < INFINITY ? vsc[1] : 0.0f;  // (NaN: 0)
-          float v = fmaxf(v0, v1);
-          if (__any_sync(0xffffffffu, v > 64.0f * vref)) {
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            const bool tiny = v < 1.2e-38f;  // such values are zero next to any output type's smallest step
-            const float be = tiny ? 1.0f : __fdividef(vref, v);
-            vinv = tiny ? 0.0f : __frcp_rn(v);
-            vref = v;
+        fence_proxy_async_shared();  // the ring slot is written by TMA next
+        __syncwarp();
+        if constexpr (!Q8) slow = __any_sync(0xffffffffu, bad);
+      }
+      // references: taken up for the rows that need it
+      float top[2 * NT];
+      bool need = false;
 #pragma unroll
-            for (int mt = 0; mt < KT; ++mt)
+      for (int x = 0; x < 2 * NT; ++x) {
+        float v = fmaxf(sc[0][x >> 1][x & 1], sc[0][x >> 1][2 + (x & 1)]);
 #pragma unroll
-              for (int j = 0; j < NT; ++j)
+        for (int i = 1; i < MK; ++i) v = fmaxf(v, fmaxf(sc[i][x >> 1][x & 1], sc[i][x >> 1][2 + (x & 1)]));
+        top[x] = v;
+        need |= v > m[x] + 6.0f;
+      }
+      if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][j][e] *= be;
+        for (int x = 0; x < 2 * NT; ++x) {
+          float v = top[x];
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          if (v > m[x] + 6.0f) {  // (for m = -inf as well)
+            const float al = ex2(m[x] - v);
+            m[x] = v;
+            l[x] *= al;
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt) {
+              o[mt][x >> 1][x & 1] *= al;
+              o[mt][x >> 1][2 + (x & 1)] *= al;
+            }
           }
         }
-        uint32_t pb[NT][2];
+      }
+      if constexpr (Q8) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MK; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) v = fmaxf(v, vsc[i][e] < INFINITY ? vsc[i][e] : 0.0f);  // (NaN: 0)
+        if (__any_sync(0xffffffffu, v > 64.0f * vref)) {
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          const bool tiny = v < 1.2e-38f;  // such values are zero next to any output type's smallest step
+          const float be = tiny ? 1.0f : __fdividef(vref, v);
+          vinv = tiny ? 0.0f : __frcp_rn(v);
+          vref = v;
+#pragma unroll
+          for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][j][e] *= be;
+        }
+      }
+      uint32_t pb[MK][NT][2];
+#pragma unroll
+      for (int i = 0; i < MK; ++i) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = 2 * j + (e & 1);
-            p[e] = ex2(sc[j][e] - (m[i] == -INFINITY ? 0.0f : m[i]));
+            const float ref = m[2 * j + (e & 1)];
+            p[e] = ex2(sc[i][j][e] - (ref == -INFINITY ? 0.0f : ref));
           }
           l[2 * j] += p[0] + p[2];
           l[2 * j + 1] += p[1] + p[3];
           if constexpr (Q8) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // a key that is not seen has a scale that may be anything
-              p[e] *= vsc[e >> 1] * vinv;
-              if (!((bits >> (2 * (2 * j + (e & 1)) + (e >> 1))) & 1u)) p[e] = 0.0f;
+            for (int e = 0; e < 4; ++e) p[e] *= vsc[i][e >> 1] * vinv;
+            if (!whole) {  // a key that is not seen has a scale that may be anything
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((hidden >> ((i * NT + j) * 4 + e)) & 1u) p[e] = 0.0f;
             }
           }
-          pb[j][0] = movmatrix_t(MF16 ? pack2<__half>(p[0], p[1]) : pack_bf16(p[0], p[1]));
-          pb[j][1] = movmatrix_t(MF16 ? pack2<__half>(p[2], p[3]) : pack_bf16(p[2], p[3]));
+          pb[i][j][0] = movmatrix_t(MF16 ? pack2<__half>(p[0], p[1]) : pack_bf16(p[0], p[1]));
+          pb[i][j][1] = movmatrix_t(MF16 ? pack2<__half>(p[2], p[3]) : pack_bf16(p[2], p[3]));
         }
-        const int mi = lane >> 3;
-        if (!Q8 && slow) {
-          // one product at a time: a weight of 0 leaves a value out that is not finite
+      }
+      const int mi = lane >> 3;
+      if (!Q8 && slow) {
+        // one product at a time: a weight of 0 leaves a value out that is not finite
 #pragma unroll 1
-          for (int kk = 0; kk < 16; ++kk) {
+        for (int kk = 0; kk < 16 * MK; ++kk) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                // weight of (row 8 j + qc + e, key kk): in pb[j][kk / 8] of lane (qc + e) * 4 + (kk % 8) / 2
-                const uint32_t w = __shfl_sync(0xffffffffu, kk < 8 ? pb[j][0] : pb[j][1], (qc + e) * 4 + ((kk & 7) >> 1));
-                const uint32_t w16 = (kk & 1) ? w >> 16 : w & 0xffffu;
-                const float p = F16 ? __half2float(__ushort_as_half((uint16_t)w16)) : __uint_as_float(w16 << 16);
+            for (int e = 0; e < 2; ++e) {
+              // weight of (row 8 j + qc + e, key kk): in pb[kk / 16][j][kk / 8 % 2] of lane (qc + e) * 4 + kk % 8 / 2
+              uint32_t w = 0;
 #pragma unroll
-                for (int mt = 0; mt < KT; ++mt)
+              for (int x = 0; x < 2 * MK; ++x)
+                if ((kk >> 3) == x) w = pb[x >> 1][j][x & 1];
+              w = __shfl_sync(0xffffffffu, w, (qc + e) * 4 + ((kk & 7) >> 1));
+              const uint32_t w16 = (kk & 1) ? w >> 16 : w & 0xffffu;
+              const float p = F16 ? __half2float(__ushort_as_half((uint16_t)w16)) : __uint_as_float(w16 << 16);
 #pragma unroll
-                  for (int u = 0; u < 2; ++u) {
-                    const int d = mt * 16 + qr + 8 * u;
-                    const uint16_t vr = *reinterpret_cast<const uint16_t*>(vs + pr_at<C::PITCH, C::HALF>(k0 + kk, d >> 3) + (d & 7) * 2);
-                    const float v = F16 ? __half2float(__ushort_as_half(vr)) : __uint_as_float((uint32_t)vr << 16);
-                    if (p != 0.0f) o[mt][j][2 * u + e] += p * v;
-                  }
-              }
-          }
-        } else {
+              for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const int d = mt * 16 + qr + 8 * u;
+                  const uint16_t vr = *reinterpret_cast<const uint16_t*>(vs + pr_at<C::PITCH, C::HALF>(kk, d >> 3) + (d & 7) * 2);
+                  const float v = F16 ? __half2float(__ushort_as_half(vr)) : __uint_as_float((uint32_t)vr << 16);
+                  if (p != 0.0f) o[mt][j][2 * u + e] += p * v;
+                }
+            }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MK; ++i) {
+          const uint32_t vbase = ex_smem_u32(vs) +
+                                 (Q8 ? pr_at<C::PITCH, C::HALF>(16 * i + (mi & 1) * 8 + (lane & 7), mi >> 1)
+                                     : pr_at<C::PITCH, C::HALF>(16 * i + (mi >> 1) * 8 + (lane & 7), mi & 1));
 #pragma unroll
           for (int mt = 0; mt < KT; mt += (Q8 ? 2 : 1)) {
-            uint32_t va[2][4];
+            const int c = Q8 ? mt : 2 * mt;
+            uint32_t va[2][4], w[4];  // codes: keys 0-7 | 8-15 of a 16-byte chunk (16 dims), then of the next
+            ldsm_x4_t((vbase ^ ((c & 7) << 4)) + (c >> 3) * C::HALF, w);
             if constexpr (Q8) {
-              uint32_t w[4];  // keys 0-7 | 8-15 of a 16-byte chunk (16 dims), then of the next
-              ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(k0 + (mi & 1) * 8 + (lane & 7), mt + (mi >> 1)), w);
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 transposed_to_f16<CODE>(w[2 * u], va[u][0], va[u][1]);
                 transposed_to_f16<CODE>(w[2 * u + 1], va[u][2], va[u][3]);
               }
             } else {
-              ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(k0 + (mi >> 1) * 8 + (lane & 7), mt * 2 + (mi & 1)), va[0]);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) va[0][x] = w[x];
             }
 #pragma unroll
             for (int u = 0; u < (Q8 ? 2 : 1); ++u)
 #pragma unroll
-              for (int j = 0; j < NT; ++j) mma_16816<MF16>(o[mt + u][j], va[u], pb[j][0], pb[j][1]);
+              for (int j = 0; j < NT; ++j) mma_16816<MF16>(o[mt + u][j], va[u], pb[i][j][0], pb[i][j][1]);
           }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(empty_bar + st);
+      if (++st == STAGES) st = 0, phase ^= 1;
+      load_block();  // into the slot that was just read
     }
-
-    // the four warps, in order: all brought to the largest m, then added up
+    if (!ok) break;
+    const bool single = pr_segments(keys) == 1;
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      float v = l[i];
-      v += __shfl_xor_sync(0xffffffffu, v, 4);
-      v += __shfl_xor_sync(0xffffffffu, v, 8);
-      v += __shfl_xor_sync(0xffffffffu, v, 16);
-      l[i] = v;
-      if (qr == 0) {
-        sm[warp * ROWS + (i >> 1) * 8 + qc + (i & 1)] = m[i];
-        sl[warp * ROWS + (i >> 1) * 8 + qc + (i & 1)] = v;
-      }
-    }
-    PR_BAR();
-    if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
-    float mall[2 * NT], lall[2 * NT];
+    for (int x = 0; x < 2 * NT; ++x) {
+      float lx = l[x];
+      lx += __shfl_xor_sync(0xffffffffu, lx, 4);
+      lx += __shfl_xor_sync(0xffffffffu, lx, 8);
+      lx += __shfl_xor_sync(0xffffffffu, lx, 16);
+      const int c = (x >> 1) * 8 + qc + (x & 1);
+      if (c >= R) continue;
+      const int t = c / a.G, h = g * a.G + c % a.G;
+      const float up = Q8 ? vref : 1.0f;
+      // 16 dims a tile: codes 2 qr, 2 qr + 1; 16-bit qr, qr + 8
+      if (single) {
+        const float inv = lx > 0.0f ? up / lx : (lx == 0.0f ? 0.0f : lx);  // nothing seen: zeros; NaN stays NaN
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t + (int64_t)h * a.so_h;
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      const int c = (i >> 1) * 8 + qc + (i & 1);
-      float v = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v = fmaxf(v, sm[w * ROWS + c]);
-      mall[i] = v;
-      const float sub = v == -INFINITY ? 0.0f : v;
-      float t = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) t += sl[w * ROWS + c] * ex2(sm[w * ROWS + c] - sub);
-      lall[i] = t;
-      const float f = ex2(m[i] - sub) * (Q8 ? vref : 1.0f);
-      const float keep = m[i] == -INFINITY ? 0.0f : f;
-#pragma unroll
-      for (int mt = 0; mt < KT; ++mt) {
-        o[mt][i >> 1][i & 1] *= keep;
-        o[mt][i >> 1][2 + (i & 1)] *= keep;
-      }
-    }
-    float* mine = so + (warp & 1) * ROWS * D;
-#pragma unroll
-    for (int phase = 0; phase < 2; ++phase) {
-      if ((warp >> 1) == phase) {
-#pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-          const int c = (i >> 1) * 8 + qc + (i & 1);
-          if (c < R) {
-#pragma unroll
-            for (int mt = 0; mt < KT; ++mt) {
-              // codes: dims 2 qr, 2 qr + 1 of the 16; 16-bit: qr, qr + 8
-              float* x = mine + c * D + mt * 16 + (Q8 ? 2 * qr : qr);
-              const float u = o[mt][i >> 1][i & 1], v = o[mt][i >> 1][2 + (i & 1)];
-              if (phase == 0) {
-                x[0] = u;
-                x[Q8 ? 1 : 8] = v;
-              } else {
-                x[0] += u;
-                x[Q8 ? 1 : 8] += v;
-              }
-            }
+        for (int mt = 0; mt < KT; ++mt) {
+          const float u = o[mt][x >> 1][x & 1] * inv, v = o[mt][x >> 1][2 + (x & 1)] * inv;
+          if constexpr (Q8) {
+            *reinterpret_cast<uint32_t*>(dst + mt * 16 + 2 * qr) = a.q_is_f16 ? pack2<__half>(u, v) : pack_bf16(u, v);
+          } else {
+            ex_store_out<F16 ? EX_DTYPE_F16 : EX_DTYPE_BF16>(dst, mt * 16 + qr, u);
+            ex_store_out<F16 ? EX_DTYPE_F16 : EX_DTYPE_BF16>(dst, mt * 16 + qr + 8, v);
           }
         }
-      }
-      PR_BAR();
-    }
-    const bool single = pr_segments(keys) == 1;
-    if (warp == 0 && qr == 0) {  // one thread per column
+      } else {
+        const int64_t pi = ((int64_t)(first + t) * a.H + h) * a.NS + s;
+        float* dst = a.ws_acc + pi * D;
 #pragma unroll
-      for (int i = 0; i < 2 * NT; ++i) {
-        const int c = (i >> 1) * 8 + qc + (i & 1);
-        sl[c] = lall[i];  // (every warp has read sm and sl: two barriers ago)
-        if (!single && c < R) {
-          const int64_t pi = ((int64_t)(first + c / a.G) * a.H + g * a.G + c % a.G) * a.NS + s;
-          a.ws_m[pi] = mall[i];
-          a.ws_l[pi] = lall[i];
+        for (int mt = 0; mt < KT; ++mt) {
+          const float u = o[mt][x >> 1][x & 1] * up, v = o[mt][x >> 1][2 + (x & 1)] * up;
+          if constexpr (Q8) {
+            *reinterpret_cast<float2*>(dst + mt * 16 + 2 * qr) = make_float2(u, v);
+          } else {
+            dst[mt * 16 + qr] = u;
+            dst[mt * 16 + qr + 8] = v;
+          }
+        }
+        if (qr == 0) {
+          a.ws_m[pi] = m[x];
+          a.ws_l[pi] = lx;
         }
       }
     }
-    PR_BAR();
-    for (int x = tid; x < R * (D / 4); x += 128) {
-      const int c = x / (D / 4), d = (x % (D / 4)) * 4;
-      const float4 u = *reinterpret_cast<const float4*>(so + c * D + d);
-      const float4 v = *reinterpret_cast<const float4*>(so + (ROWS + c) * D + d);
-      const float4 w = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
-      const int t = c / a.G, h = g * a.G + c % a.G;
-      if (single) {
-        const float lx = sl[c];
-        const float inv = lx > 0.0f ? 1.0f / lx : (lx == 0.0f ? 0.0f : lx);  // nothing seen: zeros; NaN stays NaN
-        uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t +
-                                                    (int64_t)h * a.so_h + d);
-        const bool f16 = Q8 ? a.q_is_f16 != 0 : F16;
-        dst[0] = f16 ? pack2<__half>(w.x * inv, w.y * inv) : pack_bf16(w.x * inv, w.y * inv);
-        dst[1] = f16 ? pack2<__half>(w.z * inv, w.w * inv) : pack_bf16(w.z * inv, w.w * inv);
-      } else {
-        *reinterpret_cast<float4*>(a.ws_acc + (((int64_t)(first + t) * a.H + h) * a.NS + s) * D + d) = w;
-      }
-    }
-    PR_BAR();  // before the buffers are written again
+  }
+  // after a wait that ran out: the loads in flight land before the CTA ends (each slot's own last phase, bounded)
+  if (!ok) {
+    for (int i = 0; i < STAGES; ++i) mbar_wait(full_bar + (st + i) % STAGES, phase ^ (st + i >= STAGES ? 1u : 0u), EX_DEVERR_WAIT_TMA);
   }
 }
 
-// Segments of a row merged in order; one warp per (token, query head), D/32 numbers a lane.
+// Segments of a row merged in order. D/2 threads a (token, query head), two numbers each: many loads in flight, and no
+// shared memory, so that the grid is resident before the first kernel, which takes all of it, has ended.
 template <int D, bool F16>
-__global__ void __launch_bounds__(256) k_paged_rows_merge(const __grid_constant__ PrArgs a) {
-  constexpr int V = D / 32;
+__global__ void __launch_bounds__(128) k_paged_rows_merge(const __grid_constant__ PrArgs a) {
+  constexpr int WARPS = D / 64;  // of a row
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int64_t row = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) / WARPS;
+  const int lane = threadIdx.x & 31, d = ((threadIdx.x >> 5) % WARPS * 32 + lane) * 2;
   if (row >= a.tokens * a.H) return;
   const int64_t tok = row / a.H;
   const int h = (int)(row % a.H);
@@ -1196,31 +1297,34 @@ __global__ void __launch_bounds__(256) k_paged_rows_merge(const __grid_constant_
   if (T == 0 || ns == 1) return;  // untouched, or written by the first kernel
   const float* pm = a.ws_m + row * a.NS;
   const float* pl = a.ws_l + row * a.NS;
-  float m = -INFINITY;
-  for (int s = lane; s < ns; s += 32) m = fmaxf(m, pm[s]);
+  const float* src = a.ws_acc + row * a.NS * D + d;
+  float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+  for (int s0 = 0; s0 < ns; s0 += 32) {  // 32 segments at a time: their factors first, a segment a lane
+    const bool have = s0 + lane < ns;
+    const float ms = have ? pm[s0 + lane] : -INFINITY, ls = have ? pl[s0 + lane] : 0.0f;
+    float mn = ms;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float sub = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < ns; ++s) {
-    const float c = ex2(pm[s] - sub);
-    l += pl[s] * c;
-    const float* src = a.ws_acc + (row * a.NS + s) * D + lane * V;
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(src + i);
-      acc[i] += v.x * c;
-      acc[i + 1] += v.y * c;
+    for (int o = 16; o; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mn = fmaxf(mn, m);
+    const float sub = mn == -INFINITY ? 0.0f : mn;
+    const float c = ex2(ms - sub), old = ex2(m - sub);
+    m = mn;
+    l *= old;
+    x *= old;
+    y *= old;
+    const int cnt = min(32, ns - s0);
+#pragma unroll 16
+    for (int s = 0; s < cnt; ++s) {
+      const float cs = __shfl_sync(0xffffffffu, c, s);
+      l += __shfl_sync(0xffffffffu, ls, s) * cs;
+      const float2 v = *reinterpret_cast<const float2*>(src + (int64_t)(s0 + s) * D);
+      x += v.x * cs;
+      y += v.y * cs;
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + tok * a.so_t + (int64_t)h * a.so_h + lane * V);
-#pragma unroll
-  for (int i = 0; i < V; i += 2)
-    dst[i / 2] = F16 ? pack2<__half>(acc[i] * inv, acc[i + 1] * inv) : pack_bf16(acc[i] * inv, acc[i + 1] * inv);
+  *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + tok * a.so_t + (int64_t)h * a.so_h + d) =
+      F16 ? pack2<__half>(x * inv, y * inv) : pack_bf16(x * inv, y * inv);
 }
 
 }  // namespace ex
