@@ -17,6 +17,7 @@
 #include "ex_cache_q8.cuh"
 #include "ex_paged_rows.cuh"
 #include "ex_prompt_attn.cuh"
+#include "ex_tree_tc.cuh"
 
 // Split-K scratch of ex_linear_noalloc: a file-scope device array, so that entry point never allocates. Host code
 // must not hand this symbol to a kernel (on the host it is only a stand-in); the device address is looked up once per
@@ -292,15 +293,6 @@ cudaError_t launch_smem(K kernel, bool (&done)[128], int grid, int threads, int 
 }
 
 template <int D, int CODE, bool F16, int NT>
-cudaError_t launch_rows_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
-                          cudaStream_t st) {
-  using C = ex::PrCfg<D, CODE, NT>;
-  static bool done[128] = {};
-  const int grid = (int)std::min<int64_t>(items, (int64_t)C::PER_SM * num_sms());
-  return launch_smem(ex::k_paged_rows<D, CODE, F16, NT>, done, grid, ex::PR_THREADS, C::SMEM, st, mk, mv, a);
-}
-
-template <int D, int CODE, bool F16, int NT>
 cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
                          cudaStream_t st) {
   using C = ex::PfCfg<D, CODE, NT>;
@@ -309,31 +301,37 @@ cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex:
   return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, done, grid, 32 * C::NW, C::SMEM, st, mk, mv, a);
 }
 
-// Requests of at most 16 rows a KV head go to k_paged_few, the others to k_paged_rows: by their own number of rows, so
-// that a request's bits do not depend on the longest one of the batch.
+struct CacheStrides {
+  const void* v;
+  int64_t block, page, head;
+};
+
+// Requests of at most 16 rows a KV head go to k_paged_few, the others to k_tree_tc: by their own number of rows, so that
+// a request's bits do not depend on the longest one of the batch.
 template <int D, int CODE, bool F16>
-cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, ex::PrArgs a, int64_t per_tile,
-                           cudaStream_t st) {
+cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const CacheStrides& c, ex::PrArgs a,
+                           int64_t per_tile, cudaStream_t st) {
   a.rows_lo = 0;
-  a.rows_hi = 16;
+  a.rows_hi = ex::PR_FEW;
   if (rows <= 8) return launch_few_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
   cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
-  if (rows <= 16 || e != cudaSuccess) return e;
-  a.rows_lo = 16;
+  if (rows <= ex::PR_FEW || e != cudaSuccess) return e;
+  a.rows_lo = ex::PR_FEW;
   a.rows_hi = INT32_MAX;
-  if (rows <= 32 || D == 256) return launch_rows_t<D, CODE, F16, 4>(mk, mv, a, per_tile * cdiv(rows, 32), st);
-  if constexpr (D != 256) return launch_rows_t<D, CODE, F16, 8>(mk, mv, a, per_tile * cdiv(rows, 64), st);
-  return cudaErrorInvalidValue;
+  using C = ex::PtcCfg<D, CODE>;
+  static bool done[128] = {};
+  const int grid = (int)std::min<int64_t>(per_tile * cdiv(rows, 128), num_sms());
+  return launch_smem(ex::k_tree_tc<D, CODE, F16>, done, grid, C::THREADS, C::SMEM, st, mk, mv, a, c.v, c.block, c.page, c.head);
 }
 
 template <int D>
 cudaError_t launch_rows_d(int code, int q_dtype, int rows, const CUtensorMap& mk, const CUtensorMap& mv,
-                          const ex::PrArgs& a, int64_t per_tile, cudaStream_t st) {
+                          const CacheStrides& c, const ex::PrArgs& a, int64_t per_tile, cudaStream_t st) {
   cudaError_t e;
-  if (code == ex::CODE_INT8) e = launch_rows_nt<D, ex::CODE_INT8, true>(rows, mk, mv, a, per_tile, st);
-  else if (code == ex::CODE_E4M3) e = launch_rows_nt<D, ex::CODE_E4M3, true>(rows, mk, mv, a, per_tile, st);
-  else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, a, per_tile, st);
-  else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, a, per_tile, st);
+  if (code == ex::CODE_INT8) e = launch_rows_nt<D, ex::CODE_INT8, true>(rows, mk, mv, c, a, per_tile, st);
+  else if (code == ex::CODE_E4M3) e = launch_rows_nt<D, ex::CODE_E4M3, true>(rows, mk, mv, c, a, per_tile, st);
+  else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, c, a, per_tile, st);
+  else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, c, a, per_tile, st);
   if (e != cudaSuccess || a.NS == 1) return e;
   const dim3 grid((unsigned)cdiv(a.tokens * a.H * (D / 64), 4)), block(128);
   if (q_dtype == EX_DTYPE_F16) return ex_launch_pdl(ex::k_paged_rows_merge<D, true>, grid, block, 0, st, a);
@@ -395,10 +393,11 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   if (!encode_rows_map(&mk, k_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box) ||
       !encode_rows_map(&mv, v_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box))
     return EX_ERR_UNSUPPORTED;
+  const CacheStrides c = {v_cache, s_block, s_page, s_head};
   cudaError_t e;
-  if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
-  else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
-  else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
+  else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
+  else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
   return cuda_status(e);
 }
 

@@ -4,17 +4,13 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - m),  x_j = (q . k_j) scale log2 e,  m the largest x_j so far
 //
 // The rows of a KV head are the (token, query head) pairs of its group, token-major. Keys are taken in segments whose
-// length depends on the request's own length only, in blocks of 64 inside a segment, and segments are merged in order:
+// length depends on the request's own length only, and segments are merged in order:
 // a row's bits do not depend on the other requests, the other rows, or where pages lie.
 //
-// Work: items (request, segment, KV head, tile of 8 NT rows), numbered by walking the requests' lengths on the device
-// (no host sync); CTA c takes items c, c + gridDim.x, ... Neighbouring items share keys or their pages' DRAM rows.
-//   warp 4     producer: TMA boxes of 8 or 16 tokens (one page each) into an mbarrier ring that runs ahead across
-//              items; scales of an 8-bit cache by bulk copies.
-//   warps 0-3  S^T = K Q^T: warp w owns keys 16w .. 16w + 15 of the block (MMA rows), the query rows are MMA columns.
-//              The block's row maxima are exchanged through shared memory, P goes there in 16 bits, and
-//              O^T += V^T P^T: warp w owns a quarter of the head dimension over all 64 keys, so O never needs a merge
-//              and an 8-bit code is converted once.
+// Work: items (request, segment, KV head, tile of rows), numbered by walking the requests' lengths on the device (no host
+// sync), dealt out in turn: neighbouring items share keys' pages. Requests of at most 16 rows a KV head are k_paged_few's,
+// the others k_tree_tc's (ex_tree_tc.cuh), by their own number of rows.
+//
 // 8-bit codes become float16 (exact). The key scale multiplies the score; the value scale goes into P, divided by the
 // largest value scale so far, which multiplies O in the end: float16 P keeps 11 bits of every weight that counts.
 // Queries are brought to float16 by a power of two per row, exact for all elements above 2^-14 of the row's largest.
@@ -27,53 +23,48 @@
 #define XSEG_A 256
 #define XSEG_B 512
 #endif
+#ifndef XTSEG
+#define XTSEG(L) ((L) <= 2048 ? 512 : 2048)
+#endif
 #ifndef XNW
 #define XNW ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 12 : (CODE == CODE_NONE ? 2 : 1) * D <= 256 ? 8 : 4)
 #endif
 #ifndef XMK
 #define XMK ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 2 : 1)
 #endif
-#ifndef XPER
-#define XPER (D == 256 && (NT == 2 || CODE == CODE_NONE) ? 1 : 2)
-#endif
 namespace ex {
 
-constexpr int PR_THREADS = 160;
-constexpr int PR_BLK = 64;       // keys a block
 constexpr int PR_MAX_TOKENS = 64;  // drafted tokens of a request (bits of a mask word)
 constexpr float PR_LOG2E = 1.4426950408889634f;
 
-// Keys a segment, by the request's own length.
+// Keys a segment, by the request's own length; of requests with at most 16 rows a KV head, and with more (whose results take
+// more memory traffic a segment).
 __host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? XSEG_A : XSEG_B; }
+__host__ __device__ inline int pr_segment_many(int64_t L) { return XTSEG(L); }
 __host__ __device__ inline int pr_segments(int64_t L) {
-  const int s = pr_segment(L);
-  const int n = (int)((L + s - 1) / s);
+  const int s = pr_segment(L), n = (int)((L + s - 1) / s);
   return n < 1 ? 1 : n;
 }
+__host__ __device__ inline int pr_segments_many(int64_t L) {
+  const int s = pr_segment_many(L), n = (int)((L + s - 1) / s);
+  return n < 1 ? 1 : n;
+}
+constexpr int PR_FEW = 16;  // rows a KV head
 // most segments of any request of at most max_len keys
 __host__ inline int pr_max_segments(int64_t max_len) {
   const int a = pr_segments(max_len < 2048 ? max_len : 2048), b = pr_segments(max_len);
   return a > b ? a : b;
 }
 
-template <int D, int CODE, int NT, int BLK = PR_BLK>
-struct PrCfg {
+// a block of keys in shared memory, as TMA writes it
+template <int D, int CODE, int BLK>
+struct PrTile {
   static constexpr int ESZ = CODE == CODE_NONE ? 2 : 1;
-  static constexpr int ROW = D * ESZ;                       // bytes of a key
-  static constexpr int PITCH = ROW < 128 ? ROW : 128;       // bytes of a row of a TMA box
-  static constexpr int NH = ROW / PITCH;                    // boxes across the head dimension
+  static constexpr int ROW = D * ESZ;                  // bytes of a key
+  static constexpr int PITCH = ROW < 128 ? ROW : 128;  // bytes of a row of a TMA box
+  static constexpr int NH = ROW / PITCH;               // boxes across the head dimension
   static constexpr int HALF = BLK * PITCH;
-  static constexpr int TILE = BLK * ROW;                 // K or V of a block
-  static constexpr int STAGE = 2 * TILE + (CODE == CODE_NONE ? 0 : 1024);  // + scales of the keys and of the values, padded
-  static constexpr int Q_BYTES = 8 * NT * D * 2;
-  static constexpr int P_BYTES = 8 * NT * 128;
-  static constexpr int MISC = 4 * 8 * NT * 4 /* maxima */ + 8 * NT * 4 /* row factors or sums */ + 512;
-  static constexpr int FIXED = Q_BYTES + P_BYTES + MISC + 1024;
-  static constexpr int PER_SM = (D == 256 && CODE == CODE_NONE) ? 1 : 2;
-  static constexpr int ROOM = (PER_SM == 1 ? 225 : 112) * 1024 - FIXED;
-  static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
-  static constexpr int SMEM = FIXED + STAGES * STAGE;
-  static_assert(STAGES >= 2, "ring");
+  static constexpr int TILE = BLK * ROW;               // K or V
 };
 
 struct PrArgs {
@@ -112,6 +103,7 @@ __device__ __forceinline__ void pr_request(const PrArgs& a, int b, int& first, i
 __device__ __forceinline__ int pr_keys(const PrArgs& a, int L) { return min(L, a.max_keys); }
 
 // Items in request order; all lanes of a warp walk together.
+template <bool MANY>
 struct PrWalk {
   int base = -32, total = 0, start = 0;  // window of 32 requests, its items, its first item
   int cnt = 0, incl = 0, first = 0, T = 0, L = 0;
@@ -128,7 +120,7 @@ struct PrWalk {
       if (r < a.n) {
         pr_request(a, r, first, T, L);
         if (T > 0 && T * a.G > a.rows_lo && T * a.G <= a.rows_hi)
-          cnt = pr_segments(pr_keys(a, L)) * a.KV * ((T * a.G + rows_per_tile - 1) / rows_per_tile);
+          cnt = (MANY ? pr_segments_many(pr_keys(a, L)) : pr_segments(pr_keys(a, L))) * a.KV * ((T * a.G + rows_per_tile - 1) / rows_per_tile);
       }
       incl = cnt;
 #pragma unroll
@@ -195,110 +187,6 @@ __device__ __forceinline__ uint32_t pr_at(int row, int chunk) {
   }
 }
 
-#define PR_BAR() asm volatile("bar.sync 1, 128;" ::: "memory")
-
-// The producer warp: every block of the CTA's items through the ring, running ahead of the consumers.
-template <int D, int CODE, int NT, int STAGES, int BLK = PR_BLK>
-__device__ __forceinline__ void pr_produce(const PrArgs& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* smem,
-                                           uint64_t* full_bar, uint64_t* empty_bar, uint32_t* sgood) {
-  using C = PrCfg<D, CODE, NT, BLK>;
-  constexpr bool Q8 = CODE != CODE_NONE;
-  const int lane = threadIdx.x & 31;
-  PrWalk walk;
-  uint32_t blkno = 0;
-  const int group = 1 << a.group_log2, per = BLK >> a.group_log2;  // at most 16 groups a block
-  // an item's keys and, a window of 32 groups at a time, where they lie: lane l holds the page of group l (-1: none)
-  int it = blockIdx.x, g = 0, start = 0, end = 0;
-  const int32_t* btr = a.bt;
-  auto next_item = [&]() {
-    int b, first, T, L, rem;
-    if (!walk.find(a, 8 * NT, it, b, first, T, L, rem)) return false;
-    it += gridDim.x;
-    const int tiles = (T * a.G + 8 * NT - 1) / (8 * NT);
-    const int keys = pr_keys(a, L), seg = pr_segment(keys);
-    g = (rem / tiles) % a.KV;
-    start = rem / (tiles * a.KV) * seg;
-    end = min(keys, start + seg);
-    btr = a.bt + (int64_t)b * a.sbt;
-    return true;
-  };
-  auto window = [&](int key, int last, int& page, int& off) {
-    const int key0 = key + lane * group;
-    page = -1;
-    if (key0 < last) {
-      page = btr[key0 / a.BS];
-      off = key0 % a.BS;
-    }
-  };
-  bool ok = true, have = next_item();
-  int page = -1, off = 0;
-  if (have) window(start, end, page, off);
-  while (have && ok) {
-    const int cg = g, cend = end;
-    int wkey = start;
-    bool more = true;
-    // the window after this one is looked up while this one is loaded: of this item, or the first of the next
-    while (more && ok) {
-      const int after = wkey + 32 * group;
-      int npage = -1, noff = 0;
-      more = after < cend;
-      if (more) {
-        window(after, cend, npage, noff);
-      } else {
-        have = next_item();
-        if (have) window(start, end, npage, noff);
-      }
-      const unsigned goods = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
-      for (int base = 0; base < 32; base += per) {
-        if (wkey + base * group >= cend) break;
-        const int st = blkno % STAGES;
-        ok = mbar_wait(empty_bar + st, ((blkno / STAGES) & 1u) ^ 1u, EX_DEVERR_WAIT_SLOT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const unsigned good = (goods >> base) & ((1u << per) - 1u);
-        if (lane == 0) {
-          sgood[st] = good;
-          mbar_arrive_expect_tx(full_bar + st, (uint32_t)(__popc(good) * group * (2 * C::ROW)));
-        }
-        __syncwarp();
-        const int sub = lane - base;
-        if (sub >= 0 && sub < per && ((good >> sub) & 1u)) {
-          uint8_t* ks = smem + st * C::STAGE;
-          uint8_t* vs = ks + C::TILE;
-#pragma unroll
-          for (int h = 0; h < C::NH; ++h) {
-            tma_load_4d(ks + h * C::HALF + sub * group * C::PITCH, tm_k, full_bar + st, h * (C::PITCH / C::ESZ), cg, off, page);
-            tma_load_4d(vs + h * C::HALF + sub * group * C::PITCH, tm_v, full_bar + st, h * (C::PITCH / C::ESZ), cg, off, page);
-          }
-        }
-        if constexpr (Q8) {
-          // scales: 16 bytes of four tokens a lane. Not by bulk copies: as many of them as of the codes' boxes, 64 bytes
-          // each, would take as much of the TMA unit as the codes.
-          const int from = min(base + ((lane * 4) >> a.group_log2), 31);
-          const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
-          if (lane < BLK / 4 && ((goods >> from) & 1u)) {
-            float* ss = reinterpret_cast<float*>(smem + st * C::STAGE + 2 * C::TILE) + lane * 4;
-            const int64_t so = (int64_t)pg * a.ss_block + cg * a.ss_head + po + ((lane * 4) & (group - 1));
-            cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
-            cp_async16(ex_smem_u32(ss + BLK), a.v_scale + so, true);
-          }
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(full_bar + st)) : "memory");
-        }
-        __syncwarp();
-        ++blkno;
-      }
-      wkey = after;
-      page = npage;
-      off = noff;
-    }
-  }
-  // every load has landed before the CTA ends (also after a wait that ran out)
-  if (lane == 0) {
-    for (uint32_t i = blkno > (uint32_t)STAGES ? blkno - STAGES : 0; i < blkno; ++i)
-      mbar_wait(full_bar + i % STAGES, (i / STAGES) & 1u, EX_DEVERR_WAIT_TMA);
-  }
-  __syncwarp();
-}
 
 // 1 / f and f = 2^e with m in [f, 2f): what a row with largest element m is divided by on its way to float16. Exponents
 // are kept where both are normal numbers.
@@ -324,459 +212,6 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
   }
 }
 
-template <int D, int CODE, bool F16, int NT>
-__global__ void __launch_bounds__(PR_THREADS, PrCfg<D, CODE, NT>::PER_SM)
-    k_paged_rows(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ PrArgs a) {
-  using C = PrCfg<D, CODE, NT>;
-  constexpr bool Q8 = CODE != CODE_NONE;
-  constexpr bool MF16 = Q8 || F16;  // MMA type
-  constexpr int ROWS = 8 * NT;
-  constexpr int MT = D / 64;        // 16-dim tiles of a warp's quarter
-  extern __shared__ uint8_t pr_smem_raw[];
-  uint8_t* smem = pr_smem_raw + ((0u - ex_smem_u32(pr_smem_raw)) & 1023u);
-  uint8_t* sq = smem + C::STAGES * C::STAGE;
-  uint8_t* sp = sq + C::Q_BYTES;
-  float* smax = reinterpret_cast<float*>(sp + C::P_BYTES);  // [4][ROWS]
-  float* sfac = smax + 4 * ROWS;                            // [ROWS]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sfac + ROWS);
-  uint64_t* empty_bar = full_bar + 8;
-  uint32_t* sgood = reinterpret_cast<uint32_t*>(empty_bar + 8);  // groups of a stage whose page exists
-  volatile int* sfail = reinterpret_cast<int*>(sgood + 8);       // a wait ran out
-  volatile int* sbad = reinterpret_cast<int*>(sgood + 9);        // [4] a warp's keys have values that are not finite
-
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_launch_dependents();
-  if (tid == 0) {
-    *sfail = 0;
-    for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(full_bar + i, Q8 ? 33 : 1);  // codes: and every producer lane's copies of scales
-      mbar_init(empty_bar + i, 4);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  pdl_wait();
-
-  if (warp == 4) {
-    pr_produce<D, CODE, NT, C::STAGES>(a, &tm_k, &tm_v, smem, full_bar, empty_bar, sgood);
-    return;
-  }
-  PrWalk walk;
-  uint32_t blkno = 0;  // blocks through the ring so far
-  // -------------------------------------------------------------------------------------------------- consumers
-  const int qr = lane >> 2, qc = (lane & 3) * 2;
-  const uint32_t sq0 = ex_smem_u32(sq), sp0 = ex_smem_u32(sp);
-  bool alive = true;
-  for (int it = blockIdx.x; alive; it += gridDim.x) {
-    int b, first, T, L, rem;
-    if (!walk.find(a, ROWS, it, b, first, T, L, rem)) break;
-    const int R = T * a.G;
-    const int tiles = (R + ROWS - 1) / ROWS;
-    const int row0 = (rem % tiles) * ROWS;
-    const int g = (rem / tiles) % a.KV, s = rem / (tiles * a.KV);
-    const int keys = pr_keys(a, L), seg = pr_segment(keys);
-    const int start = s * seg, end = min(keys, start + seg);
-    const int ctx = L - T;  // keys before the drafted tokens
-
-    // queries to shared memory: row-major, 16-byte chunks swizzled; a row takes D/8 lanes
-    PR_BAR();  // the last item's readers are done
-    {
-      constexpr int LANES = D / 8;
-      const int c = tid % LANES;
-      for (int r = tid / LANES; r < ROWS; r += 128 / LANES) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row0 + r < R) {
-          const int t = (row0 + r) / a.G, h = (row0 + r) % a.G;
-          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + t) * a.sq_t +
-                                              (int64_t)(g * a.G + h) * a.sq_h + c * 8);
-        }
-        if constexpr (!Q8) {
-          *reinterpret_cast<uint4*>(sq + r * D * 2 + ((c ^ (r & 7)) << 4)) = v;
-        } else {
-          float f = 1.0f;
-          if (!a.q_is_f16) {
-            float x[8];
-            unpack2<__nv_bfloat16>(v.x, x[0], x[1]);
-            unpack2<__nv_bfloat16>(v.y, x[2], x[3]);
-            unpack2<__nv_bfloat16>(v.z, x[4], x[5]);
-            unpack2<__nv_bfloat16>(v.w, x[6], x[7]);
-            float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-#pragma unroll
-            for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float inv = pr_query_scale(m, f);
-            v.x = pack2<__half>(x[0] * inv, x[1] * inv);
-            v.y = pack2<__half>(x[2] * inv, x[3] * inv);
-            v.z = pack2<__half>(x[4] * inv, x[5] * inv);
-            v.w = pack2<__half>(x[6] * inv, x[7] * inv);
-          }
-          if (c == 0) sfac[r] = f * a.scale_log2;
-          // A thread's four code bytes are four consecutive dims, MMA slots 2i, 2i+1, 2i+8, 2i+9 of a 16-dim step: the
-          // query dims are stored in slot order. Dims 8c' .. 8c'+7 of the step: pairs go to slots (4c'+0, 4c'+8, 4c'+2, 4c'+10).
-          uint8_t* base = sq + r * D * 2;
-          const int step = c >> 1, half = c & 1;  // this chunk holds dims 8 half .. of the 16-dim step
-          auto put = [&](int slot, uint32_t val) {
-            const int chunk = step * 2 + (slot >> 3);
-            *reinterpret_cast<uint32_t*>(base + ((chunk ^ (r & 7)) << 4) + (slot & 7) * 2) = val;
-          };
-          put(4 * half, v.x);
-          put(4 * half + 8, v.y);
-          put(4 * half + 2, v.z);
-          put(4 * half + 10, v.w);
-        }
-      }
-    }
-    PR_BAR();
-    float fac[2 * NT];  // score factors of this thread's columns
-#pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) fac[i] = Q8 ? sfac[(i >> 1) * 8 + qc + (i & 1)] : a.scale_log2;
-
-    float m_run[2 * NT], l_run[2 * NT];
-    float o[MT][NT][4];
-    float vm = 0.0f;  // largest value scale so far
-#pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      m_run[i] = -INFINITY;
-      l_run[i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
-
-    for (int kb = start; kb < end; kb += PR_BLK, ++blkno) {
-      const int st = blkno % C::STAGES;
-      if (!mbar_wait(full_bar + st, (blkno / C::STAGES) & 1u, EX_DEVERR_WAIT_TMA)) *sfail = 1;
-      uint8_t* ks = smem + st * C::STAGE;
-      uint8_t* vs = ks + C::TILE;
-      const uint32_t ks0 = ex_smem_u32(ks), vs0 = ex_smem_u32(vs);
-      const float* kscale = reinterpret_cast<const float*>(ks + 2 * C::TILE);
-      const float* vscale = kscale + PR_BLK;
-      const uint32_t good = sgood[st];
-      const int per = PR_BLK >> a.group_log2;
-      const bool whole = kb + PR_BLK <= min(end, ctx) && good == (1u << per) - 1u;  // every row sees every key
-
-      // S^T: 16 keys x ROWS
-      float sc[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
-#pragma unroll
-      for (int kt = 0; kt < D / 16; kt += (Q8 ? 2 : 1)) {
-        uint32_t af[2][4];
-        if constexpr (Q8) {
-          uint32_t w[4];  // keys 0-7 | 8-15 of dims 16 kt .., then of the next 16 dims
-          const int row = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-          ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(row, kt + (lane >> 4)), w);
-          codes_to_f16<CODE>(w[0], af[0][0], af[0][2]);
-          codes_to_f16<CODE>(w[1], af[0][1], af[0][3]);
-          codes_to_f16<CODE>(w[2], af[1][0], af[1][2]);
-          codes_to_f16<CODE>(w[3], af[1][1], af[1][3]);
-        } else {
-          ldsm_x4(ks0 + pr_at<C::PITCH, C::HALF>(warp * 16 + (lane & 15), kt * 2 + (lane >> 4)), af[0]);
-        }
-#pragma unroll
-        for (int u = 0; u < (Q8 ? 2 : 1); ++u) {
-          const int k2 = (kt + u) * 2;
-          if constexpr (NT == 1) {
-            uint32_t b0, b1;
-            const uint32_t ad = sq0 + (lane & 7) * D * 2 + (((k2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(ad));
-            mma_16816<MF16>(sc[0], af[u], b0, b1);
-          } else {
-#pragma unroll
-            for (int j = 0; j < NT; j += 2) {
-              uint32_t bf[4];
-              const int r = j * 8 + (lane & 7) + (lane >> 4) * 8;
-              ldsm_x4(sq0 + r * D * 2 + (((k2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4), bf);
-              mma_16816<MF16>(sc[j], af[u], bf[0], bf[1]);
-              mma_16816<MF16>(sc[j + 1], af[u], bf[2], bf[3]);
-            }
-          }
-        }
-      }
-      // scale, mask, block maxima
-      const int k0 = warp * 16 + qr;  // this thread's keys are kb + k0 and kb + k0 + 8
-      float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
-      if constexpr (Q8) {
-        ksc[0] = kscale[k0];
-        ksc[1] = kscale[k0 + 8];
-        vsc[0] = vscale[k0];
-        vsc[1] = vscale[k0 + 8];
-      }
-      float mx[2 * NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[j][e] *= Q8 ? fac[2 * j + (e & 1)] * ksc[e >> 1] : fac[2 * j + (e & 1)];
-      uint32_t bits = 0xffffffffu;  // visible: bit (2 * j + (e & 1)) * 2 + (e >> 1)
-      if (!whole) {
-        bits = 0;
-#pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-          const int r = row0 + (i >> 1) * 8 + qc + (i & 1);
-          const int t = r / a.G;
-          uint64_t w = 0;
-          if (r < R) w = a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int kk = k0 + 8 * h, key = kb + kk;
-            const int d = key - ctx;
-            const bool see = r < R && key < end && ((good >> (kk >> a.group_log2)) & 1u) && (d < 0 || ((w >> d) & 1ull));
-            if (see) bits |= 1u << (2 * i + h);
-          }
-        }
-        // values of keys that may not be read: zeroed, since 0 * NaN would reach O
-        int bad = 0;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          const int kk = warp * 16 + i;
-          const bool none = kb + kk >= end || !((good >> (kk >> a.group_log2)) & 1u);
-          for (int c = lane; c < C::ROW / 16; c += 32) {
-            uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(kk, c));
-            if (none) {
-              *x = make_uint4(0, 0, 0, 0);
-            } else if constexpr (!Q8) {  // (codes are finite; a scale that is not only reaches rows that see it)
-              const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-              const uint32_t w[4] = {x->x, x->y, x->z, x->w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
-            }
-          }
-        }
-        if constexpr (!Q8) {
-          bad = __any_sync(0xffffffffu, bad);
-          if (lane == 0) sbad[warp] = bad;
-        }
-        fence_proxy_async_shared();  // the ring slot is written by TMA next
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * NT; ++i) {
-        float& s0 = sc[i >> 1][i & 1];
-        float& s1 = sc[i >> 1][2 + (i & 1)];
-        if (!((bits >> (2 * i)) & 1u)) s0 = -INFINITY;
-        if (!((bits >> (2 * i + 1)) & 1u)) s1 = -INFINITY;
-        float v = fmaxf(s0, s1);
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        mx[i] = v;
-      }
-      if (qr == 0) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          *reinterpret_cast<float2*>(smax + warp * ROWS + j * 8 + qc) = make_float2(mx[2 * j], mx[2 * j + 1]);
-      }
-      float beta = 1.0f, vinv = 1.0f;
-      if constexpr (Q8) {  // the largest finite value scale among the keys that may be read
-        float v = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int kk = lane + 32 * h;
-          if (kb + kk < end && ((good >> (kk >> a.group_log2)) & 1u) && vscale[kk] < INFINITY) v = fmaxf(v, vscale[kk]);
-        }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-        const float vn = fmaxf(vm, v);
-        const bool tiny = vn < 1.2e-38f;  // such values are zero next to any output type's smallest step
-        beta = tiny ? 1.0f : __fdividef(vm, vn);
-        vinv = tiny ? 0.0f : __frcp_rn(vn);
-        vm = vn;
-      }
-      PR_BAR();
-      if (*sfail) {  // the same for every thread here: the flag is only set before the barrier
-        alive = false;
-        break;
-      }
-      float alpha[2 * NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float2 v = *reinterpret_cast<const float2*>(smax + j * 8 + qc);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) {
-          const float2 u = *reinterpret_cast<const float2*>(smax + w * ROWS + j * 8 + qc);
-          v.x = fmaxf(v.x, u.x);
-          v.y = fmaxf(v.y, u.y);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * j + e;
-          const float mn = fmaxf(m_run[i], e ? v.y : v.x);
-          const float sub = mn == -INFINITY ? 0.0f : mn;
-          alpha[i] = mn == -INFINITY ? 1.0f : ex2(m_run[i] - mn);
-          m_run[i] = mn;
-          const float p0 = ex2(sc[j][e] - sub), p1 = ex2(sc[j][2 + e] - sub);
-          l_run[i] = l_run[i] * alpha[i] + (p0 + p1);
-          sc[j][e] = p0;
-          sc[j][2 + e] = p1;
-          if constexpr (Q8) {  // a key that is not seen has a scale that may be anything
-            sc[j][e] = ((bits >> (2 * i)) & 1u) ? p0 * (vsc[0] * vinv) : 0.0f;
-            sc[j][2 + e] = ((bits >> (2 * i + 1)) & 1u) ? p1 * (vsc[1] * vinv) : 0.0f;
-          }
-        }
-        // P^T (rows x keys): 8 x 8 blocks transposed on the way, so that a B fragment is one ldmatrix row
-        const uint32_t p01 = movmatrix_t(MF16 ? pack2<__half>(sc[j][0], sc[j][1]) : pack_bf16(sc[j][0], sc[j][1]));
-        const uint32_t p23 = movmatrix_t(MF16 ? pack2<__half>(sc[j][2], sc[j][3]) : pack_bf16(sc[j][2], sc[j][3]));
-        const int r = j * 8 + qr;
-        *reinterpret_cast<uint32_t*>(sp + r * 128 + (((warp * 2) ^ (r & 7)) << 4) + qc * 2) = p01;
-        *reinterpret_cast<uint32_t*>(sp + r * 128 + (((warp * 2 + 1) ^ (r & 7)) << 4) + qc * 2) = p23;
-      }
-      PR_BAR();
-      // O^T: this warp's quarter of the head dimension
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          o[i][j][0] *= alpha[2 * j] * beta;
-          o[i][j][1] *= alpha[2 * j + 1] * beta;
-          o[i][j][2] *= alpha[2 * j] * beta;
-          o[i][j][3] *= alpha[2 * j + 1] * beta;
-        }
-      bool slow = false;
-      if constexpr (!Q8) {
-        // values that are not finite behind a row's mask: a product of tensor cores would give 0 * inf to rows that
-        // do not see them, so such a block's products are made one by one
-        slow = !whole && (sbad[0] | sbad[1] | sbad[2] | sbad[3]);
-        if (slow) {
-#pragma unroll 1
-          for (int kk = 0; kk < PR_BLK; ++kk) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int d = (warp * MT + i) * 16 + qr + (e >> 1) * 8;
-                const uint16_t vr = *reinterpret_cast<const uint16_t*>(vs + pr_at<C::PITCH, C::HALF>(kk, d >> 3) + (d & 7) * 2);
-                const float v = F16 ? __half2float(__ushort_as_half(vr)) : __uint_as_float((uint32_t)vr << 16);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                  const int r = j * 8 + qc + (e & 1);
-                  const uint16_t pr = *reinterpret_cast<const uint16_t*>(sp + r * 128 + (((kk >> 3) ^ (r & 7)) << 4) + (kk & 7) * 2);
-                  const float p = F16 ? __half2float(__ushort_as_half(pr)) : __uint_as_float((uint32_t)pr << 16);
-                  if (p != 0.0f) o[i][j][e] += p * v;
-                }
-              }
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {  // 16 keys a step
-        if (slow) break;
-        uint32_t va[MT][4];
-        const int mi = lane >> 3;
-        if constexpr (!Q8) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)  // 16 dims: chunks 2x, 2x + 1; dims qr and qr + 8
-            ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(kt * 16 + (mi >> 1) * 8 + (lane & 7), (warp * MT + i) * 2 + (mi & 1)), va[i]);
-        } else {
-          // one 16-byte chunk is 16 dims; after the transposing load a word holds dims 2 qr, 2 qr + 1 of two keys
-          if constexpr (MT == 1) {
-            uint32_t w0, w1;
-            const uint32_t ad = vs0 + pr_at<C::PITCH, C::HALF>(kt * 16 + (mi & 1) * 8 + (lane & 7), warp);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(w0), "=r"(w1) : "r"(ad));
-            transposed_to_f16<CODE>(w0, va[0][0], va[0][1]);
-            transposed_to_f16<CODE>(w1, va[0][2], va[0][3]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < MT; i += 2) {
-              uint32_t w[4];
-              ldsm_x4_t(vs0 + pr_at<C::PITCH, C::HALF>(kt * 16 + (mi & 1) * 8 + (lane & 7), warp * MT + i + (mi >> 1)), w);
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                transposed_to_f16<CODE>(w[2 * u], va[i + u][0], va[i + u][1]);
-                transposed_to_f16<CODE>(w[2 * u + 1], va[i + u][2], va[i + u][3]);
-              }
-            }
-          }
-        }
-        if constexpr (NT == 1) {
-          uint32_t b0, b1;
-          const uint32_t ad = sp0 + (lane & 7) * 128 + (((kt * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-          asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(ad));
-#pragma unroll
-          for (int i = 0; i < MT; ++i) mma_16816<MF16>(o[i][0], va[i], b0, b1);
-        } else {
-#pragma unroll
-          for (int j = 0; j < NT; j += 2) {
-            uint32_t bf[4];
-            const int r = j * 8 + (lane & 7) + (lane >> 4) * 8;
-            ldsm_x4(sp0 + r * 128 + (((kt * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4), bf);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              mma_16816<MF16>(o[i][j], va[i], bf[0], bf[1]);
-              mma_16816<MF16>(o[i][j + 1], va[i], bf[2], bf[3]);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty_bar + st);
-    }
-
-    if (!alive) break;
-    // the segment's sums: a warp holds those of its own keys
-#pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      float v = l_run[i];
-      v += __shfl_xor_sync(0xffffffffu, v, 4);
-      v += __shfl_xor_sync(0xffffffffu, v, 8);
-      v += __shfl_xor_sync(0xffffffffu, v, 16);
-      l_run[i] = v;
-    }
-    PR_BAR();  // the last block's maxima have been read
-    if (qr == 0) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        *reinterpret_cast<float2*>(smax + warp * ROWS + j * 8 + qc) = make_float2(l_run[2 * j], l_run[2 * j + 1]);
-    }
-    PR_BAR();
-    const bool single = pr_segments(keys) == 1;
-#pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      const int c = (i >> 1) * 8 + qc + (i & 1);
-      const int r = row0 + c;
-      if (r >= R) continue;
-      const float l = (smax[c] + smax[ROWS + c]) + (smax[2 * ROWS + c] + smax[3 * ROWS + c]);
-      const int t = r / a.G, h = g * a.G + r % a.G;
-      const float up = Q8 ? vm : 1.0f;
-      if (single) {
-        const float inv = l > 0.0f ? up / l : (l == 0.0f ? 0.0f : l);  // nothing seen: zeros; NaN stays NaN
-        const int64_t at = (int64_t)(first + t) * a.so_t + (int64_t)h * a.so_h;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float x = o[mt][i >> 1][i & 1] * inv, y = o[mt][i >> 1][2 + (i & 1)] * inv;
-          const int d0 = (warp * MT + mt) * 16;
-          if constexpr (Q8) {
-            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + at + d0 + 2 * qr);
-            *dst = a.q_is_f16 ? pack2<__half>(x, y) : pack_bf16(x, y);
-          } else {
-            ex_store_out<F16 ? EX_DTYPE_F16 : EX_DTYPE_BF16>(a.out, at + d0 + qr, x);
-            ex_store_out<F16 ? EX_DTYPE_F16 : EX_DTYPE_BF16>(a.out, at + d0 + qr + 8, y);
-          }
-        }
-      } else {
-        const int64_t pi = ((int64_t)(first + t) * a.H + h) * a.NS + s;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float x = o[mt][i >> 1][i & 1] * up, y = o[mt][i >> 1][2 + (i & 1)] * up;
-          float* dst = a.ws_acc + pi * D + (warp * MT + mt) * 16;
-          if constexpr (Q8) {
-            *reinterpret_cast<float2*>(dst + 2 * qr) = make_float2(x, y);
-          } else {
-            dst[qr] = x;
-            dst[qr + 8] = y;
-          }
-        }
-        if (warp == 0 && qr == 0) {
-          a.ws_m[pi] = m_run[i];
-          a.ws_l[pi] = l;
-        }
-      }
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------------------------------------
 // At most 16 rows of a KV head: a decode step, or a few drafted tokens.
 //
@@ -791,7 +226,7 @@ struct PfCfg {
   static constexpr int MK = XMK;                       // 16-key tiles of a block
   static constexpr int NW = XNW;                       // warps of a CTA, one CTA per SM
   static constexpr int BLK = 16 * MK;
-  using R = PrCfg<D, CODE, NT, BLK>;
+  using R = PrTile<D, CODE, BLK>;
   static constexpr int STAGE = 2 * R::TILE;
   static constexpr int SCALES = CODE == CODE_NONE ? 0 : 8 * BLK;  // bytes of a block's scales, keys' first
   static constexpr int ROOM = (225 * 1024) / NW;
@@ -832,7 +267,7 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
   const int stride = gridDim.x * NW;
   const int glog = a.group_log2, group = 1 << glog, per = BLK >> glog;  // groups of a block
   // ---- what is loaded next: an item's keys and, for groups lane and lane + 32 of it, where they lie
-  PrWalk lwalk;
+  PrWalk<false> lwalk;
   int lit = warp * gridDim.x + blockIdx.x, lg = 0, lkey = 0, lend = 0, lgi = 0, page[2] = {-1, -1}, off[2] = {0, 0};
   bool lhave = true;
   int lslot = 0;
@@ -903,7 +338,7 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
   for (int i = 0; i < STAGES; ++i) load_block();
 
   // ---- what is computed
-  PrWalk walk;
+  PrWalk<false> walk;
   int st = 0;  // ring slot of the next block and its phase
   uint32_t phase = 0;
   const int qr = lane >> 2, qc = (lane & 3) * 2;
@@ -1293,7 +728,7 @@ __global__ void __launch_bounds__(128) k_paged_rows_merge(const __grid_constant_
   }
   int first, T, L;
   pr_request(a, b, first, T, L);
-  const int ns = pr_segments(pr_keys(a, L));
+  const int ns = T * a.G > PR_FEW ? pr_segments_many(pr_keys(a, L)) : pr_segments(pr_keys(a, L));
   if (T == 0 || ns == 1) return;  // untouched, or written by the first kernel
   const float* pm = a.ws_m + row * a.NS;
   const float* pl = a.ws_l + row * a.NS;

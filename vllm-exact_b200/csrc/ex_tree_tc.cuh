@@ -1,0 +1,682 @@
+// Attention of many query rows per KV head (more than 16: drafted tokens times grouped heads) over a 16-bit or 8-bit
+// paged cache, on tcgen05. The mathematics and the masks are those of ex_paged_rows.cuh.
+//
+// One CTA per SM takes items (request, segment of its keys, KV head, tile of 128 rows) and walks the segment in blocks
+// of 128 keys: S = Q K^T with both operands in shared memory, O += P V with P in tensor memory over the S it came
+// from. D <= 128: blocks alternate between two streams, each with its own S, O, m and l and its own four softmax warps, so
+// that one stream's softmax runs beside the other's products; the streams are added up at the end of the segment.
+// D = 256: one O, two S buffers.
+//   warps 0-3, 4-7  softmax, one row a thread (they also bring Q to shared memory and write the results)
+//   warp 8          issues the products
+//   warp 9          producer: TMA boxes of 8 or 16 tokens through the block table into a ring of slots
+//   warp 10         16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
+//                   are not finite are zeroed and noted, and added in the end to the rows that see them
+//   warps 12-15     8-bit: codes to float16 tiles (exact; keys behind the end to zeros)
+// Bound by reading the cache once: a block of 128 keys of a 16-bit cache is 64 KB (D = 128), 1.5 us of an SM's share of HBM;
+// its products take 0.55 us and the 128 exponentials of a row 0.55 us on every scheduler that has rows.
+#pragma once
+#include "ex_paged_rows.cuh"
+#include "ex_prompt_attn.cuh"
+
+namespace ex {
+
+template <int D, int CODE>
+struct PtcCfg {
+  static constexpr bool Q8 = CODE != CODE_NONE;
+  static constexpr int STREAMS = D == 256 ? 1 : 2;
+  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr int SW = D < 128 ? D : 128;       // dims of a 16-bit slot
+  static constexpr int PARTS = D / SW;               // slots of a block's K or V
+  static constexpr int SUB = 128 * 128;              // 128 rows x 64 dims of 16 bits, one swizzled column
+  static constexpr int SLOT = SW / 64 * SUB;
+  static constexpr int Q_BYTES = (D / 64) * SUB;
+  static constexpr int RAW = Q8 ? 128 * SW : 0;      // bytes of a slot of codes: 128 keys, SW dims
+  static constexpr int SLOTS = D == 64 ? (Q8 ? 6 : 8) : (Q8 ? 3 : 5);
+  static constexpr int RAWS = !Q8 ? 0 : D == 64 ? 6 : D == 128 ? 5 : 3;  // slots of codes
+  static constexpr int GROUPS = 256;                 // page table entries of a segment (2048 keys, boxes of 8)
+  // Blocks whose scales and pages are kept. While block j's weights are made, its values are the first tile not used up:
+  // number 2 j + 2 in the order K0 K1 V0 K2 V1 .. of loading. The rings hold SLOTS + RAWS more, keys of block m being number
+  // 2 m - 1: m < j + 8 as long as they are at most 13.
+  static constexpr int SCALE_BLOCKS = 8;
+  static_assert((SLOTS + RAWS) / PARTS <= 13, "blocks ahead");
+  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + GROUPS * 4 + (Q8 ? SCALE_BLOCKS * 1024 + 512 : 0) + 768;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+};
+
+constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
+constexpr int PTC_POISON = 8;  // items whose notes of values that are not finite are kept (the ring runs ahead of the rows)
+
+template <int D, int CODE, bool F16>
+__global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
+    k_tree_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+              const __grid_constant__ PrArgs a, const void* vcache, int64_t s_block, int64_t s_page, int64_t s_head) {
+  using C = PtcCfg<D, CODE>;
+  constexpr bool Q8 = C::Q8;
+  constexpr bool MF16 = Q8 || F16;
+  constexpr int ESZ = Q8 ? 1 : 2;
+  constexpr int TM_S = 0, TM_O = 256;
+  extern __shared__ uint8_t pr_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + C::Q_BYTES;
+  uint8_t* raw = ring + C::SLOTS * C::SLOT;
+  int* tpage = reinterpret_cast<int*>(raw + C::RAWS * C::RAW);      // [GROUPS] the producer's page table
+  float* sscale = reinterpret_cast<float*>(tpage + C::GROUPS);      // [SCALE_BLOCKS][128 of keys, 128 of values]
+  float* sfac = sscale + (Q8 ? C::SCALE_BLOCKS * 256 : 0);          // [128] 8-bit: score factors of the rows
+  float* sm = reinterpret_cast<float*>(smem);                       // [2][128] at a segment's end, over the queries
+  float* sl = sm + 256;                                             // [2][128]
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sfac + (Q8 ? 128 : 0));
+  uint64_t* full_bar = bar;             // [8] 16-bit slots
+  uint64_t* empty_bar = bar + 8;        // [8]
+  uint64_t* rfull_bar = bar + 16;       // [8] slots of codes
+  uint64_t* rempty_bar = bar + 24;      // [8]
+  uint64_t* s_bar = bar + 32;           // [2]
+  uint64_t* p_bar = bar + 34;           // [2]
+  uint64_t* q_bar = bar + 36;
+  uint64_t* o_bar = bar + 37;
+  uint64_t* end_bar = bar + 38;
+  uint64_t* done_bar = bar + 39;
+  uint64_t* ask_bar = bar + 40;         // [PTC_EDGES] by number of the edge block: its values' loads have been issued
+  uint64_t* fix_bar = bar + 48;         // [PTC_EDGES] they have been looked at
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 56);
+  volatile int* sfail = reinterpret_cast<int*>(tmem_slot + 1);  // [2] a wait ran out: softmax warps, converters
+  uint32_t* sgood = tmem_slot + 3;      // [8] by block: groups whose page exists
+  uint32_t* poison = sgood + 8;         // [PTC_POISON][8]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+  if (tid == 0) {
+    sfail[0] = sfail[1] = 0;
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(full_bar + i, Q8 ? 128 : 1);
+      mbar_init(empty_bar + i, 1);
+      mbar_init(rfull_bar + i, 33);  // every producer lane's copies of scales, and the codes
+      mbar_init(rempty_bar + i, 128);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_bar + i, 1);
+      mbar_init(p_bar + i, 128);
+    }
+    for (int i = 0; i < PTC_EDGES; ++i) {
+      mbar_init(ask_bar + i, 1);
+      mbar_init(fix_bar + i, 32);
+    }
+    mbar_init(done_bar, 1);
+    mbar_init(q_bar, 256);
+    mbar_init(o_bar, 1);
+    mbar_init(end_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  PrWalk<true> walk;
+  // item `it`: everything the roles need; false: no such item
+  int it = blockIdx.x, b, first, T, L, g, s, row0, R, start, end, ctx, nblk, jedge;
+  auto next = [&]() {
+    int rem;
+    if (!walk.find(a, 128, it, b, first, T, L, rem)) return false;
+    it += gridDim.x;
+    R = T * a.G;
+    const int tiles = (R + 127) / 128;
+    row0 = rem % tiles * 128;
+    g = rem / tiles % a.KV;
+    s = rem / (tiles * a.KV);
+    const int keys = pr_keys(a, L), seg = pr_segment_many(keys);
+    start = s * seg;
+    end = min(keys, start + seg);
+    ctx = L - T;
+    nblk = max(0, end - start + 127) >> 7;
+    jedge = min(max(min(ctx, end) - start, 0) >> 7, nblk);  // blocks before it are seen by every row
+    return true;
+  };
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------------------------------------ producer
+    const int group = 1 << a.group_log2, per = 128 >> a.group_log2;
+    int slot = 0, made = 0;
+    uint32_t ph = 1, blocks = 0, edges = 0;  // blocks, edge blocks of all items so far
+    uint64_t* fulls = Q8 ? rfull_bar : full_bar;
+    uint64_t* empties = Q8 ? rempty_bar : empty_bar;
+    constexpr int SLOTS = Q8 ? C::RAWS : C::SLOTS;
+    bool ok = true;
+    while (ok && next()) {
+      for (int i = lane; i < (end - start + group - 1) / group; i += 32) {
+        const int key = start + i * group;
+        tpage[i] = a.bt[(int64_t)b * a.sbt + key / a.BS];
+      }
+      __syncwarp();
+      auto load = [&](const CUtensorMap* m, int j, bool is_k) {
+        const int gi = j * per + lane;
+        int page = -1, off = 0;
+        if (lane < per && start + gi * group < end) {
+          page = tpage[gi];
+          off = (start + gi * group) % a.BS;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, lane < per && start + gi * group < end);
+        const unsigned good = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
+        for (int p = 0; p < C::PARTS && ok; ++p) {
+          ok = mbar_wait(empties + slot, ph, EX_DEVERR_WAIT_SLOT);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          uint8_t* dst = Q8 ? raw + slot * C::RAW : ring + slot * C::SLOT;
+          constexpr int PITCH = C::SW * ESZ < 128 ? C::SW * ESZ : 128;  // bytes of a box row
+          constexpr int NB = C::SW * ESZ / PITCH;
+          if (good != there) {  // tokens on pages that do not exist: zeros
+            for (int i = 0; i < per; ++i) {
+              if (!((there & ~good) >> i & 1)) continue;
+              for (int c = lane; c < NB * group * PITCH / 16; c += 32) {
+                const int n = c / (group * PITCH / 16), x = c % (group * PITCH / 16);
+                *reinterpret_cast<uint4*>(dst + n * 128 * PITCH + i * group * PITCH + x * 16) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+          }
+          if (lane == 0) {
+            if (is_k) sgood[(blocks + j) & 7] = good;
+            mbar_arrive_expect_tx(fulls + slot, (uint32_t)(__popc(good) * group * C::SW * ESZ));
+          }
+          __syncwarp();
+          if ((good >> lane) & 1u) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+              tma_load_4d(dst + n * 128 * PITCH + lane * group * PITCH, m, fulls + slot, (p * C::SW * ESZ + n * PITCH) / ESZ, g,
+                          off, page);
+          }
+          if constexpr (Q8) {
+            if (is_k && p == 0) {  // both scales come with the keys: the weights need them before the values
+              float* ss = sscale + ((blocks + j) & (C::SCALE_BLOCKS - 1)) * 256 + lane * 4;
+              const int from = (lane * 4) >> a.group_log2;
+              const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
+              if ((good >> from) & 1u) {
+                const int64_t so = (int64_t)pg * a.ss_block + g * a.ss_head + po + ((lane * 4) & (group - 1));
+                cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
+                cp_async16(ex_smem_u32(ss + 128), a.v_scale + so, true);
+              }
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(fulls + slot)) : "memory");
+          }
+          ++made;
+          if (++slot == SLOTS) slot = 0, ph ^= 1;
+        }
+      };
+      for (int j = 0; j < min(2, nblk); ++j) load(&tm_k, j, true);
+      for (int j = 0; j < nblk && ok; ++j) {
+        load(&tm_v, j, false);
+        if (!Q8 && j >= jedge) {
+          if (ok && lane == 0) mbar_arrive(ask_bar + (edges & (PTC_EDGES - 1)));
+          ++edges;
+        }
+        if (j + 2 < nblk && ok) load(&tm_k, j + 2, true);
+      }
+      blocks += nblk;
+      __syncwarp();
+    }
+    // every load has landed before the CTA ends (also after a wait that ran out)
+    for (int i = max(0, made - SLOTS); i < made; ++i)
+      mbar_wait(fulls + i % SLOTS, (uint32_t)(i / SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------------------------------------ products
+    constexpr uint32_t id_s = make_idesc_16(128, 128, MF16, false), id_o = make_idesc_16(128, C::SW, MF16, true);
+    const uint32_t sq = ex_smem_u32(smem), sr = ex_smem_u32(ring);
+    int slot = 0;
+    uint32_t ph = 0, php[2] = {0, 0}, phq = 0, edges = 0;
+    bool ok = true;
+    while (ok && next()) {  // (the whole warp walks; lane 0 issues)
+      if (nblk == 0) continue;
+      if (lane == 0) {
+        ok = mbar_wait(q_bar, phq, EX_DEVERR_WAIT_TMEM);
+        auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1; };
+        auto s_of = [&](int j) {
+#pragma unroll
+          for (int p = 0; p < C::PARTS; ++p) {
+            if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
+            if (!ok) return;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < C::SW / 64; ++x) {
+              const uint64_t da = make_sw128_desc(sq + (p * (C::SW / 64) + x) * C::SUB);
+              const uint64_t db = make_sw128_desc(sr + slot * C::SLOT + x * C::SUB);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc_mma_16(tmem + TM_S + (j & 1) * 128, da + 2 * k, db + 2 * k, id_s, (p | x | k) != 0);
+            }
+            tc_commit(empty_bar + slot);
+            advance();
+          }
+          tc_commit(s_bar + (j & 1));
+        };
+        s_of(0);
+        if (nblk > 1) s_of(1);
+        for (int j = 0; j < nblk && ok; ++j) {
+          if (!Q8 && j >= jedge) {
+            ok = mbar_wait(fix_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_MMA);
+            ++edges;
+          }
+          if (ok) ok = mbar_wait(p_bar + (j & 1), php[j & 1], EX_DEVERR_WAIT_TMEM);
+          php[j & 1] ^= 1;
+#pragma unroll
+          for (int p = 0; p < C::PARTS; ++p) {
+            if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t db = make_sw128_desc_n(sr + slot * C::SLOT, C::SUB);
+            const uint32_t d = tmem + TM_O + (C::STREAMS == 2 ? (j & 1) * D : p * C::SW);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              tc_mma_16_ta(d, tmem + TM_S + (j & 1) * 128 + k * 8, db + k * (2048 >> 4), id_o,
+                           (j >= C::STREAMS || k > 0) ? 1u : 0u);
+            tc_commit(empty_bar + slot);
+            advance();
+          }
+          if (C::STREAMS == 1 && ok) tc_commit(o_bar);
+          if (j + 2 < nblk && ok) s_of(j + 2);
+        }
+        if (ok) tc_commit(end_bar);
+        phq ^= 1;
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    // every product is done before tensor memory is given back
+    if (lane == 0) {
+      tc_commit(done_bar);
+      mbar_wait(done_bar, 0, EX_DEVERR_WAIT_MMA);
+    }
+    __syncwarp();
+  } else if (warp == 10 && !Q8) {
+    // ---------------------------------------------------------------------------------------------- edge values
+    int base = 0;   // slots of the items before
+    uint32_t edges = 0;
+    int item = 0;
+    bool ok = true;
+    while (ok && next()) {
+      uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
+      if (jedge < nblk) {
+        if (lane < 8) mine[lane] = 0;
+        __syncwarp();
+      }
+      for (int j = jedge; j < nblk && ok; ++j) {
+        const int e = j - jedge;
+        // the producer's word that the slots are this block's
+        ok = mbar_wait(ask_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_SLOT);
+        for (int p = 0; p < C::PARTS && ok; ++p) {
+          const int at = base + (min(j + 2, nblk) + j) * C::PARTS + p;  // in the order of loading
+          uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
+          ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
+          ok = __all_sync(0xffffffffu, ok);
+          for (int r = lane; r < 128 && ok; r += 32) {
+            const int key = start + j * 128 + r;
+            bool bad = false;
+            for (int c = 0; c < C::SW / 8; ++c) {
+              uint4* x = reinterpret_cast<uint4*>(vs + (c >> 3) * C::SUB + r * 128 + (c & 7) * 16);
+              if (key >= end) {
+                *x = make_uint4(0, 0, 0, 0);
+              } else {
+                const uint4 w = *x;
+                if (!(finite_word<F16>(w.x) && finite_word<F16>(w.y) && finite_word<F16>(w.z) && finite_word<F16>(w.w))) {
+                  bad = true;
+                  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
+                    if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
+                  }
+                  *x = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+              }
+            }
+            if (bad) atomicOr(mine + e * 4 + (r >> 5), 1u << (r & 31));
+          }
+        }
+        fence_proxy_async_shared();  // the products read shared memory through the async proxy
+        if (ok) mbar_arrive(fix_bar + (edges & (PTC_EDGES - 1)));
+        ++edges;
+      }
+      base += 2 * nblk * C::PARTS;
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------------------------------------ converters
+    if constexpr (Q8) {
+      const int t = tid - 384;
+      int rslot = 0, slot = 0;
+      uint32_t rph = 0, ph = 1;
+      bool ok = true;
+      while (ok && next()) {
+        auto convert = [&](int j, bool is_v) {
+          for (int p = 0; p < C::PARTS && ok; ++p) {
+            if (!mbar_wait(rfull_bar + rslot, rph, EX_DEVERR_WAIT_TMA) || !mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT))
+              sfail[1] = 1;
+            asm volatile("bar.sync 3, 128;" ::: "memory");
+            if (sfail[1]) {  // the same for every thread here: the flag is only set before the barrier
+              ok = false;
+              return;
+            }
+            const uint8_t* src = raw + rslot * C::RAW;
+            uint8_t* dst = ring + slot * C::SLOT;
+            constexpr int CH = C::SW / 16;  // 16-byte chunks of codes of a key
+#pragma unroll 4
+            for (int i = t; i < 128 * CH; i += 128) {
+              const int r = i / CH, c = i % CH;
+              uint4 w = *reinterpret_cast<const uint4*>(
+                  src + (C::SW == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4)));
+              if (is_v && start + j * 128 + r >= end) w = make_uint4(0, 0, 0, 0);
+              uint32_t o[8];
+              codes_to_f16<CODE>(w.x, o[0], o[1]);
+              codes_to_f16<CODE>(w.y, o[2], o[3]);
+              codes_to_f16<CODE>(w.z, o[4], o[5]);
+              codes_to_f16<CODE>(w.w, o[6], o[7]);
+              uint8_t* d = dst + (c >> 2) * C::SUB + r * 128;
+              const int c2 = (c & 3) * 2;
+              *reinterpret_cast<uint4*>(d + ((c2 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(d + (((c2 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            fence_proxy_async_shared();
+            mbar_arrive(full_bar + slot);
+            mbar_arrive(rempty_bar + rslot);
+            if (++rslot == C::RAWS) rslot = 0, rph ^= 1;
+            if (++slot == C::SLOTS) slot = 0, ph ^= 1;
+          }
+        };
+        for (int j = 0; j < min(2, nblk); ++j) convert(j, false);
+        for (int j = 0; j < nblk && ok; ++j) {
+          convert(j, true);
+          if (j + 2 < nblk && ok) convert(j + 2, false);
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // -------------------------------------------------------------------------------------------------- softmax
+    const int wg = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t phs[2] = {0, 0}, pho = 0, phe = 0, blocks = 0;
+    int item = 0;
+    bool ok = true;
+    while (ok && next()) {
+      const uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
+      const bool active = row0 + (warp & 3) * 32 < R;  // some row of this warp is real
+      float m = -INFINITY, l = 0.0f, vref = 0.0f;
+      if (nblk > 0) {
+        // queries: row-major in swizzled columns of 64 dims; D/8 lanes a row
+        constexpr int LANES = D / 8;
+        const int c = tid % LANES;
+        for (int x = tid / LANES; x < 128; x += 256 / LANES) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (row0 + x < R) {
+            const int t = (row0 + x) / a.G, h = (row0 + x) % a.G;
+            v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + t) * a.sq_t +
+                                                (int64_t)(g * a.G + h) * a.sq_h + c * 8);
+          }
+          if constexpr (Q8) {
+            float f = 1.0f;
+            if (!a.q_is_f16) {
+              float y[8];
+              unpack2<__nv_bfloat16>(v.x, y[0], y[1]);
+              unpack2<__nv_bfloat16>(v.y, y[2], y[3]);
+              unpack2<__nv_bfloat16>(v.z, y[4], y[5]);
+              unpack2<__nv_bfloat16>(v.w, y[6], y[7]);
+              float mq = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) mq = fmaxf(mq, fabsf(y[i]));
+#pragma unroll
+              for (int o = LANES / 2; o; o >>= 1) mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, o));
+              const float inv = pr_query_scale(mq, f);
+              v.x = pack2<__half>(y[0] * inv, y[1] * inv);
+              v.y = pack2<__half>(y[2] * inv, y[3] * inv);
+              v.z = pack2<__half>(y[4] * inv, y[5] * inv);
+              v.w = pack2<__half>(y[6] * inv, y[7] * inv);
+            }
+            if (c == 0) sfac[x] = f * a.scale_log2;
+          }
+          *reinterpret_cast<uint4*>(smem + (c >> 3) * C::SUB + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
+        }
+        fence_proxy_async_shared();
+        tc_fence_before();  // the last item's O has been read
+        mbar_arrive(q_bar);
+        if constexpr (Q8) asm volatile("bar.sync 2, 256;" ::: "memory");  // sfac
+      }
+      const float fac = Q8 ? sfac[r] : a.scale_log2;
+      uint64_t word = 0;
+      if (row0 + r < R) {
+        const int t = (row0 + r) / a.G;
+        word = (a.mask ? a.mask[first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - T));  // (T >= 1)
+      }
+      const uint32_t all_good = (uint32_t)((1ull << (128 >> a.group_log2)) - 1ull);
+      for (int j = (C::STREAMS == 2 ? wg : 0); j < (C::STREAMS == 2 || wg == 0 ? nblk : 0); j += C::STREAMS) {
+        const int buf = j & 1;
+        if (!mbar_wait(s_bar + buf, phs[buf], EX_DEVERR_WAIT_MMA)) *sfail = 1;
+        phs[buf] ^= 1;
+        __syncwarp();
+        tc_fence_after();
+        if (active) {
+          const uint32_t s_addr = tmem + lanes + TM_S + buf * 128;
+          const uint32_t o_addr = tmem + lanes + TM_O + (C::STREAMS == 2 ? wg * D : 0);
+          const int kb = start + j * 128;
+          const uint32_t good = sgood[(blocks + j) & 7];
+          const float* ks = sscale + ((blocks + j) & (C::SCALE_BLOCKS - 1)) * 256;
+          const bool whole = j < jedge && good == all_good;
+          uint32_t vis[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            vis[q] = ~0u;
+            if (!whole) {
+              const int at = kb + 32 * q, d = at - ctx;  // drafted token of the chunk's first column
+              uint32_t v = d >= 64 ? 0u : d >= 0 ? (uint32_t)(word >> d) : d > -32 ? (uint32_t)(word << -d) | ((1u << -d) - 1u) : ~0u;
+              const int left = end - at;
+              if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
+              uint32_t pages = 0;
+              for (int i = 0; i < 32 >> a.group_log2; ++i)
+                if ((good >> ((32 * q >> a.group_log2) + i)) & 1u) pages |= ((1u << (1 << a.group_log2)) - 1u) << (i << a.group_log2);
+              vis[q] = v & pages;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t u[32];
+            tmem_ld32(s_addr + q * 32, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 kv = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+              if constexpr (Q8) kv = *reinterpret_cast<const float4*>(ks + q * 32 + i);
+              const float x[4] = {__uint_as_float(u[i]) * kv.x, __uint_as_float(u[i + 1]) * kv.y, __uint_as_float(u[i + 2]) * kv.z,
+                                  __uint_as_float(u[i + 3]) * kv.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], ((vis[q] >> (i + k)) & 1u) ? x[k] * fac : -INFINITY);
+            }
+          }
+          const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          float vmax = 0.0f;
+          if constexpr (Q8) {  // the largest finite value scale of the block's readable keys: lane l looks at 4 l ..
+            const float4 v = *reinterpret_cast<const float4*>(ks + 128 + lane * 4);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (kb + lane * 4 + k < end && ((good >> ((lane * 4 + k) >> a.group_log2)) & 1u) && x[k] < INFINITY) vmax = fmaxf(vmax, x[k]);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+          }
+          const bool take = mb > m + 8.0f;  // (m = -inf: any finite score)
+          const bool vtake = Q8 && vmax > 64.0f * vref;
+          if (__any_sync(0xffffffffu, take) || vtake) {
+            const float mn = take ? mb : m;
+            float al = m == -INFINITY ? 0.0f : ex2(m - mn);
+            if (m == -INFINITY && mn == -INFINITY) al = 1.0f;
+            m = mn;
+            l *= al;
+            if (vtake) {
+              if (vmax >= 1.2e-38f) al *= __fdividef(vref, vmax);
+              vref = vmax;
+            }
+            if (j >= C::STREAMS) {
+              // the last product on this O is done: it was issued before this S (D = 256: after it)
+              if (C::STREAMS == 1) {
+                if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
+                __syncwarp();
+                tc_fence_after();
+              }
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                tmem_st32(o_addr + c, o);
+              }
+            }
+          }
+          const float sub = m == -INFINITY ? 0.0f : m;
+          const float vinv = Q8 && vref >= 1.2e-38f ? __frcp_rn(vref) : 0.0f;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t u[32], p[16];
+            tmem_ld32(s_addr + q * 32, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 kv = make_float4(1.0f, 1.0f, 1.0f, 1.0f), vv = kv;
+              if constexpr (Q8) {
+                kv = *reinterpret_cast<const float4*>(ks + q * 32 + i);
+                vv = *reinterpret_cast<const float4*>(ks + 128 + q * 32 + i);
+              }
+              const float kvx[4] = {kv.x, kv.y, kv.z, kv.w}, vvx[4] = {vv.x, vv.y, vv.z, vv.w};
+              float w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float x = Q8 ? __uint_as_float(u[i + k]) * kvx[k] * fac - sub : __fmaf_rn(__uint_as_float(u[i + k]), fac, -sub);
+                const bool see = (vis[q] >> (i + k)) & 1u;
+                w[k] = see ? ex2(x) : 0.0f;
+                sum[k] += w[k];
+                if constexpr (Q8) w[k] = see ? w[k] * (vvx[k] * vinv) : 0.0f;
+              }
+              p[i / 2] = MF16 ? pack2<__half>(w[0], w[1]) : pack_bf16(w[0], w[1]);
+              p[i / 2 + 1] = MF16 ? pack2<__half>(w[2], w[3]) : pack_bf16(w[2], w[3]);
+            }
+            // 16 columns of weights over scores of the same or an earlier chunk, which have been read
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                "%14, %15};" ::EX_I8(p, 0),
+                EX_I8(p, 8), "r"(s_addr + q * 16)
+                : "memory");
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(p_bar + buf);
+      }
+      // the streams and, of each row, the two halves of the head dimension: one for each four warps
+      if (nblk > 0 && !mbar_wait(end_bar, phe, EX_DEVERR_WAIT_MMA)) *sfail = 1;
+      if (nblk > 0) phe ^= 1;
+      sm[wg * 128 + r] = m;
+      sl[wg * 128 + r] = l;
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
+      tc_fence_after();
+      pho += nblk;
+      blocks += nblk;
+      if (!active) vref = 0.0f;
+      float f[2], lall = 0.0f;
+      const float m0 = sm[r], m1 = C::STREAMS == 2 ? sm[128 + r] : -INFINITY;
+      const float mall = fmaxf(m0, m1), sub = mall == -INFINITY ? 0.0f : mall;
+      f[0] = m0 == -INFINITY ? 0.0f : ex2(m0 - sub);
+      f[1] = m1 == -INFINITY ? 0.0f : ex2(m1 - sub);
+      lall = sl[r] * f[0] + (C::STREAMS == 2 ? sl[128 + r] * f[1] : 0.0f);
+      if constexpr (Q8) {
+        // the reference of each stream's value scales
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        sm[wg * 128 + r] = vref;
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        f[0] *= sm[r];
+        if (C::STREAMS == 2) f[1] *= sm[128 + r];
+      }
+      const bool have1 = C::STREAMS == 2 && nblk > 1;
+      const bool single = pr_segments_many(pr_keys(a, L)) == 1;
+      const bool edges = !Q8 && jedge < nblk;
+      bool any = false;
+      if (edges)
+        for (int i = 0; i < 8; ++i) any |= mine[i] != 0;
+      if (active) {
+        const bool real = row0 + r < R;
+        const int t = real ? (row0 + r) / a.G : 0, h = g * a.G + (real ? (row0 + r) % a.G : 0);
+        const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
+        const int64_t pi = ((int64_t)(first + t) * a.H + h) * a.NS + s;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t + (int64_t)h * a.so_h;
+#pragma unroll 1
+        for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
+          uint32_t u[32];
+          float o[32];
+          __syncwarp();
+          if (nblk > 0) {
+            tmem_ld32(tmem + lanes + TM_O + c, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
+          if (have1) {
+            tmem_ld32(tmem + lanes + TM_O + D + c, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[1];
+          }
+          if (any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
+#pragma unroll 1
+            for (int k = 0; k < 256; ++k) {
+              if (!((mine[k >> 5] >> (k & 31)) & 1u)) continue;
+              const int key = start + jedge * 128 + k, d = key - ctx;
+              if (!real || key >= end || (d >= 0 && !((word >> d) & 1ull))) continue;
+              const int page = a.bt[(int64_t)b * a.sbt + key / a.BS];
+              if (page < 0 || page >= a.blocks) continue;
+              const uint16_t* v = reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
+                                  (int64_t)(key % a.BS) * s_page + (int64_t)g * s_head + c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float x = F16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
+                if (!(fabsf(x) < INFINITY)) o[i] += x;
+              }
+            }
+            __syncwarp();
+          }
+          if (real && single) {
+            const bool f16 = Q8 ? a.q_is_f16 != 0 : F16;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              *reinterpret_cast<uint32_t*>(dst + c + i) = f16 ? pack2<__half>(o[i] * inv, o[i + 1] * inv) : pack_bf16(o[i] * inv, o[i + 1] * inv);
+          } else if (real) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(a.ws_acc + pi * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+        if (real && !single && wg == 0) {
+          a.ws_m[pi] = mall;
+          a.ws_l[pi] = lall;
+        }
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // before sm, sl and sfac are written again
+    }
+    __syncwarp();
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace ex
