@@ -278,27 +278,36 @@ bool misaligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t
 bool half_dtype(int d) { return d == EX_DTYPE_BF16 || d == EX_DTYPE_F16; }
 bool head_size_ok(int D) { return D == 64 || D == 128 || D == 256; }
 
-// One launch of a kernel that takes dynamic shared memory, the attribute set once per device.
+// One launch of a kernel that takes dynamic shared memory, the attribute set once per device. regs > 0: its warps share out
+// the registers of the launch and count on this many a thread (else cudaErrorNotSupported).
+struct KernelReady {
+  signed char dev[128] = {};  // 1: ready, -1: other registers than planned
+};
 template <typename K, typename... Args>
-cudaError_t launch_smem(K kernel, bool (&done)[128], int grid, int threads, int smem, cudaStream_t st, const Args&... args) {
+cudaError_t launch_smem(K kernel, KernelReady& ready, int regs, dim3 grid, int threads, int smem, cudaStream_t st,
+                        const Args&... args) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 128 || !done[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (dev < 128) done[dev] = true;
+  if (dev >= 128) return cudaErrorNotSupported;
+  if (ready.dev[dev] == 0) {
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, kernel)) != cudaSuccess) return e;
+    ready.dev[dev] = regs > 0 && fa.numRegs != regs ? -1 : 1;
   }
-  return ex_launch_pdl(kernel, dim3(grid), dim3(threads), smem, st, args...);
+  if (ready.dev[dev] < 0) return cudaErrorNotSupported;
+  return ex_launch_pdl(kernel, grid, dim3(threads), smem, st, args...);
 }
+int rows_status(cudaError_t e) { return e == cudaErrorNotSupported ? EX_ERR_UNSUPPORTED : cuda_status(e); }
 
 template <int D, int CODE, bool F16, int NT>
 cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex::PrArgs& a, int64_t items,
                          cudaStream_t st) {
   using C = ex::PfCfg<D, CODE, NT>;
-  static bool done[128] = {};
+  static KernelReady ready;
   const int grid = (int)std::min<int64_t>(items, num_sms());
-  return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, done, grid, 32 * C::NW, C::SMEM, st, mk, mv, a);
+  return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, ready, 0, dim3(grid), 32 * C::NW, C::SMEM, st, mk, mv, a);
 }
 
 struct CacheStrides {
@@ -319,9 +328,10 @@ cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& m
   a.rows_lo = ex::PR_FEW;
   a.rows_hi = INT32_MAX;
   using C = ex::PtcCfg<D, CODE>;
-  static bool done[128] = {};
+  static KernelReady ready;
   const int grid = (int)std::min<int64_t>(per_tile * cdiv(rows, 128), num_sms());
-  return launch_smem(ex::k_tree_tc<D, CODE, F16>, done, grid, C::THREADS, C::SMEM, st, mk, mv, a, c.v, c.block, c.page, c.head);
+  return launch_smem(ex::k_tree_tc<D, CODE, F16>, ready, C::REGS, dim3(grid), C::THREADS, C::SMEM, st, mk, mv, a, c.v,
+                     c.block, c.page, c.head);
 }
 
 template <int D>
@@ -398,7 +408,7 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
   else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
   else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
-  return cuda_status(e);
+  return rows_status(e);
 }
 
 // 3-D tensor map over packed rows (D, heads, rows): boxes of 128 rows of one head, 64 dims wide.
@@ -417,23 +427,11 @@ bool encode_packed_map(CUtensorMap* map, const void* base, int D, int heads, int
 template <int D, bool F16>
 int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, ex::PaArgs a, cudaStream_t st) {
   using C = ex::PaCfg<D>;
-  static int ready[128] = {};  // per device: 1 = the kernel can run as planned, -1 = it cannot
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_status(e);
-  if (dev >= 128) return EX_ERR_UNSUPPORTED;
-  if (ready[dev] == 0) {
-    e = cudaFuncSetAttribute(ex::k_prompt_attn<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return cuda_status(e);
-    cudaFuncAttributes fa;
-    if ((e = cudaFuncGetAttributes(&fa, ex::k_prompt_attn<D, F16>)) != cudaSuccess) return cuda_status(e);
-    ready[dev] = fa.numRegs == ex::PA_REGS_LAUNCH ? 1 : -1;  // the warps share out the registers of the launch
-  }
-  if (ready[dev] < 0) return EX_ERR_UNSUPPORTED;
+  static KernelReady ready;
   a.tiles = (int)(cdiv(a.tokens, C::ROWS) + a.n);  // at least as many as there are
   if ((int64_t)a.tiles * a.H > INT32_MAX) return EX_ERR_UNSUPPORTED;
-  return cuda_status(ex_launch_pdl(ex::k_prompt_attn<D, F16>, dim3((unsigned)(a.tiles * a.H)), dim3(ex::PA_THREADS),
-                                   C::SMEM, st, mq, mk, mv, a));
+  return rows_status(launch_smem(ex::k_prompt_attn<D, F16>, ready, ex::PA_REGS_LAUNCH, dim3((unsigned)(a.tiles * a.H)),
+                                 ex::PA_THREADS, C::SMEM, st, mq, mk, mv, a));
 }
 
 template <int D, int CODE>

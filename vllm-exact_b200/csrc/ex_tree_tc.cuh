@@ -6,12 +6,17 @@
 // from. D <= 128: blocks alternate between two streams, each with its own S, O, m and l and its own four softmax warps, so
 // that one stream's softmax runs beside the other's products; the streams are added up at the end of the segment.
 // D = 256: one O, two S buffers.
-//   warps 0-3, 4-7  softmax, one row a thread (they also bring Q to shared memory and write the results)
+//   warps 0-3, 4-7  softmax (they also bring Q to shared memory and write the results). A thread has one row of the tile and,
+//                   where the request has at most 64 (32) rows, 64 (32) of the block's keys: Q is then there two (four)
+//                   times, every copy weighs its own keys and has zeros for the others, and the copies are added up
+//                   at the end. A row's exponentials are what takes longest, and this spreads them over all schedulers.
 //   warp 8          issues the products
-//   warp 9          producer: TMA boxes of 8 or 16 tokens through the block table into a ring of slots
+//   warps 12-15, for codes 9-11   producers: TMA boxes of 8 or 16 tokens through the block table into a ring of slots. Issuing
+//                   a box takes a warp about 75 cycles (its operands are uniform registers), 16 boxes of a 32 KB tile longer
+//                   than HBM takes to deliver it: so several warps share the boxes of every tile.
 //   warp 10         16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
 //                   are not finite are zeroed and noted, and added in the end to the rows that see them
-//   warps 12-15     8-bit: codes to float16 tiles (exact; keys behind the end to zeros)
+//   warps 12-15     for codes: codes to float16 tiles (exact; keys behind the end to zeros)
 // Bound by reading the cache once: a block of 128 keys of a 16-bit cache is 64 KB (D = 128), 1.5 us of an SM's share of HBM;
 // its products take 0.55 us and the 128 exponentials of a row 0.55 us on every scheduler that has rows.
 #pragma once
@@ -24,7 +29,11 @@ template <int D, int CODE>
 struct PtcCfg {
   static constexpr bool Q8 = CODE != CODE_NONE;
   static constexpr int STREAMS = D == 256 ? 1 : 2;
-  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr int THREADS = 512;
+  static constexpr int FEEDERS = Q8 ? 3 : 4;         // producer warps
+  // registers a thread: at launch, of the softmax warps and of the others, which give theirs up
+  static constexpr int REGS = 128, REGS_SOFTMAX = 168, REGS_OTHER = 88;
+  static_assert(256 * REGS_SOFTMAX + (THREADS - 256) * REGS_OTHER <= THREADS * REGS, "register shares");
   static constexpr int SW = D < 128 ? D : 128;       // dims of a 16-bit slot
   static constexpr int PARTS = D / SW;               // slots of a block's K or V
   static constexpr int SUB = 128 * 128;              // 128 rows x 64 dims of 16 bits, one swizzled column
@@ -33,15 +42,86 @@ struct PtcCfg {
   static constexpr int RAW = Q8 ? 128 * SW : 0;      // bytes of a slot of codes: 128 keys, SW dims
   static constexpr int SLOTS = D == 64 ? (Q8 ? 6 : 8) : (Q8 ? 3 : 5);
   static constexpr int RAWS = !Q8 ? 0 : D == 64 ? 6 : D == 128 ? 5 : 3;  // slots of codes
-  static constexpr int GROUPS = 256;                 // page table entries of a segment (2048 keys, boxes of 8)
   // Blocks whose scales and pages are kept. While block j's weights are made, its values are the first tile not used up:
   // number 2 j + 2 in the order K0 K1 V0 K2 V1 .. of loading. The rings hold SLOTS + RAWS more, keys of block m being number
   // 2 m - 1: m < j + 8 as long as they are at most 13.
   static constexpr int SCALE_BLOCKS = 8;
   static_assert((SLOTS + RAWS) / PARTS <= 13, "blocks ahead");
-  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + GROUPS * 4 + (Q8 ? SCALE_BLOCKS * 1024 + 512 : 0) + 768;
+  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + (Q8 ? SCALE_BLOCKS * 1024 + 512 : 0) + 768;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
+
+// One row's part of a block: `chunks` times 32 columns of S from s_addr on, their weights (over S, from p_addr on) in 16 bits.
+// see(q): the columns of chunk q that are seen, if MASKED. update(x): brings m, l and O up to date with the part's largest
+// score. The scores are read twice rather than kept: the loops stay small, and with many warps in different places
+// fetching instructions is what costs.
+template <bool Q8, bool MF16, bool MASKED, typename See, typename Update>
+__device__ __forceinline__ void ptc_weigh(uint32_t s_addr, uint32_t p_addr, int chunks, const float* ks, float fac, float& m,
+                                          float& l, float& vinv, See see, Update update) {
+  float x[32];
+  auto take = [&](int q) {
+    tmem_ld32(s_addr + q * 32, reinterpret_cast<uint32_t*>(x));
+    tmem_ld_wait();
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(ks + q * 32 + i);
+        x[i] *= k.x;
+        x[i + 1] *= k.y;
+        x[i + 2] *= k.z;
+        x[i + 3] *= k.w;
+      }
+    }
+    uint32_t v = ~0u;
+    if constexpr (MASKED) {
+      v = see(q);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (!((v >> i) & 1u)) x[i] = -INFINITY;
+    }
+    return v;
+  };
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int q = 0; q < chunks; ++q) {
+    take(q);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+  }
+  update(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
+  const float sub = m == -INFINITY ? 0.0f : m;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int q = 0; q < chunks; ++q) {
+    const uint32_t seen = take(q);
+    uint32_t p[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] = ex2(__fmaf_rn(x[i + k], fac, -sub));
+        sum[k] += w[k];
+      }
+      if constexpr (Q8) {
+        const float4 v = *reinterpret_cast<const float4*>(ks + 128 + q * 32 + i);
+        w[0] *= v.x * vinv;
+        w[1] *= v.y * vinv;
+        w[2] *= v.z * vinv;
+        w[3] *= v.w * vinv;
+        if constexpr (MASKED) {  // a key that is not seen has a scale that may be anything
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (!((seen >> (i + k)) & 1u)) w[k] = 0.0f;
+        }
+      }
+      p[i / 2] = MF16 ? pack2<__half>(w[0], w[1]) : pack_bf16(w[0], w[1]);
+      p[i / 2 + 1] = MF16 ? pack2<__half>(w[2], w[3]) : pack_bf16(w[2], w[3]);
+    }
+    tmem_st16(p_addr + q * 16, p);  // over scores of the same or an earlier chunk, which have been read
+  }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
 
 constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
 constexpr int PTC_POISON = 8;  // items whose notes of values that are not finite are kept (the ring runs ahead of the rows)
@@ -55,15 +135,13 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   constexpr bool MF16 = Q8 || F16;
   constexpr int ESZ = Q8 ? 1 : 2;
   constexpr int TM_S = 0, TM_O = 256;
+  constexpr int CD = D == 64 ? 16 : 32;  // dims of a piece of the results: two pieces of 128 rows fit where Q was
   extern __shared__ uint8_t pr_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + C::Q_BYTES;
   uint8_t* raw = ring + C::SLOTS * C::SLOT;
-  int* tpage = reinterpret_cast<int*>(raw + C::RAWS * C::RAW);      // [GROUPS] the producer's page table
-  float* sscale = reinterpret_cast<float*>(tpage + C::GROUPS);      // [SCALE_BLOCKS][128 of keys, 128 of values]
+  float* sscale = reinterpret_cast<float*>(raw + C::RAWS * C::RAW);  // [SCALE_BLOCKS][128 of keys, 128 of values]
   float* sfac = sscale + (Q8 ? C::SCALE_BLOCKS * 256 : 0);          // [128] 8-bit: score factors of the rows
-  float* sm = reinterpret_cast<float*>(smem);                       // [2][128] at a segment's end, over the queries
-  float* sl = sm + 256;                                             // [2][128]
   uint64_t* bar = reinterpret_cast<uint64_t*>(sfac + (Q8 ? 128 : 0));
   uint64_t* full_bar = bar;             // [8] 16-bit slots
   uint64_t* empty_bar = bar + 8;        // [8]
@@ -78,14 +156,14 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   uint64_t* ask_bar = bar + 40;         // [PTC_EDGES] by number of the edge block: its values' loads have been issued
   uint64_t* fix_bar = bar + 48;         // [PTC_EDGES] they have been looked at
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 56);
-  volatile int* sfail = reinterpret_cast<int*>(tmem_slot + 1);  // [2] a wait ran out: softmax warps, converters
+  volatile int* sfail = reinterpret_cast<int*>(tmem_slot + 1);  // a wait of the softmax warps ran out
   uint32_t* sgood = tmem_slot + 3;      // [8] by block: groups whose page exists
   uint32_t* poison = sgood + 8;         // [PTC_POISON][8]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   if (tid == 0) {
-    sfail[0] = sfail[1] = 0;
+    *sfail = 0;
     for (int i = 0; i < 8; ++i) {
       mbar_init(full_bar + i, Q8 ? 128 : 1);
       mbar_init(empty_bar + i, 1);
@@ -97,7 +175,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       mbar_init(p_bar + i, 128);
     }
     for (int i = 0; i < PTC_EDGES; ++i) {
-      mbar_init(ask_bar + i, 1);
+      mbar_init(ask_bar + i, C::FEEDERS);
       mbar_init(fix_bar + i, 32);
     }
     mbar_init(done_bar, 1);
@@ -137,84 +215,120 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     return true;
   };
 
-  if (warp == 9) {
-    // ------------------------------------------------------------------------------------------------ producer
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
+  constexpr int FEED0 = Q8 ? 9 : 12;
+  if (warp >= FEED0 && warp < FEED0 + C::FEEDERS) {
+    // ------------------------------------------------------------------------------------------------ producers
+    // Every producer follows all groups; it issues those of its own, the first one also announces each tile.
+    const int feeder = warp - FEED0;
     const int group = 1 << a.group_log2, per = 128 >> a.group_log2;
     int slot = 0, made = 0;
     uint32_t ph = 1, blocks = 0, edges = 0;  // blocks, edge blocks of all items so far
     uint64_t* fulls = Q8 ? rfull_bar : full_bar;
     uint64_t* empties = Q8 ? rempty_bar : empty_bar;
     constexpr int SLOTS = Q8 ? C::RAWS : C::SLOTS;
+    constexpr int PITCH = C::SW * ESZ < 128 ? C::SW * ESZ : 128;  // bytes of a box row
+    constexpr int NB = C::SW * ESZ / PITCH;
     bool ok = true;
     while (ok && next()) {
-      for (int i = lane; i < (end - start + group - 1) / group; i += 32) {
-        const int key = start + i * group;
-        tpage[i] = a.bt[(int64_t)b * a.sbt + key / a.BS];
-      }
-      __syncwarp();
-      auto load = [&](const CUtensorMap* m, int j, bool is_k) {
-        const int gi = j * per + lane;
-        int page = -1, off = 0;
-        if (lane < per && start + gi * group < end) {
-          page = tpage[gi];
-          off = (start + gi * group) % a.BS;
-        }
-        const unsigned there = __ballot_sync(0xffffffffu, lane < per && start + gi * group < end);
-        const unsigned good = __ballot_sync(0xffffffffu, page >= 0 && page < a.blocks);
+      // one tile (K or V) of a block whose group `lane` lies on `page` at `off`; bits of the groups there and of the good
+      auto load = [&](const CUtensorMap* m, int page, int off, uint32_t there, uint32_t good, bool is_k, uint32_t no) {
+#pragma unroll 1
         for (int p = 0; p < C::PARTS && ok; ++p) {
           ok = mbar_wait(empties + slot, ph, EX_DEVERR_WAIT_SLOT);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           uint8_t* dst = Q8 ? raw + slot * C::RAW : ring + slot * C::SLOT;
-          constexpr int PITCH = C::SW * ESZ < 128 ? C::SW * ESZ : 128;  // bytes of a box row
-          constexpr int NB = C::SW * ESZ / PITCH;
-          if (good != there) {  // tokens on pages that do not exist: zeros
-            for (int i = 0; i < per; ++i) {
-              if (!((there & ~good) >> i & 1)) continue;
-              for (int c = lane; c < NB * group * PITCH / 16; c += 32) {
-                const int n = c / (group * PITCH / 16), x = c % (group * PITCH / 16);
-                *reinterpret_cast<uint4*>(dst + n * 128 * PITCH + i * group * PITCH + x * 16) = make_uint4(0, 0, 0, 0);
+          if (feeder == 0) {
+            if (good != there) {  // tokens on pages that do not exist: zeros
+#pragma unroll 1
+              for (int i = 0; i < per; ++i) {
+                if (!((there & ~good) >> i & 1)) continue;
+#pragma unroll 1
+                for (int c = lane; c < NB * group * PITCH / 16; c += 32) {
+                  const int n = c / (group * PITCH / 16), x = c % (group * PITCH / 16);
+                  *reinterpret_cast<uint4*>(dst + n * 128 * PITCH + i * group * PITCH + x * 16) = make_uint4(0, 0, 0, 0);
+                }
               }
+              fence_proxy_async_shared();
+              __syncwarp();
             }
-            fence_proxy_async_shared();
-            __syncwarp();
+            if (lane == 0) {
+              if (is_k) sgood[no & 7] = good;
+              mbar_arrive_expect_tx(fulls + slot, (uint32_t)(__popc(good) * group * C::SW * ESZ));
+            }
           }
-          if (lane == 0) {
-            if (is_k) sgood[(blocks + j) & 7] = good;
-            mbar_arrive_expect_tx(fulls + slot, (uint32_t)(__popc(good) * group * C::SW * ESZ));
-          }
-          __syncwarp();
-          if ((good >> lane) & 1u) {
+          if (((good >> lane) & 1u) && lane % C::FEEDERS == feeder) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
               tma_load_4d(dst + n * 128 * PITCH + lane * group * PITCH, m, fulls + slot, (p * C::SW * ESZ + n * PITCH) / ESZ, g,
                           off, page);
           }
+          __syncwarp();
           if constexpr (Q8) {
-            if (is_k && p == 0) {  // both scales come with the keys: the weights need them before the values
-              float* ss = sscale + ((blocks + j) & (C::SCALE_BLOCKS - 1)) * 256 + lane * 4;
-              const int from = (lane * 4) >> a.group_log2;
-              const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
-              if ((good >> from) & 1u) {
-                const int64_t so = (int64_t)pg * a.ss_block + g * a.ss_head + po + ((lane * 4) & (group - 1));
-                cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
-                cp_async16(ex_smem_u32(ss + 128), a.v_scale + so, true);
+            if (feeder == C::FEEDERS - 1) {
+              if (is_k && p == 0) {  // both scales come with the keys: the weights need them before the values
+                float* ss = sscale + (no & (C::SCALE_BLOCKS - 1)) * 256 + lane * 4;
+                const int from = (lane * 4) >> a.group_log2;
+                const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
+                if ((good >> from) & 1u) {
+                  const int64_t so = (int64_t)pg * a.ss_block + g * a.ss_head + po + ((lane * 4) & (group - 1));
+                  cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
+                  cp_async16(ex_smem_u32(ss + 128), a.v_scale + so, true);
+                }
               }
+              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(fulls + slot)) : "memory");
             }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(fulls + slot)) : "memory");
           }
           ++made;
           if (++slot == SLOTS) slot = 0, ph ^= 1;
         }
       };
-      for (int j = 0; j < min(2, nblk); ++j) load(&tm_k, j, true);
-      for (int j = 0; j < nblk && ok; ++j) {
-        load(&tm_v, j, false);
-        if (!Q8 && j >= jedge) {
-          if (ok && lane == 0) mbar_arrive(ask_bar + (edges & (PTC_EDGES - 1)));
-          ++edges;
+      // where the groups lie: a window of 32 groups, a group a lane, and the next one looked up ahead
+      int wpage = -1, woff = 0, npage = -1, noff = 0;
+      auto look = [&](int key, int& page, int& off) {
+        page = -1;
+        if (key < end) {
+          const int i = key / a.BS;
+          page = a.bt[(int64_t)b * a.sbt + i];
+          off = key - i * a.BS;
         }
-        if (j + 2 < nblk && ok) load(&tm_k, j + 2, true);
+      };
+      if (nblk > 0) look(start + lane * group, npage, noff);
+      // keys are loaded two blocks ahead of values: pages of blocks j - 2, j - 1, j
+      int page[3] = {-1, -1, -1}, off[3] = {0, 0, 0};
+      uint32_t there[3] = {0, 0, 0}, good[3] = {0, 0, 0};
+#pragma unroll 1
+      for (int j = 0; j < nblk + 2 && ok; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          page[i] = page[i + 1];
+          off[i] = off[i + 1];
+          there[i] = there[i + 1];
+          good[i] = good[i + 1];
+        }
+        if (j < nblk) {
+          const int at = (j * per) & 31;  // the block's first group in the window
+          if (at == 0) {
+            wpage = npage;
+            woff = noff;
+            look(start + (j * per + 32 + lane) * group, npage, noff);
+          }
+          page[2] = __shfl_sync(0xffffffffu, wpage, (at + lane) & 31);
+          off[2] = __shfl_sync(0xffffffffu, woff, (at + lane) & 31);
+          there[2] = __ballot_sync(0xffffffffu, lane < per && start + (j * per + lane) * group < end);
+          good[2] = __ballot_sync(0xffffffffu, page[2] >= 0 && page[2] < a.blocks) & there[2];
+        }
+        // the order of use: K0 K1 V0 K2 V1 .. (V of block j - 2 goes before K of block j)
+        if (j >= 2) {
+          load(&tm_v, page[0], off[0], there[0], good[0], false, 0);
+          if (!Q8 && j - 2 >= jedge) {
+            if (ok && lane == 0) mbar_arrive(ask_bar + (edges & (PTC_EDGES - 1)));
+            ++edges;
+          }
+        }
+        if (j < nblk && ok) load(&tm_k, page[2], off[2], there[2], good[2], true, blocks + j);
       }
       blocks += nblk;
       __syncwarp();
@@ -225,9 +339,11 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   } else if (warp == 8) {
     // ------------------------------------------------------------------------------------------------ products
     constexpr uint32_t id_s = make_idesc_16(128, 128, MF16, false), id_o = make_idesc_16(128, C::SW, MF16, true);
-    const uint32_t sq = ex_smem_u32(smem), sr = ex_smem_u32(ring);
+    // low words of the operands' descriptors
+    const uint32_t desc_q = (uint32_t)make_sw128_desc(ex_smem_u32(smem)), desc_r = (uint32_t)make_sw128_desc(ex_smem_u32(ring)),
+                   desc_v = (uint32_t)make_sw128_desc_n(ex_smem_u32(ring), C::SUB);
     int slot = 0;
-    uint32_t ph = 0, php[2] = {0, 0}, phq = 0, edges = 0;
+    uint32_t ph = 0, php = 0, phq = 0, edges = 0;
     bool ok = true;
     while (ok && next()) {  // (the whole warp walks; lane 0 issues)
       if (nblk == 0) continue;
@@ -235,19 +351,18 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         ok = mbar_wait(q_bar, phq, EX_DEVERR_WAIT_TMEM);
         auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1; };
         auto s_of = [&](int j) {
-#pragma unroll
+#pragma unroll 1
           for (int p = 0; p < C::PARTS; ++p) {
             if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
             if (!ok) return;
             tc_fence_after();
+            const uint32_t da = desc_q + p * (C::SW / 64) * (C::SUB >> 4), db = desc_r + slot * (C::SLOT >> 4);
 #pragma unroll
-            for (int x = 0; x < C::SW / 64; ++x) {
-              const uint64_t da = make_sw128_desc(sq + (p * (C::SW / 64) + x) * C::SUB);
-              const uint64_t db = make_sw128_desc(sr + slot * C::SLOT + x * C::SUB);
+            for (int x = 0; x < C::SW / 64; ++x)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                tc_mma_16(tmem + TM_S + (j & 1) * 128, da + 2 * k, db + 2 * k, id_s, (p | x | k) != 0);
-            }
+                tc_mma_16_lo(tmem + TM_S + (j & 1) * 128, da + x * (C::SUB >> 4) + 2 * k, db + x * (C::SUB >> 4) + 2 * k, id_s,
+                             (p | x | k) != 0);
             tc_commit(empty_bar + slot);
             advance();
           }
@@ -255,24 +370,25 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         };
         s_of(0);
         if (nblk > 1) s_of(1);
+#pragma unroll 1
         for (int j = 0; j < nblk && ok; ++j) {
           if (!Q8 && j >= jedge) {
             ok = mbar_wait(fix_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_MMA);
             ++edges;
           }
-          if (ok) ok = mbar_wait(p_bar + (j & 1), php[j & 1], EX_DEVERR_WAIT_TMEM);
-          php[j & 1] ^= 1;
-#pragma unroll
+          if (ok) ok = mbar_wait(p_bar + (j & 1), (php >> (j & 1)) & 1u, EX_DEVERR_WAIT_TMEM);
+          php ^= 1u << (j & 1);
+#pragma unroll 1
           for (int p = 0; p < C::PARTS; ++p) {
             if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t db = make_sw128_desc_n(sr + slot * C::SLOT, C::SUB);
+            const uint32_t db = desc_v + slot * (C::SLOT >> 4);
             const uint32_t d = tmem + TM_O + (C::STREAMS == 2 ? (j & 1) * D : p * C::SW);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              tc_mma_16_ta(d, tmem + TM_S + (j & 1) * 128 + k * 8, db + k * (2048 >> 4), id_o,
-                           (j >= C::STREAMS || k > 0) ? 1u : 0u);
+              tc_mma_16_ta_lo(d, tmem + TM_S + (j & 1) * 128 + k * 8, db + k * (2048 >> 4), id_o,
+                              (j >= C::STREAMS || k > 0) ? 1u : 0u);
             tc_commit(empty_bar + slot);
             advance();
           }
@@ -311,9 +427,11 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
           ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
           ok = __all_sync(0xffffffffu, ok);
+#pragma unroll 1
           for (int r = lane; r < 128 && ok; r += 32) {
             const int key = start + j * 128 + r;
             bool bad = false;
+#pragma unroll 1
             for (int c = 0; c < C::SW / 8; ++c) {
               uint4* x = reinterpret_cast<uint4*>(vs + (c >> 3) * C::SUB + r * 128 + (c & 7) * 16);
               if (key >= end) {
@@ -341,7 +459,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       }
       base += 2 * nblk * C::PARTS;
     }
-  } else if (warp >= 12) {
+  } else if (Q8 && warp >= 12) {
     // ------------------------------------------------------------------------------------------------ converters
     if constexpr (Q8) {
       const int t = tid - 384;
@@ -351,19 +469,15 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       while (ok && next()) {
         auto convert = [&](int j, bool is_v) {
           for (int p = 0; p < C::PARTS && ok; ++p) {
-            if (!mbar_wait(rfull_bar + rslot, rph, EX_DEVERR_WAIT_TMA) || !mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT))
-              sfail[1] = 1;
-            asm volatile("bar.sync 3, 128;" ::: "memory");
-            if (sfail[1]) {  // the same for every thread here: the flag is only set before the barrier
-              ok = false;
-              return;
-            }
+            ok = mbar_wait(rfull_bar + rslot, rph, EX_DEVERR_WAIT_TMA) && mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
             const uint8_t* src = raw + rslot * C::RAW;
             uint8_t* dst = ring + slot * C::SLOT;
             constexpr int CH = C::SW / 16;  // 16-byte chunks of codes of a key
 #pragma unroll 4
             for (int i = t; i < 128 * CH; i += 128) {
-              const int r = i / CH, c = i % CH;
+              const int r = (i & 7) + i / (8 * CH) * 8, c = (i >> 3) % CH;  // 8 lanes, 8 rows: no bank twice
               uint4 w = *reinterpret_cast<const uint4*>(
                   src + (C::SW == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4)));
               if (is_v && start + j * 128 + r >= end) w = make_uint4(0, 0, 0, 0);
@@ -391,7 +505,9 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         }
       }
     }
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     // -------------------------------------------------------------------------------------------------- softmax
     const int wg = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile
@@ -401,16 +517,21 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     bool ok = true;
     while (ok && next()) {
       const uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
-      const bool active = row0 + (warp & 3) * 32 < R;  // some row of this warp is real
-      float m = -INFINITY, l = 0.0f, vref = 0.0f;
+      // copies of the rows: each weighs W keys of a block
+      const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1, rows = 128 / copies, W = 128 / copies;
+      const int rl = copies == 1 ? row0 + r : r & (rows - 1);  // row of the request (at least R: none)
+      const int col = copies == 1 ? 0 : r / rows * W;
+      const bool active = copies > 1 || row0 + (warp & 3) * 32 < R;  // some row of this warp is real
+      float m = -INFINITY, l = 0.0f, vref = 0.0f, vinv = 0.0f;
       if (nblk > 0) {
         // queries: row-major in swizzled columns of 64 dims; D/8 lanes a row
         constexpr int LANES = D / 8;
         const int c = tid % LANES;
         for (int x = tid / LANES; x < 128; x += 256 / LANES) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (row0 + x < R) {
-            const int t = (row0 + x) / a.G, h = (row0 + x) % a.G;
+          const int xl = copies == 1 ? row0 + x : x & (rows - 1);
+          if (xl < R) {
+            const int t = xl / a.G, h = xl % a.G;
             v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + t) * a.sq_t +
                                                 (int64_t)(g * a.G + h) * a.sq_h + c * 8);
           }
@@ -433,7 +554,13 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               v.z = pack2<__half>(y[4] * inv, y[5] * inv);
               v.w = pack2<__half>(y[6] * inv, y[7] * inv);
             }
-            if (c == 0) sfac[x] = f * a.scale_log2;
+            if (c == 0) sfac[x] = f * fabsf(a.scale_log2);
+          }
+          if (a.scale_log2 < 0.0f) {  // the largest score is looked for before it is scaled
+            v.x ^= 0x80008000u;
+            v.y ^= 0x80008000u;
+            v.z ^= 0x80008000u;
+            v.w ^= 0x80008000u;
           }
           *reinterpret_cast<uint4*>(smem + (c >> 3) * C::SUB + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
         }
@@ -442,10 +569,10 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         mbar_arrive(q_bar);
         if constexpr (Q8) asm volatile("bar.sync 2, 256;" ::: "memory");  // sfac
       }
-      const float fac = Q8 ? sfac[r] : a.scale_log2;
+      const float fac = Q8 ? sfac[r] : fabsf(a.scale_log2);
       uint64_t word = 0;
-      if (row0 + r < R) {
-        const int t = (row0 + r) / a.G;
+      if (rl < R) {
+        const int t = rl / a.G;
         word = (a.mask ? a.mask[first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - T));  // (T >= 1)
       }
       const uint32_t all_good = (uint32_t)((1ull << (128 >> a.group_log2)) - 1ull);
@@ -462,211 +589,195 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           const uint32_t good = sgood[(blocks + j) & 7];
           const float* ks = sscale + ((blocks + j) & (C::SCALE_BLOCKS - 1)) * 256;
           const bool whole = j < jedge && good == all_good;
-          uint32_t vis[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            vis[q] = ~0u;
-            if (!whole) {
-              const int at = kb + 32 * q, d = at - ctx;  // drafted token of the chunk's first column
-              uint32_t v = d >= 64 ? 0u : d >= 0 ? (uint32_t)(word >> d) : d > -32 ? (uint32_t)(word << -d) | ((1u << -d) - 1u) : ~0u;
-              const int left = end - at;
-              if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
-              uint32_t pages = 0;
-              for (int i = 0; i < 32 >> a.group_log2; ++i)
-                if ((good >> ((32 * q >> a.group_log2) + i)) & 1u) pages |= ((1u << (1 << a.group_log2)) - 1u) << (i << a.group_log2);
-              vis[q] = v & pages;
-            }
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t u[32];
-            tmem_ld32(s_addr + q * 32, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float4 kv = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-              if constexpr (Q8) kv = *reinterpret_cast<const float4*>(ks + q * 32 + i);
-              const float x[4] = {__uint_as_float(u[i]) * kv.x, __uint_as_float(u[i + 1]) * kv.y, __uint_as_float(u[i + 2]) * kv.z,
-                                  __uint_as_float(u[i + 3]) * kv.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], ((vis[q] >> (i + k)) & 1u) ? x[k] * fac : -INFINITY);
-            }
-          }
-          const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          auto see = [&](int q) {  // 32 columns from col + 32 q on
+            const int at = kb + col + 32 * q, d = at - ctx;  // key, drafted token of the first
+            uint32_t v = d >= 64 ? 0u : d >= 0 ? (uint32_t)(word >> d) : d > -32 ? (uint32_t)(word << -d) | ((1u << -d) - 1u) : ~0u;
+            const int left = end - at;
+            if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
+            uint32_t pages = 0;
+            for (int i = 0; i < 32 >> a.group_log2; ++i)
+              if ((good >> (((col + 32 * q) >> a.group_log2) + i)) & 1u) pages |= ((1u << (1 << a.group_log2)) - 1u) << (i << a.group_log2);
+            return v & pages;
+          };
           float vmax = 0.0f;
           if constexpr (Q8) {  // the largest finite value scale of the block's readable keys: lane l looks at 4 l ..
             const float4 v = *reinterpret_cast<const float4*>(ks + 128 + lane * 4);
             const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (kb + lane * 4 + k < end && ((good >> ((lane * 4 + k) >> a.group_log2)) & 1u) && x[k] < INFINITY) vmax = fmaxf(vmax, x[k]);
+              if ((whole || (kb + lane * 4 + k < end && ((good >> ((lane * 4 + k) >> a.group_log2)) & 1u))) && x[k] < INFINITY)
+                vmax = fmaxf(vmax, x[k]);
+            vmax = __any_sync(0xffffffffu, vmax > 64.0f * vref) ? vmax : 0.0f;
+            if (__any_sync(0xffffffffu, vmax > 0.0f)) {
 #pragma unroll
-            for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+              for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            }
           }
-          const bool take = mb > m + 8.0f;  // (m = -inf: any finite score)
-          const bool vtake = Q8 && vmax > 64.0f * vref;
-          if (__any_sync(0xffffffffu, take) || vtake) {
-            const float mn = take ? mb : m;
-            float al = m == -INFINITY ? 0.0f : ex2(m - mn);
-            if (m == -INFINITY && mn == -INFINITY) al = 1.0f;
+          auto update = [&](float mb) {
+            const bool grows = mb > m + 8.0f;  // (m = -inf: any finite score)
+            const bool vgrows = Q8 && vmax > 64.0f * vref;
+            if (!__any_sync(0xffffffffu, grows) && !vgrows) return;
+            const float mn = grows ? mb : m;
+            float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
             m = mn;
             l *= al;
-            if (vtake) {
+            if (vgrows) {
               if (vmax >= 1.2e-38f) al *= __fdividef(vref, vmax);
               vref = vmax;
+              vinv = vref >= 1.2e-38f ? __frcp_rn(vref) : 0.0f;
             }
-            if (j >= C::STREAMS) {
-              // the last product on this O is done: it was issued before this S (D = 256: after it)
-              if (C::STREAMS == 1) {
-                if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
-                __syncwarp();
-                tc_fence_after();
-              }
+            if (j < C::STREAMS) return;  // nothing on O yet
+            // the last product on this O is done: it was issued before this S (D = 256: after it)
+            if (C::STREAMS == 1) {
+              if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
+              __syncwarp();
+              tc_fence_after();
+            }
 #pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(o_addr + c, o);
-                tmem_ld_wait();
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + c, o);
+              tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                tmem_st32(o_addr + c, o);
-              }
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+              tmem_st32(o_addr + c, o);
             }
+          };
+          if (whole)
+            ptc_weigh<Q8, MF16, false>(s_addr + col, s_addr + (col >> 1), W >> 5, ks + col, fac, m, l, vinv, see, update);
+          else
+            ptc_weigh<Q8, MF16, true>(s_addr + col, s_addr + (col >> 1), W >> 5, ks + col, fac, m, l, vinv, see, update);
+          if (copies > 1) {  // no weight of this copy for the other keys
+            const uint32_t z[16] = {};
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q)
+              if (q * 32 < col || q * 32 >= col + W) tmem_st16(s_addr + q * 16, z);
           }
-          const float sub = m == -INFINITY ? 0.0f : m;
-          const float vinv = Q8 && vref >= 1.2e-38f ? __frcp_rn(vref) : 0.0f;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t u[32], p[16];
-            tmem_ld32(s_addr + q * 32, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float4 kv = make_float4(1.0f, 1.0f, 1.0f, 1.0f), vv = kv;
-              if constexpr (Q8) {
-                kv = *reinterpret_cast<const float4*>(ks + q * 32 + i);
-                vv = *reinterpret_cast<const float4*>(ks + 128 + q * 32 + i);
-              }
-              const float kvx[4] = {kv.x, kv.y, kv.z, kv.w}, vvx[4] = {vv.x, vv.y, vv.z, vv.w};
-              float w[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float x = Q8 ? __uint_as_float(u[i + k]) * kvx[k] * fac - sub : __fmaf_rn(__uint_as_float(u[i + k]), fac, -sub);
-                const bool see = (vis[q] >> (i + k)) & 1u;
-                w[k] = see ? ex2(x) : 0.0f;
-                sum[k] += w[k];
-                if constexpr (Q8) w[k] = see ? w[k] * (vvx[k] * vinv) : 0.0f;
-              }
-              p[i / 2] = MF16 ? pack2<__half>(w[0], w[1]) : pack_bf16(w[0], w[1]);
-              p[i / 2 + 1] = MF16 ? pack2<__half>(w[2], w[3]) : pack_bf16(w[2], w[3]);
-            }
-            // 16 columns of weights over scores of the same or an earlier chunk, which have been read
-            asm volatile(
-                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                "%14, %15};" ::EX_I8(p, 0),
-                EX_I8(p, 8), "r"(s_addr + q * 16)
-                : "memory");
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st_wait();
         }
         tc_fence_before();
         mbar_arrive(p_bar + buf);
       }
-      // the streams and, of each row, the two halves of the head dimension: one for each four warps
+      // the streams and copies of each row, CD dims at a time through shared memory (over the queries); four warps each
+      // take every other piece of the head dimension
       if (nblk > 0 && !mbar_wait(end_bar, phe, EX_DEVERR_WAIT_MMA)) *sfail = 1;
       if (nblk > 0) phe ^= 1;
-      sm[wg * 128 + r] = m;
-      sl[wg * 128 + r] = l;
-      asm volatile("bar.sync 2, 256;" ::: "memory");
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // (every product is done: the queries may be written over)
       if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
       tc_fence_after();
+      float* sm = reinterpret_cast<float*>(smem);  // [2 streams][128]: m, then l, then the references of the value scales
+      sm[wg * 128 + r] = m;
+      sm[256 + wg * 128 + r] = l;
+      sm[512 + wg * 128 + r] = vref;
+      asm volatile("bar.sync 2, 256;" ::: "memory");
       pho += nblk;
       blocks += nblk;
-      if (!active) vref = 0.0f;
-      float f[2], lall = 0.0f;
-      const float m0 = sm[r], m1 = C::STREAMS == 2 ? sm[128 + r] : -INFINITY;
-      const float mall = fmaxf(m0, m1), sub = mall == -INFINITY ? 0.0f : mall;
-      f[0] = m0 == -INFINITY ? 0.0f : ex2(m0 - sub);
-      f[1] = m1 == -INFINITY ? 0.0f : ex2(m1 - sub);
-      lall = sl[r] * f[0] + (C::STREAMS == 2 ? sl[128 + r] * f[1] : 0.0f);
-      if constexpr (Q8) {
-        // the reference of each stream's value scales
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-        sm[wg * 128 + r] = vref;
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-        f[0] *= sm[r];
-        if (C::STREAMS == 2) f[1] *= sm[128 + r];
+      float mall = -INFINITY, lall = 0.0f, f[2];
+      for (int k = 0; k < copies; ++k) {
+        const int x = copies == 1 ? r : (r & (rows - 1)) + k * rows;
+        mall = fmaxf(mall, fmaxf(sm[x], sm[128 + x]));
       }
+      const float sub = mall == -INFINITY ? 0.0f : mall;
+      for (int k = 0; k < copies; ++k) {
+        const int x = copies == 1 ? r : (r & (rows - 1)) + k * rows;
+        lall += sm[256 + x] * ex2(sm[x] - sub) + sm[256 + 128 + x] * ex2(sm[128 + x] - sub);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        f[i] = sm[i * 128 + r] == -INFINITY ? 0.0f : ex2(sm[i * 128 + r] - sub) * (Q8 ? sm[512 + i * 128 + r] : 1.0f);
       const bool have1 = C::STREAMS == 2 && nblk > 1;
       const bool single = pr_segments_many(pr_keys(a, L)) == 1;
-      const bool edges = !Q8 && jedge < nblk;
       bool any = false;
-      if (edges)
+      if (!Q8 && jedge < nblk)
         for (int i = 0; i < 8; ++i) any |= mine[i] != 0;
-      if (active) {
-        const bool real = row0 + r < R;
-        const int t = real ? (row0 + r) / a.G : 0, h = g * a.G + (real ? (row0 + r) % a.G : 0);
-        const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
-        const int64_t pi = ((int64_t)(first + t) * a.H + h) * a.NS + s;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t + (int64_t)h * a.so_h;
+      const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // sm has been read
+      float* piece = reinterpret_cast<float*>(smem) + wg * 128 * CD;  // [128][CD], 4 floats a chunk, swizzled
+      const int t2 = tid & 127;
 #pragma unroll 1
-        for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
-          uint32_t u[32];
-          float o[32];
-          __syncwarp();
+      for (int c = wg * CD; c < D; c += 2 * CD) {
+        if (active) {
+          uint32_t u[CD];
+          float o[CD];
+#pragma unroll
+          for (int i = 0; i < CD; ++i) o[i] = 0.0f;
           if (nblk > 0) {
-            tmem_ld32(tmem + lanes + TM_O + c, u);
+            tmem_ld_n<CD>(tmem + lanes + TM_O + c, u);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+            for (int i = 0; i < CD; ++i) o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
           }
           if (have1) {
-            tmem_ld32(tmem + lanes + TM_O + D + c, u);
+            tmem_ld_n<CD>(tmem + lanes + TM_O + D + c, u);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[1];
+            for (int i = 0; i < CD; ++i) o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[1];
           }
+          if (single) {
+#pragma unroll
+            for (int i = 0; i < CD; ++i) o[i] *= inv;
+          }
+#pragma unroll
+          for (int i = 0; i < CD; i += 4)
+            *reinterpret_cast<float4*>(piece + r * CD + (((i >> 2) ^ (r & (CD / 4 - 1))) << 2)) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+        if (wg == 0) asm volatile("bar.sync 4, 128;" ::: "memory");
+        else asm volatile("bar.sync 5, 128;" ::: "memory");
+        const int real = copies == 1 ? min(128, R - row0) : R;
+        for (int i = t2; i < real * (CD / 4); i += 128) {
+          const int x = i / (CD / 4), q = i % (CD / 4);
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int k = 0; k < copies; ++k) {
+            const int y = x + k * rows;
+            const float4 w = *reinterpret_cast<const float4*>(piece + y * CD + ((q ^ (y & (CD / 4 - 1))) << 2));
+            v.x += w.x;
+            v.y += w.y;
+            v.z += w.z;
+            v.w += w.w;
+          }
+          const int row = row0 + x, t = row / a.G, h = g * a.G + row % a.G, d0 = c + q * 4;
           if (any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
+            const uint64_t rw = (a.mask ? a.mask[first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - T));
 #pragma unroll 1
             for (int k = 0; k < 256; ++k) {
               if (!((mine[k >> 5] >> (k & 31)) & 1u)) continue;
               const int key = start + jedge * 128 + k, d = key - ctx;
-              if (!real || key >= end || (d >= 0 && !((word >> d) & 1ull))) continue;
+              if (key >= end || (d >= 0 && !((rw >> d) & 1ull))) continue;
               const int page = a.bt[(int64_t)b * a.sbt + key / a.BS];
               if (page < 0 || page >= a.blocks) continue;
-              const uint16_t* v = reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
-                                  (int64_t)(key % a.BS) * s_page + (int64_t)g * s_head + c;
+              const uint16_t* e = reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
+                                  (int64_t)(key % a.BS) * s_page + (int64_t)g * s_head + d0;
+              float y[4];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float x = F16 ? __half2float(__ushort_as_half(v[i])) : __uint_as_float((uint32_t)v[i] << 16);
-                if (!(fabsf(x) < INFINITY)) o[i] += x;
+              for (int n = 0; n < 4; ++n) {
+                y[n] = F16 ? __half2float(__ushort_as_half(e[n])) : __uint_as_float((uint32_t)e[n] << 16);
+                if (fabsf(y[n]) < INFINITY) y[n] = 0.0f;
               }
+              v.x += y[0];
+              v.y += y[1];
+              v.z += y[2];
+              v.w += y[3];
             }
-            __syncwarp();
           }
-          if (real && single) {
+          if (single) {
             const bool f16 = Q8 ? a.q_is_f16 != 0 : F16;
-#pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              *reinterpret_cast<uint32_t*>(dst + c + i) = f16 ? pack2<__half>(o[i] * inv, o[i + 1] * inv) : pack_bf16(o[i] * inv, o[i + 1] * inv);
-          } else if (real) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(a.ws_acc + pi * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t +
+                                                        (int64_t)h * a.so_h + d0);
+            dst[0] = f16 ? pack2<__half>(v.x, v.y) : pack_bf16(v.x, v.y);
+            dst[1] = f16 ? pack2<__half>(v.z, v.w) : pack_bf16(v.z, v.w);
+          } else {
+            *reinterpret_cast<float4*>(a.ws_acc + (((int64_t)(first + t) * a.H + h) * a.NS + s) * D + d0) = v;
           }
         }
-        if (real && !single && wg == 0) {
-          a.ws_m[pi] = mall;
-          a.ws_l[pi] = lall;
-        }
+        if (wg == 0) asm volatile("bar.sync 4, 128;" ::: "memory");
+        else asm volatile("bar.sync 5, 128;" ::: "memory");
       }
-      asm volatile("bar.sync 2, 256;" ::: "memory");  // before sm, sl and sfac are written again
+      if (wg == 0 && !single && rl < R && (copies == 1 || r < rows)) {
+        const int64_t pi = ((int64_t)(first + rl / a.G) * a.H + g * a.G + rl % a.G) * a.NS + s;
+        a.ws_m[pi] = mall;
+        a.ws_l[pi] = lall;
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // before the queries and sfac are written again
     }
     __syncwarp();
     tc_fence_before();
