@@ -323,9 +323,12 @@ cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& m
   a.rows_lo = 0;
   a.rows_hi = ex::PR_FEW;
   if (rows <= 8) return launch_few_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
-  cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
-  if (rows <= ex::PR_FEW || e != cudaSuccess) return e;
-  a.rows_lo = ex::PR_FEW;
+  if (rows <= ex::PR_FEW) return launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
+  if (a.tokens != (int64_t)a.n * a.max_tokens) {  // else every request has max_tokens rows
+    const cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
+    if (e != cudaSuccess) return e;
+    a.rows_lo = ex::PR_FEW;
+  }
   a.rows_hi = INT32_MAX;
   using C = ex::PtcCfg<D, CODE>;
   static KernelReady ready;

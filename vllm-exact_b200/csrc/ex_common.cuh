@@ -124,6 +124,23 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   }
 }
 
+// mbar_wait for a warp that is well ahead of the others (a producer waiting for a free slot): it sleeps between tries, so that
+// it does not take instruction slots from them.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = ex_globaltimer();
+  for (;;) {
+    __nanosleep(64);
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t dt = ex_globaltimer() - t0;
+    if (dt > EX_WAIT_TIMEOUT_NS) {
+      ex_set_error(code);
+      return false;
+    }
+    if (dt > 1000000ull && *(volatile int*)&g_ex_dev_error != 0) return false;  // someone else already failed
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor), tiled 2D loads into this CTA's shared memory, completion counted on an mbarrier.
 // Every tensor load of this library writes only the issuing CTA's shared memory (no multicast form is used).

@@ -69,38 +69,29 @@ __device__ __forceinline__ uint64_t make_sw128_desc_n(uint32_t smem_addr, uint32
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void tc_mma_16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void tc_mma_16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
-// The same with the low words of the descriptors alone: the high words (1024 bytes between groups of 8 rows, version 1,
-// 128-byte swizzle) are the same for every operand here.
+// Products of one tile, issued by one lane of a warp that is here as a whole. Where every operand is uniform over the warp
+// (and the compiler can see it: see warp_uniform), they are in uniform registers from the start; a single lane's copies
+// would be moved there one by one, 80 cycles a product of 64.
+// D[tmem] (+)= A B^T over 64 elements of K, operands in shared memory: low words of the descriptors (the high words, 1024
+// bytes between groups of 8 rows, version 1, 128-byte swizzle, are the same for every operand here).
 constexpr uint32_t SW128_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ void tc_mma_16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(SW128_DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_16_ta_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+// the same with A in tensor memory
+__device__ __forceinline__ void tc_mma_16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(SW128_DESC_HI)
       : "memory");
 }
+// The value that every lane has, in a register the compiler knows to be uniform.
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 #define EX_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
 #define EX_I8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
@@ -263,7 +254,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         bool ok = true;
         auto load = [&](const CUtensorMap* m, int j) {
           for (int p = 0; p < C::PARTS && ok; ++p) {
-            ok = mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
+            ok = mbar_wait_idle(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
             if (!ok) return;
             mbar_arrive_expect_tx(full_bar + slot, C::SLOT);
 #pragma unroll
@@ -288,106 +279,105 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     } else if (warp == 8) {
       // -------------------------------------------------------------------------------------------- products
-      if (lane == 0 && nmax > 0) {
-        constexpr uint32_t id_s = make_idesc_16(128, 128, F16, false), id_o = make_idesc_16(128, C::SW, F16, true);
-        const uint32_t sq = ex_smem_u32(smem), sr = ex_smem_u32(ring);
-        int slot = 0;  // next slot to be used
-        uint32_t ph = 0;
-        bool ok = mbar_wait(q_bar, 0, EX_DEVERR_WAIT_TMA);
-        auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1; };
-        auto full = [&]() { if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA); };
-        // S (buffer) = Q (tile) K^T over the dims of one slot
-        auto issue_s = [&](int tile, int buf, int part) {
+      // The whole warp walks and waits, one lane issues. A wait that ran out is not looked at: what is issued then is wrong and
+      // harmless, the error is recorded, and every later wait ends at once.
+      constexpr uint32_t id_s = make_idesc_16(128, 128, F16, false), id_o = make_idesc_16(128, C::SW, F16, true);
+      const uint32_t dq = warp_uniform((uint32_t)make_sw128_desc(ex_smem_u32(smem))),
+                     dr = warp_uniform((uint32_t)make_sw128_desc(ex_smem_u32(ring))),
+                     dv = warp_uniform((uint32_t)make_sw128_desc_n(ex_smem_u32(ring), C::SUB)), tm = warp_uniform(tmem);
+      const int n0 = (int)warp_uniform((uint32_t)nblk[0]), n1 = (int)warp_uniform((uint32_t)nblk[1]), nm = max(n0, n1);
+      const int first_edge = (int)warp_uniform((uint32_t)edge);
+      uint32_t slot = 0, ph = 0;  // next slot to be used
+      // S (buffer) = Q (tile) K^T over the dims of the slot
+      auto issue_s = [&](uint32_t at, int tile, int buf, int part) {
+        if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < C::SW / 64; ++s) {
-            const uint64_t da = make_sw128_desc(sq + (tile * (D / 64) + part * (C::SW / 64) + s) * C::SUB);
-            const uint64_t db = make_sw128_desc(sr + slot * C::SLOT + s * C::SUB);
+          for (int x = 0; x < C::SW / 64; ++x)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              tc_mma_16(tmem + C::TM_S + buf * 128, da + 2 * k, db + 2 * k, id_s, (part | s | k) != 0);
-          }
-        };
-        auto issue_o = [&](int tile, int buf, int part, int j) {
-          const uint64_t db = make_sw128_desc_n(sr + slot * C::SLOT, C::SUB);
+              tc_mma_16(tm + C::TM_S + buf * 128, dq + ((tile * (D / 64) + part * (C::SW / 64) + x) * (C::SUB >> 4) + 2 * k),
+                        dr + at * (C::SLOT >> 4) + (x * (C::SUB >> 4) + 2 * k), id_s, (part | x | k) != 0);
+        }
+      };
+      auto issue_o = [&](uint32_t at, int tile, int buf, int part, uint32_t acc) {
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < PA_KEYS / 16; ++k)
-            tc_mma_16_ta(tmem + C::TM_O + tile * D + part * C::SW, tmem + C::TM_S + buf * 128 + k * 8, db + k * (2048 >> 4),
-                         id_o, (j | k) != 0);
-        };
+            tc_mma_16_ta(tm + C::TM_O + tile * D + part * C::SW, tm + C::TM_S + buf * 128 + k * 8,
+                         dv + at * (C::SLOT >> 4) + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
+        }
+      };
+      auto commit = [&](uint64_t* b) { if (elect_one()) tc_commit(b); };
+      auto wait_full = [&](uint32_t at, uint32_t p) {
+        mbar_wait(full_bar + at, p, EX_DEVERR_WAIT_TMA);
+        __syncwarp();
+        tc_fence_after();
+      };
+      if (nm > 0) {
+        mbar_wait(q_bar, 0, EX_DEVERR_WAIT_TMA);
         if constexpr (C::NQ == 2) {
-          full();
-          tc_fence_after();
-          for (int i = 0; i < 2 && ok; ++i)
-            if (nblk[i] > 0) {
-              issue_s(i, i, 0);
-              tc_commit(s_bar + i);
-            }
-          if (ok) tc_commit(empty_bar + slot);
-          advance();
-          for (int j = 0; j < nmax && ok; ++j) {
-            const int vslot = slot;
-            bool have_v = false, have_k = false;
-            for (int i = 0; i < 2 && ok; ++i) {
-              if (j >= nblk[i]) continue;
-              if (!have_v) {
-                full();
-                if (ok && j >= edge) ok = mbar_wait(fix_bar + (j - edge), 0, EX_DEVERR_WAIT_MMA);
-                have_v = true;
-              }
-              if (ok) ok = mbar_wait(p_bar + i, (uint32_t)j & 1u, EX_DEVERR_WAIT_TMEM);
-              if (!ok) break;
+          wait_full(0, 0);
+          if (n0 > 0) {
+            issue_s(0, 0, 0, 0);
+            commit(s_bar);
+          }
+          if (n1 > 0) {
+            issue_s(0, 1, 1, 0);
+            commit(s_bar + 1);
+          }
+          commit(empty_bar);
+          slot = 1;
+#pragma unroll 1
+          for (int j = 0; j < nm; ++j) {
+            const bool more = j + 1 < nm;
+            const uint32_t kslot = slot + 1 == C::SLOTS ? 0 : slot + 1, kph = kslot == 0 ? ph ^ 1u : ph;
+            wait_full(slot, ph);
+            if (j >= first_edge) mbar_wait(fix_bar + (j - first_edge), 0, EX_DEVERR_WAIT_MMA);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (j >= (i ? n1 : n0)) continue;
+              mbar_wait(p_bar + i, (uint32_t)j & 1u, EX_DEVERR_WAIT_TMEM);
+              __syncwarp();
               tc_fence_after();
-              issue_o(i, i, 0, j);
-              if (j + 1 < nblk[i]) {
-                advance();  // to K of the next block
-                if (!have_k) full();
-                have_k = true;
-                if (ok) {
-                  tc_fence_after();
-                  issue_s(i, i, 0);
-                  tc_commit(s_bar + i);
-                }
-                if (--slot < 0) slot = C::SLOTS - 1, ph ^= 1;  // back to V
+              issue_o(slot, i, i, 0, j > 0 ? 1u : 0u);
+              if (j + 1 < (i ? n1 : n0)) {
+                if (i == 0 || j + 1 >= n0) wait_full(kslot, kph);
+                issue_s(kslot, i, i, 0);
+                commit(s_bar + i);
               }
             }
-            if (!ok) break;
-            tc_commit(empty_bar + vslot);
-            advance();
-            if (j + 1 < nmax) {
-              tc_commit(empty_bar + slot);
-              advance();
+            commit(empty_bar + slot);
+            if (more) commit(empty_bar + kslot);
+            slot = kslot;
+            ph = kph;
+            if (more) {
+              ++slot;
+              if (slot == C::SLOTS) slot = 0, ph ^= 1u;
             }
           }
         } else {
-          auto s_of = [&](int j) {
-            for (int p = 0; p < C::PARTS && ok; ++p) {
-              full();
-              if (!ok) return;
-              tc_fence_after();
-              issue_s(0, j & 1, p);
-              tc_commit(empty_bar + slot);
+          auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1u; };
+          // K0 K1 V0 K2 V1 ..: S of a block is issued a block ahead of its P V
+#pragma unroll 1
+          for (int n = 0; n < 2 * nm; ++n) {
+            const bool is_v = n == 2 * nm - 1 || (n > 0 && !(n & 1));
+            const int j = n == 2 * nm - 1 ? nm - 1 : is_v ? (n >> 1) - 1 : (n + 1) >> 1;
+            if (is_v) {
+              if (j >= first_edge) mbar_wait(fix_bar + (j - first_edge), 0, EX_DEVERR_WAIT_MMA);
+              mbar_wait(p_bar + (j & 1), (uint32_t)(j >> 1) & 1u, EX_DEVERR_WAIT_TMEM);
+            }
+#pragma unroll
+            for (int p = 0; p < C::PARTS; ++p) {
+              wait_full(slot, ph);
+              if (is_v) issue_o(slot, 0, j & 1, p, j > 0 ? 1u : 0u);
+              else issue_s(slot, 0, j & 1, p);
+              commit(empty_bar + slot);
               advance();
             }
-            if (ok) tc_commit(s_bar + (j & 1));
-          };
-          s_of(0);
-          if (nmax > 1) s_of(1);
-          for (int j = 0; j < nmax && ok; ++j) {
-            if (ok && j >= edge) ok = mbar_wait(fix_bar + (j - edge), 0, EX_DEVERR_WAIT_MMA);
-            if (ok) ok = mbar_wait(p_bar + (j & 1), (uint32_t)(j >> 1) & 1u, EX_DEVERR_WAIT_TMEM);
-            for (int p = 0; p < C::PARTS && ok; ++p) {
-              full();
-              if (!ok) break;
-              tc_fence_after();
-              issue_o(0, j & 1, p, j);
-              tc_commit(empty_bar + slot);
-              advance();
-            }
-            if (ok) tc_commit(o_bar);
-            if (j + 2 < nmax && ok) s_of(j + 2);
+            commit(is_v ? o_bar : s_bar + (j & 1));
           }
         }
-        tc_commit(end_bar);
+        commit(end_bar);
         mbar_wait(end_bar, 0, EX_DEVERR_WAIT_MMA);
       }
     } else {
@@ -396,7 +386,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       bool ok = true;
       for (int j = edge; j < nmax && ok; ++j) {
         // the producer may be any number of blocks behind: its word that the slots are this block's comes first
-        ok = mbar_wait(ask_bar + (j - edge), 0, EX_DEVERR_WAIT_SLOT);
+        ok = mbar_wait_idle(ask_bar + (j - edge), 0, EX_DEVERR_WAIT_SLOT);
         for (int p = 0; p < C::PARTS && ok; ++p) {
           // number of the slot in the order of loading: K of min(j + 2, nmax) or j + 1 blocks and V of j came before
           const int at = C::NQ == 1 ? (min(j + 2, nmax) + j) * C::PARTS + p : 2 * j + 1;

@@ -51,80 +51,71 @@ struct PtcCfg {
   static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 
-// One row's part of a block: `chunks` times 32 columns of S from s_addr on, their weights (over S, from p_addr on) in 16 bits.
-// see(q): the columns of chunk q that are seen, if MASKED. update(x): brings m, l and O up to date with the part's largest
-// score. The scores are read twice rather than kept: the loops stay small, and with many warps in different places
-// fetching instructions is what costs.
-template <bool Q8, bool MF16, bool MASKED, typename See, typename Update>
-__device__ __forceinline__ void ptc_weigh(uint32_t s_addr, uint32_t p_addr, int chunks, const float* ks, float fac, float& m,
-                                          float& l, float& vinv, See see, Update update) {
-  float x[32];
-  auto take = [&](int q) {
-    tmem_ld32(s_addr + q * 32, reinterpret_cast<uint32_t*>(x));
-    tmem_ld_wait();
-    if constexpr (Q8) {
+// N (a multiple of 32) columns of a row's scores, scaled by the keys' scales where they have some.
+template <bool Q8, int N>
+__device__ __forceinline__ void ptc_scores(uint32_t s_addr, const float* ks, float (&x)[N]) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 k = *reinterpret_cast<const float4*>(ks + q * 32 + i);
-        x[i] *= k.x;
-        x[i + 1] *= k.y;
-        x[i + 2] *= k.z;
-        x[i + 3] *= k.w;
-      }
+  for (int c = 0; c < N; c += 32) tmem_ld32(s_addr + c, reinterpret_cast<uint32_t*>(x) + c);
+  tmem_ld_wait();
+  if constexpr (Q8) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(ks + i);
+      x[i] *= k.x;
+      x[i + 1] *= k.y;
+      x[i + 2] *= k.z;
+      x[i + 3] *= k.w;
     }
-    uint32_t v = ~0u;
-    if constexpr (MASKED) {
-      v = see(q);
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!((v >> i) & 1u)) x[i] = -INFINITY;
-    }
-    return v;
-  };
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-  for (int q = 0; q < chunks; ++q) {
-    take(q);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
   }
-  update(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
-  const float sub = m == -INFINITY ? 0.0f : m;
+}
+template <int N>
+__device__ __forceinline__ float ptc_max(const float (&x)[N]) {
+  float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int i = 4; i < N; ++i) m[i & 3] = fmaxf(m[i & 3], x[i]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// Their weights 2^(x fac - sub) in 16 bits to tensor memory at p_addr (over scores that have been read); returns the weights'
+// sum. Codes: times the values' scales over their reference.
+template <bool Q8, bool MF16, int N>
+__device__ __forceinline__ float ptc_weights(uint32_t p_addr, const float* vs, float fac, float sub, float vinv, float (&x)[N]) {
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-  for (int q = 0; q < chunks; ++q) {
-    const uint32_t seen = take(q);
+#pragma unroll
+  for (int c = 0; c < N; c += 32) {
     uint32_t p[16];
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       float w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        w[k] = ex2(__fmaf_rn(x[i + k], fac, -sub));
+        w[k] = ex2(__fmaf_rn(x[c + i + k], fac, -sub));
         sum[k] += w[k];
       }
       if constexpr (Q8) {
-        const float4 v = *reinterpret_cast<const float4*>(ks + 128 + q * 32 + i);
+        const float4 v = *reinterpret_cast<const float4*>(vs + c + i);
         w[0] *= v.x * vinv;
         w[1] *= v.y * vinv;
         w[2] *= v.z * vinv;
         w[3] *= v.w * vinv;
-        if constexpr (MASKED) {  // a key that is not seen has a scale that may be anything
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (!((seen >> (i + k)) & 1u)) w[k] = 0.0f;
-        }
       }
       p[i / 2] = MF16 ? pack2<__half>(w[0], w[1]) : pack_bf16(w[0], w[1]);
       p[i / 2 + 1] = MF16 ? pack2<__half>(w[2], w[3]) : pack_bf16(w[2], w[3]);
     }
-    tmem_st16(p_addr + q * 16, p);  // over scores of the same or an earlier chunk, which have been read
+    tmem_st16(p_addr + c / 2, p);
   }
-  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
 constexpr int PTC_POISON = 8;  // items whose notes of values that are not finite are kept (the ring runs ahead of the rows)
+
+// The tiles of a segment of nblk blocks in the order of use, K0 K1 V0 K2 V1 .. (S of a block is made one block ahead of its
+// P V): tile n of 2 nblk is block j's values or keys.
+__device__ __forceinline__ bool ptc_tile(int n, int nblk, int& j) {
+  const bool v = n == 2 * nblk - 1 || (n > 0 && !(n & 1));
+  j = n == 2 * nblk - 1 ? nblk - 1 : v ? (n >> 1) - 1 : (n + 1) >> 1;
+  return v;
+}
 
 template <int D, int CODE, bool F16>
 __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
@@ -232,59 +223,6 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     constexpr int NB = C::SW * ESZ / PITCH;
     bool ok = true;
     while (ok && next()) {
-      // one tile (K or V) of a block whose group `lane` lies on `page` at `off`; bits of the groups there and of the good
-      auto load = [&](const CUtensorMap* m, int page, int off, uint32_t there, uint32_t good, bool is_k, uint32_t no) {
-#pragma unroll 1
-        for (int p = 0; p < C::PARTS && ok; ++p) {
-          ok = mbar_wait(empties + slot, ph, EX_DEVERR_WAIT_SLOT);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) return;
-          uint8_t* dst = Q8 ? raw + slot * C::RAW : ring + slot * C::SLOT;
-          if (feeder == 0) {
-            if (good != there) {  // tokens on pages that do not exist: zeros
-#pragma unroll 1
-              for (int i = 0; i < per; ++i) {
-                if (!((there & ~good) >> i & 1)) continue;
-#pragma unroll 1
-                for (int c = lane; c < NB * group * PITCH / 16; c += 32) {
-                  const int n = c / (group * PITCH / 16), x = c % (group * PITCH / 16);
-                  *reinterpret_cast<uint4*>(dst + n * 128 * PITCH + i * group * PITCH + x * 16) = make_uint4(0, 0, 0, 0);
-                }
-              }
-              fence_proxy_async_shared();
-              __syncwarp();
-            }
-            if (lane == 0) {
-              if (is_k) sgood[no & 7] = good;
-              mbar_arrive_expect_tx(fulls + slot, (uint32_t)(__popc(good) * group * C::SW * ESZ));
-            }
-          }
-          if (((good >> lane) & 1u) && lane % C::FEEDERS == feeder) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-              tma_load_4d(dst + n * 128 * PITCH + lane * group * PITCH, m, fulls + slot, (p * C::SW * ESZ + n * PITCH) / ESZ, g,
-                          off, page);
-          }
-          __syncwarp();
-          if constexpr (Q8) {
-            if (feeder == C::FEEDERS - 1) {
-              if (is_k && p == 0) {  // both scales come with the keys: the weights need them before the values
-                float* ss = sscale + (no & (C::SCALE_BLOCKS - 1)) * 256 + lane * 4;
-                const int from = (lane * 4) >> a.group_log2;
-                const int pg = __shfl_sync(0xffffffffu, page, from), po = __shfl_sync(0xffffffffu, off, from);
-                if ((good >> from) & 1u) {
-                  const int64_t so = (int64_t)pg * a.ss_block + g * a.ss_head + po + ((lane * 4) & (group - 1));
-                  cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
-                  cp_async16(ex_smem_u32(ss + 128), a.v_scale + so, true);
-                }
-              }
-              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(fulls + slot)) : "memory");
-            }
-          }
-          ++made;
-          if (++slot == SLOTS) slot = 0, ph ^= 1;
-        }
-      };
       // where the groups lie: a window of 32 groups, a group a lane, and the next one looked up ahead
       int wpage = -1, woff = 0, npage = -1, noff = 0;
       auto look = [&](int key, int& page, int& off) {
@@ -295,40 +233,90 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           off = key - i * a.BS;
         }
       };
-      if (nblk > 0) look(start + lane * group, npage, noff);
-      // keys are loaded two blocks ahead of values: pages of blocks j - 2, j - 1, j
-      int page[3] = {-1, -1, -1}, off[3] = {0, 0, 0};
-      uint32_t there[3] = {0, 0, 0}, good[3] = {0, 0, 0};
+      // keys are loaded a block ahead of values: pages (lane: group) of the block whose keys were last loaded, and the one before
+      int page[2] = {-1, -1}, off[2] = {0, 0};
+      int key = start + lane * group;  // of the next look-up
 #pragma unroll 1
-      for (int j = 0; j < nblk + 2 && ok; ++j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          page[i] = page[i + 1];
-          off[i] = off[i + 1];
-          there[i] = there[i + 1];
-          good[i] = good[i + 1];
-        }
-        if (j < nblk) {
+      for (int n = 0; n < 2 * nblk && ok; ++n) {
+        int j;
+        const bool is_v = ptc_tile(n, nblk, j);
+        if (!is_v) {
           const int at = (j * per) & 31;  // the block's first group in the window
           if (at == 0) {
+            if (n == 0) {
+              look(key, npage, noff);
+              key += 32 * group;
+            }
             wpage = npage;
             woff = noff;
-            look(start + (j * per + 32 + lane) * group, npage, noff);
+            look(key, npage, noff);
+            key += 32 * group;
           }
-          page[2] = __shfl_sync(0xffffffffu, wpage, (at + lane) & 31);
-          off[2] = __shfl_sync(0xffffffffu, woff, (at + lane) & 31);
-          there[2] = __ballot_sync(0xffffffffu, lane < per && start + (j * per + lane) * group < end);
-          good[2] = __ballot_sync(0xffffffffu, page[2] >= 0 && page[2] < a.blocks) & there[2];
+          page[0] = page[1];
+          off[0] = off[1];
+          page[1] = __shfl_sync(0xffffffffu, wpage, (at + lane) & 31);
+          off[1] = __shfl_sync(0xffffffffu, woff, (at + lane) & 31);
+          if (lane >= per) page[1] = -1;
         }
-        // the order of use: K0 K1 V0 K2 V1 .. (V of block j - 2 goes before K of block j)
-        if (j >= 2) {
-          load(&tm_v, page[0], off[0], there[0], good[0], false, 0);
-          if (!Q8 && j - 2 >= jedge) {
-            if (ok && lane == 0) mbar_arrive(ask_bar + (edges & (PTC_EDGES - 1)));
-            ++edges;
+        const bool before = is_v && j < nblk - 1;  // (the last block's values follow its own keys)
+        const int pg = before ? page[0] : page[1], po = before ? off[0] : off[1];
+        const uint32_t there = __ballot_sync(0xffffffffu, lane < per && start + (j * per + lane) * group < end);
+        const uint32_t good = __ballot_sync(0xffffffffu, pg >= 0 && pg < a.blocks) & there;
+#pragma unroll 1
+        for (int p = 0; p < C::PARTS; ++p) {
+          ok = mbar_wait_idle(empties + slot, ph, EX_DEVERR_WAIT_SLOT);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint8_t* dst = Q8 ? raw + slot * C::RAW : ring + slot * C::SLOT;
+          if (feeder == 0) {
+            if (good != there) {  // tokens on pages that do not exist: zeros
+#pragma unroll 1
+              for (int i = 0; i < per; ++i) {
+                if (!((there & ~good) >> i & 1)) continue;
+#pragma unroll 1
+                for (int c = lane; c < NB * group * PITCH / 16; c += 32) {
+                  const int h = c / (group * PITCH / 16), x = c % (group * PITCH / 16);
+                  *reinterpret_cast<uint4*>(dst + h * 128 * PITCH + i * group * PITCH + x * 16) = make_uint4(0, 0, 0, 0);
+                }
+              }
+              fence_proxy_async_shared();
+              __syncwarp();
+            }
+            if (lane == 0) {
+              if (!is_v) sgood[(blocks + j) & 7] = good;
+              mbar_arrive_expect_tx(fulls + slot, (uint32_t)(__popc(good) * group * C::SW * ESZ));
+            }
           }
+          if (((good >> lane) & 1u) && lane % C::FEEDERS == feeder) {
+            const CUtensorMap* m = is_v ? &tm_v : &tm_k;
+#pragma unroll
+            for (int h = 0; h < NB; ++h)
+              tma_load_4d(dst + h * 128 * PITCH + lane * group * PITCH, m, fulls + slot, (p * C::SW * ESZ + h * PITCH) / ESZ, g,
+                          po, pg);
+          }
+          __syncwarp();
+          if constexpr (Q8) {
+            if (feeder == C::FEEDERS - 1) {
+              if (!is_v && p == 0) {  // both scales come with the keys: the weights need them before the values
+                float* ss = sscale + ((blocks + j) & (C::SCALE_BLOCKS - 1)) * 256 + lane * 4;
+                const int from = (lane * 4) >> a.group_log2;
+                const int p2 = __shfl_sync(0xffffffffu, pg, from), o2 = __shfl_sync(0xffffffffu, po, from);
+                if ((good >> from) & 1u) {
+                  const int64_t so = (int64_t)p2 * a.ss_block + g * a.ss_head + o2 + ((lane * 4) & (group - 1));
+                  cp_async16(ex_smem_u32(ss), a.k_scale + so, true);
+                  cp_async16(ex_smem_u32(ss + 128), a.v_scale + so, true);
+                }
+              }
+              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ex_smem_u32(fulls + slot)) : "memory");
+            }
+          }
+          ++made;
+          if (++slot == SLOTS) slot = 0, ph ^= 1;
         }
-        if (j < nblk && ok) load(&tm_k, page[2], off[2], there[2], good[2], true, blocks + j);
+        if (!Q8 && is_v && j >= jedge) {
+          if (ok && lane == 0) mbar_arrive(ask_bar + (edges & (PTC_EDGES - 1)));
+          ++edges;
+        }
       }
       blocks += nblk;
       __syncwarp();
@@ -339,72 +327,63 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   } else if (warp == 8) {
     // ------------------------------------------------------------------------------------------------ products
     constexpr uint32_t id_s = make_idesc_16(128, 128, MF16, false), id_o = make_idesc_16(128, C::SW, MF16, true);
-    // low words of the operands' descriptors
-    const uint32_t desc_q = (uint32_t)make_sw128_desc(ex_smem_u32(smem)), desc_r = (uint32_t)make_sw128_desc(ex_smem_u32(ring)),
-                   desc_v = (uint32_t)make_sw128_desc_n(ex_smem_u32(ring), C::SUB);
-    int slot = 0;
-    uint32_t ph = 0, php = 0, phq = 0, edges = 0;
-    bool ok = true;
-    while (ok && next()) {  // (the whole warp walks; lane 0 issues)
-      if (nblk == 0) continue;
-      if (lane == 0) {
-        ok = mbar_wait(q_bar, phq, EX_DEVERR_WAIT_TMEM);
-        auto advance = [&]() { if (++slot == C::SLOTS) slot = 0, ph ^= 1; };
-        auto s_of = [&](int j) {
+    // The whole warp walks and waits, one lane issues. A wait that ran out is not looked at: what is issued then is wrong and
+    // harmless, the error is recorded, and every later wait ends at once.
+    const uint32_t dq = warp_uniform((uint32_t)make_sw128_desc(ex_smem_u32(smem))),
+                   dr = warp_uniform((uint32_t)make_sw128_desc(ex_smem_u32(ring))),
+                   dv = warp_uniform((uint32_t)make_sw128_desc_n(ex_smem_u32(ring), C::SUB)), tm = warp_uniform(tmem);
+    uint32_t slot = 0, ph = 0, php = 0, phq = 0, edges = 0;
+    auto commit = [&](uint64_t* b) { if (elect_one()) tc_commit(b); };
+    while (next()) {
+      const int nb = (int)warp_uniform((uint32_t)nblk), je = (int)warp_uniform((uint32_t)jedge);
+      if (nb == 0) continue;
+      mbar_wait(q_bar, phq, EX_DEVERR_WAIT_TMEM);
+      phq ^= 1;
 #pragma unroll 1
-          for (int p = 0; p < C::PARTS; ++p) {
-            if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t da = desc_q + p * (C::SW / 64) * (C::SUB >> 4), db = desc_r + slot * (C::SLOT >> 4);
-#pragma unroll
-            for (int x = 0; x < C::SW / 64; ++x)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tc_mma_16_lo(tmem + TM_S + (j & 1) * 128, da + x * (C::SUB >> 4) + 2 * k, db + x * (C::SUB >> 4) + 2 * k, id_s,
-                             (p | x | k) != 0);
-            tc_commit(empty_bar + slot);
-            advance();
-          }
-          tc_commit(s_bar + (j & 1));
-        };
-        s_of(0);
-        if (nblk > 1) s_of(1);
-#pragma unroll 1
-        for (int j = 0; j < nblk && ok; ++j) {
-          if (!Q8 && j >= jedge) {
-            ok = mbar_wait(fix_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_MMA);
+      for (int n = 0; n < 2 * nb; ++n) {
+        int j;
+        const bool is_v = ptc_tile(n, nb, j);
+        const uint32_t sbuf = tm + TM_S + (j & 1) * 128;
+        if (is_v) {
+          if (!Q8 && j >= je) {
+            mbar_wait(fix_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_MMA);
             ++edges;
           }
-          if (ok) ok = mbar_wait(p_bar + (j & 1), (php >> (j & 1)) & 1u, EX_DEVERR_WAIT_TMEM);
+          mbar_wait(p_bar + (j & 1), (php >> (j & 1)) & 1u, EX_DEVERR_WAIT_TMEM);
           php ^= 1u << (j & 1);
-#pragma unroll 1
-          for (int p = 0; p < C::PARTS; ++p) {
-            if (ok) ok = mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t db = desc_v + slot * (C::SLOT >> 4);
-            const uint32_t d = tmem + TM_O + (C::STREAMS == 2 ? (j & 1) * D : p * C::SW);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              tc_mma_16_ta_lo(d, tmem + TM_S + (j & 1) * 128 + k * 8, db + k * (2048 >> 4), id_o,
-                              (j >= C::STREAMS || k > 0) ? 1u : 0u);
-            tc_commit(empty_bar + slot);
-            advance();
-          }
-          if (C::STREAMS == 1 && ok) tc_commit(o_bar);
-          if (j + 2 < nblk && ok) s_of(j + 2);
         }
-        if (ok) tc_commit(end_bar);
-        phq ^= 1;
+#pragma unroll
+        for (int p = 0; p < C::PARTS; ++p) {
+          mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
+          __syncwarp();
+          tc_fence_after();
+          if (elect_one()) {
+            if (is_v) {
+              const uint32_t d = tm + TM_O + (C::STREAMS == 2 ? (j & 1) * D : p * C::SW), db = dv + slot * (C::SLOT >> 4);
+              const uint32_t acc = j >= C::STREAMS ? 1u : 0u;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) tc_mma_16_ta(d, sbuf + k * 8, db + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
+            } else {
+              const uint32_t db = dr + slot * (C::SLOT >> 4);
+#pragma unroll
+              for (int x = 0; x < C::SW / 64; ++x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  tc_mma_16(sbuf, dq + (p * (C::SW / 64) + x) * (C::SUB >> 4) + 2 * k, db + x * (C::SUB >> 4) + 2 * k, id_s,
+                            (p | x | k) != 0);
+            }
+            tc_commit(empty_bar + slot);
+          }
+          if (++slot == C::SLOTS) slot = 0, ph ^= 1u;
+        }
+        if (!is_v) commit(s_bar + (j & 1));
+        else if (C::STREAMS == 1) commit(o_bar);
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      commit(end_bar);
     }
     // every product is done before tensor memory is given back
-    if (lane == 0) {
-      tc_commit(done_bar);
-      mbar_wait(done_bar, 0, EX_DEVERR_WAIT_MMA);
-    }
+    commit(done_bar);
+    mbar_wait(done_bar, 0, EX_DEVERR_WAIT_MMA);
     __syncwarp();
   } else if (warp == 10 && !Q8) {
     // ---------------------------------------------------------------------------------------------- edge values
@@ -421,7 +400,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       for (int j = jedge; j < nblk && ok; ++j) {
         const int e = j - jedge;
         // the producer's word that the slots are this block's
-        ok = mbar_wait(ask_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_SLOT);
+        ok = mbar_wait_idle(ask_bar + (edges & (PTC_EDGES - 1)), (edges / PTC_EDGES) & 1u, EX_DEVERR_WAIT_SLOT);
         for (int p = 0; p < C::PARTS && ok; ++p) {
           const int at = base + (min(j + 2, nblk) + j) * C::PARTS + p;  // in the order of loading
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
@@ -467,29 +446,35 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       uint32_t rph = 0, ph = 1;
       bool ok = true;
       while (ok && next()) {
-        auto convert = [&](int j, bool is_v) {
-          for (int p = 0; p < C::PARTS && ok; ++p) {
+#pragma unroll 1
+        for (int n = 0; n < 2 * nblk && ok; ++n) {
+          int j;
+          const bool is_v = ptc_tile(n, nblk, j);
+#pragma unroll 1
+          for (int p = 0; p < C::PARTS; ++p) {
             ok = mbar_wait(rfull_bar + rslot, rph, EX_DEVERR_WAIT_TMA) && mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
+            if (!ok) break;
             const uint8_t* src = raw + rslot * C::RAW;
             uint8_t* dst = ring + slot * C::SLOT;
-            constexpr int CH = C::SW / 16;  // 16-byte chunks of codes of a key
+            // 8 lanes take the same 16 codes of 8 keys (no bank twice), then the keys STEP on: the swizzle stays the same
+            constexpr int CH = C::SW / 16, STEP = 128 / CH;
+            const int r0 = (t & 7) + t / (8 * CH) * 8, c = (t >> 3) % CH, c2 = (c & 3) * 2;
+            src += C::SW == 128 ? r0 * 128 + ((c ^ (r0 & 7)) << 4) : r0 * 64 + ((c ^ ((r0 >> 1) & 3)) << 4);
+            dst += (c >> 2) * C::SUB + r0 * 128;
+            const int d0 = (c2 ^ (r0 & 7)) << 4, d1 = ((c2 + 1) ^ (r0 & 7)) << 4;
+            const int left = is_v ? end - (start + j * 128 + r0) : 128;  // values behind the end: zeros
 #pragma unroll 4
-            for (int i = t; i < 128 * CH; i += 128) {
-              const int r = (i & 7) + i / (8 * CH) * 8, c = (i >> 3) % CH;  // 8 lanes, 8 rows: no bank twice
-              uint4 w = *reinterpret_cast<const uint4*>(
-                  src + (C::SW == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4)));
-              if (is_v && start + j * 128 + r >= end) w = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < CH; ++i) {
+              uint4 w = *reinterpret_cast<const uint4*>(src + i * STEP * C::SW);
+              if (i * STEP >= left) w = make_uint4(0, 0, 0, 0);
               uint32_t o[8];
               codes_to_f16<CODE>(w.x, o[0], o[1]);
               codes_to_f16<CODE>(w.y, o[2], o[3]);
               codes_to_f16<CODE>(w.z, o[4], o[5]);
               codes_to_f16<CODE>(w.w, o[6], o[7]);
-              uint8_t* d = dst + (c >> 2) * C::SUB + r * 128;
-              const int c2 = (c & 3) * 2;
-              *reinterpret_cast<uint4*>(d + ((c2 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(d + (((c2 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+              *reinterpret_cast<uint4*>(dst + i * STEP * 128 + d0) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(dst + i * STEP * 128 + d1) = make_uint4(o[4], o[5], o[6], o[7]);
             }
             fence_proxy_async_shared();
             mbar_arrive(full_bar + slot);
@@ -497,11 +482,6 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             if (++rslot == C::RAWS) rslot = 0, rph ^= 1;
             if (++slot == C::SLOTS) slot = 0, ph ^= 1;
           }
-        };
-        for (int j = 0; j < min(2, nblk); ++j) convert(j, false);
-        for (int j = 0; j < nblk && ok; ++j) {
-          convert(j, true);
-          if (j + 2 < nblk && ok) convert(j + 2, false);
         }
       }
     }
@@ -613,10 +593,38 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
             }
           }
-          auto update = [&](float mb) {
-            const bool grows = mb > m + 8.0f;  // (m = -inf: any finite score)
-            const bool vgrows = Q8 && vmax > 64.0f * vref;
-            if (!__any_sync(0xffffffffu, grows) && !vgrows) return;
+          // One step of 32 or 64 columns keeps its scores; more are read twice. Blocks that are not seen whole take a loop of
+          // their own, in steps of 32.
+          float x[64];
+          auto masked = [&](int q) {
+            float (&y)[32] = reinterpret_cast<float (&)[32]>(x);
+            ptc_scores<Q8>(s_addr + col + q * 32, ks + col + q * 32, y);
+            const uint32_t v = see(q);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((v >> i) & 1u)) y[i] = -INFINITY;
+          };
+          float mb = -INFINITY;
+          if (!whole) {
+#pragma unroll 1
+            for (int q = 0; q < W / 32; ++q) {
+              masked(q);
+              mb = fmaxf(mb, ptc_max(reinterpret_cast<float (&)[32]>(x)));
+            }
+          } else if (W == 32) {
+            ptc_scores<Q8>(s_addr + col, ks + col, reinterpret_cast<float (&)[32]>(x));
+            mb = ptc_max(reinterpret_cast<float (&)[32]>(x));
+          } else {
+#pragma unroll 1
+            for (int q = W / 64 - 1; q >= 0; --q) {  // (the first 64 last: they are kept)
+              ptc_scores<Q8>(s_addr + col + q * 64, ks + col + q * 64, x);
+              mb = fmaxf(mb, ptc_max(x));
+            }
+          }
+          mb *= fac;
+          const bool grows = mb > m + 8.0f;  // (m = -inf: any finite score)
+          const bool vgrows = Q8 && vmax > 64.0f * vref;
+          if (__any_sync(0xffffffffu, grows) || vgrows) {
             const float mn = grows ? mb : m;
             float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
             m = mn;
@@ -626,27 +634,48 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               vref = vmax;
               vinv = vref >= 1.2e-38f ? __frcp_rn(vref) : 0.0f;
             }
-            if (j < C::STREAMS) return;  // nothing on O yet
-            // the last product on this O is done: it was issued before this S (D = 256: after it)
-            if (C::STREAMS == 1) {
-              if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
-              __syncwarp();
-              tc_fence_after();
-            }
+            if (j >= C::STREAMS) {  // (else nothing is on O yet)
+              // the last product on this O is done: it was issued before this S (D = 256: after it)
+              if (C::STREAMS == 1) {
+                if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
+                __syncwarp();
+                tc_fence_after();
+              }
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + c, o);
-              tmem_ld_wait();
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-              tmem_st32(o_addr + c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                tmem_st16(o_addr + c, o);
+              }
             }
-          };
-          if (whole)
-            ptc_weigh<Q8, MF16, false>(s_addr + col, s_addr + (col >> 1), W >> 5, ks + col, fac, m, l, vinv, see, update);
-          else
-            ptc_weigh<Q8, MF16, true>(s_addr + col, s_addr + (col >> 1), W >> 5, ks + col, fac, m, l, vinv, see, update);
+          }
+          const float sub = m == -INFINITY ? 0.0f : m;
+          const uint32_t p_addr = s_addr + (col >> 1);
+          const float* vs = ks + 128 + col;
+          if (!whole) {
+#pragma unroll 1
+            for (int q = 0; q < W / 32; ++q) {
+              masked(q);
+              float y[32];  // scales of the keys that are seen (of others they may be anything)
+              if constexpr (Q8) {
+                const uint32_t v = see(q);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = (v >> i) & 1u ? vs[q * 32 + i] : 0.0f;
+              }
+              l += ptc_weights<Q8, MF16>(p_addr + q * 16, Q8 ? y : nullptr, fac, sub, vinv, reinterpret_cast<float (&)[32]>(x));
+            }
+          } else if (W == 32) {
+            l += ptc_weights<Q8, MF16>(p_addr, vs, fac, sub, vinv, reinterpret_cast<float (&)[32]>(x));
+          } else {
+#pragma unroll 1
+            for (int q = 0; q < W / 64; ++q) {
+              if (q > 0) ptc_scores<Q8>(s_addr + col + q * 64, ks + col + q * 64, x);
+              l += ptc_weights<Q8, MF16>(p_addr + q * 32, vs + q * 64, fac, sub, vinv, x);
+            }
+          }
           if (copies > 1) {  // no weight of this copy for the other keys
             const uint32_t z[16] = {};
 #pragma unroll 1
