@@ -4,9 +4,9 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - m) scale log2 e),  s_j = q . k_j
 //
-// m is a row's largest score so far, taken up only when it has grown by more than a factor 2^8 (p stays below 2^8, far
-// inside float16 and bf16, whose relative precision does not depend on it): O is rescaled a few times per row, not once
-// per block. All of it depends on the row alone.
+// m is a reference: the largest score of the row's first block, taken up again only when a score passes it by a factor of
+// 2^20 (2^14 for float16 weights, which end at 2^16): the precision of the weights and sums is relative and does not
+// depend on it, and O is almost never rescaled. It depends on the row alone.
 //
 // One CTA takes 256 queries of one head (128 where D = 256) and walks their keys in blocks of 128. tcgen05 products:
 // S = Q K^T with both operands in shared memory, O += P V with P in tensor memory, over the S it came from.
@@ -37,6 +37,7 @@ struct PaArgs {
 constexpr int PA_THREADS = 384;
 constexpr int PA_KEYS = 128;
 constexpr int PA_EDGES = 4;  // 256 rows reach over at most 3 blocks that are not visible to all of them
+constexpr int PA_POLY = 1;  // pairs of each eight whose exponentials go to the multiply-add units, see ex2_pair
 constexpr int PA_REGS_LAUNCH = 168, PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 static_assert(256 * PA_REGS_SOFTMAX + 128 * PA_REGS_OTHER <= PA_THREADS * PA_REGS_LAUNCH, "register shares");
 
@@ -131,13 +132,21 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// The tile'th tile of `rows` queries over all sequences: its sequence and first query in it; false if there is none.
-__device__ __forceinline__ bool pa_find_tile(const int32_t* __restrict__ cu, int n, int rows, int tile, int& b, int& row0) {
+// The tile'th tile of `rows` queries over all sequences: its first query in its sequence, and that sequence's first query
+// and key and numbers of both (offsets that leave the arrays, or run backwards, are not followed); false if there is none.
+// Every offset is loaded in the one pass: a second, dependent round of loads would cost 700 cycles.
+__device__ __forceinline__ bool pa_find_tile(const PaArgs& a, int rows, int tile, int& row0, int& q0, int& Lq, int& k0, int& Lk) {
   const int lane = threadIdx.x & 31;
   int seen = 0;
-  for (int base = 0; base < n; base += 32) {
-    int c = 0;
-    if (base + lane < n) c = (max(0, cu[base + lane + 1] - cu[base + lane]) + rows - 1) / rows;
+  for (int base = 0; base < a.n; base += 32) {
+    int c = 0, qa = 0, qb = 0, ka = 0, kb = 0;
+    if (base + lane < a.n) {
+      qa = a.cu_q[base + lane];
+      qb = a.cu_q[base + lane + 1];
+      ka = a.cu_k[base + lane];
+      kb = a.cu_k[base + lane + 1];
+      c = (int)((max((int64_t)0, (int64_t)qb - qa) + rows - 1) / rows);
+    }
     int incl = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -147,8 +156,12 @@ __device__ __forceinline__ bool pa_find_tile(const int32_t* __restrict__ cu, int
     const unsigned m = __ballot_sync(0xffffffffu, seen + incl > tile);
     if (m) {
       const int l = __ffs(m) - 1;
-      b = base + l;
       row0 = (tile - seen - __shfl_sync(0xffffffffu, incl - c, l)) * rows;
+      q0 = __shfl_sync(0xffffffffu, qa, l);
+      k0 = __shfl_sync(0xffffffffu, ka, l);
+      const int64_t q1 = __shfl_sync(0xffffffffu, qb, l), k1 = __shfl_sync(0xffffffffu, kb, l);
+      Lq = q0 >= 0 && q1 <= a.tokens ? (int)max((int64_t)0, q1 - q0) : 0;
+      Lk = k0 >= 0 && k1 <= a.keys ? (int)max((int64_t)0, k1 - k0) : 0;
       return true;
     }
     seen += __shfl_sync(0xffffffffu, incl, 31);
@@ -156,13 +169,50 @@ __device__ __forceinline__ bool pa_find_tile(const int32_t* __restrict__ cu, int
   return false;
 }
 
-// Queries and keys of sequence b; offsets that leave the arrays (or run backwards) are not followed.
-__device__ __forceinline__ void pa_sequence(const PaArgs& a, int b, int& q0, int& Lq, int& k0, int& Lk) {
-  q0 = a.cu_q[b];
-  k0 = a.cu_k[b];
-  const int64_t q1 = a.cu_q[b + 1], k1 = a.cu_k[b + 1];
-  Lq = q0 >= 0 && q1 <= a.tokens ? (int)max((int64_t)0, q1 - q0) : 0;
-  Lk = k0 >= 0 && k1 <= a.keys ? (int)max((int64_t)0, k1 - k0) : 0;
+struct f32x2 {
+  uint64_t v;
+};
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of a pair, x < 127, on the multiply-add units, which have time left where the exponential unit (16 a cycle and SM, a
+// quarter of what a block of scores asks for) has none: x = i + f with i the nearest integer (1.5 2^23 leaves no bits behind the
+// point), 2^f by a polynomial, i into the exponent. The polynomial is the least-maximum-error one of degree 4 on
+// [-0.5, 0.5], fitted by iteratively reweighted least squares (Lawson's method): relative error 2.7e-6 = 2^-18.5 in
+// float32, a hundredth of a rounding step of float16. Below 2^-126 it stays there.
+__device__ __forceinline__ void ex2_pair(f32x2 x, float& a, float& b) {
+  float x0, x1;
+  split(x, x0, x1);
+  x = pair(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const f32x2 t = add2(x, pair(12582912.0f, 12582912.0f));
+  const f32x2 f = add2(x, fma2(t, pair(-1.0f, -1.0f), pair(12582912.0f, 12582912.0f)));  // x - (t - 1.5 2^23)
+  f32x2 p = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591786280274391f, 0.05591786280274391f));
+  p = fma2(f, p, pair(0.240247443318367f, 0.240247443318367f));
+  p = fma2(f, p, pair(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(f, p, pair(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1, p0, p1;
+  split(t, t0, t1);
+  split(p, p0, p1);
+  a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 template <bool F16>
@@ -194,25 +244,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
-  pdl_wait();
-  int b, row0;
-  // the last tiles have the most keys: they start first
-  if (!pa_find_tile(a.cu_q, a.n, C::ROWS, a.tiles - 1 - (int)(blockIdx.x / a.H), b, row0)) return;
-  const int h = blockIdx.x % a.H, g = h / a.G;
-  int q0, Lq, k0, Lk;
-  pa_sequence(a, b, q0, Lq, k0, Lk);
-  if (row0 >= Lq) return;
-  const int off = Lk - Lq;  // row i sees the keys j <= i + off
-  int nblk[2];              // blocks of each tile
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = row0 + 128 * i, last = min(first + 127, Lq - 1);
-    nblk[i] = (i < C::NQ && first < Lq) ? max(0, (min(Lk, last + off + 1) + PA_KEYS - 1) / PA_KEYS) : 0;
-  }
-  const int nmax = max(nblk[0], nblk[1]);
-  const int edge = max(0, min(Lk, row0 + off + 1)) / PA_KEYS;  // blocks before it are seen by every row
-
   if (tid == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(full_bar + i, 1);
       mbar_init(empty_bar + i, 1);
@@ -231,14 +266,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int i = 0; i < 16; ++i) poison[i] = 0;
   }
-  if (warp == 8) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+  pdl_wait();
+  int row0, q0, Lq, k0, Lk;
+  // the last tiles have the most keys: they start first
+  if (!pa_find_tile(a, C::ROWS, a.tiles - 1 - (int)(blockIdx.x / a.H), row0, q0, Lq, k0, Lk) || row0 >= Lq) return;
+  const int h = blockIdx.x % a.H, g = h / a.G;
+  const int off = Lk - Lq;  // row i sees the keys j <= i + off
+  int nblk[2];              // blocks of each tile
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = row0 + 128 * i, last = min(first + 127, Lq - 1);
+    nblk[i] = (i < C::NQ && first < Lq) ? max(0, (min(Lk, last + off + 1) + PA_KEYS - 1) / PA_KEYS) : 0;
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const int nmax = max(nblk[0], nblk[1]);
+  const int edge = max(0, min(Lk, row0 + off + 1)) / PA_KEYS;  // blocks before it are seen by every row
+  __syncthreads();  // the barriers are there: the first loads are under way while tensor memory is taken
+  if (warp <= 8) {
+    if (warp == 8) {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, 288;" ::: "memory");
+    tc_fence_after();
+  }
+  const uint32_t tmem = warp <= 8 ? *(volatile uint32_t*)tmem_slot : 0u;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
@@ -392,29 +444,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const int at = C::NQ == 1 ? (min(j + 2, nmax) + j) * C::PARTS + p : 2 * j + 1;
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
           ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
-          for (int r = t; r < PA_KEYS && ok; r += 64) {
-            const int key = j * PA_KEYS + r;
-            bool bad = false;
-            for (int c = 0; c < C::SW / 8; ++c) {
-              uint4* x = reinterpret_cast<uint4*>(vs + (c >> 3) * C::SUB + r * 128 + (c & 7) * 16);
-              if (key >= Lk) {
-                *x = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 w = *x;
-                if (!(finite_word<F16>(w.x) && finite_word<F16>(w.y) && finite_word<F16>(w.z) && finite_word<F16>(w.w))) {
-                  bad = true;
-                  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          // 16 bytes of a key a thread, eight threads along a key's 128 bytes (no bank conflict), four keys in flight
+          const int sub = t & 7;
+#pragma unroll 1
+          for (int r = t >> 3; r < PA_KEYS * (C::SW / 64) && ok; r += 32) {
+            uint4 w[4];
+            uint4* x = reinterpret_cast<uint4*>(vs + r * 128 + sub * 16);  // row r of the slot's columns of 128 keys
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
-                    if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
-                  }
-                  *x = make_uint4(u[0], u[1], u[2], u[3]);
+            for (int i = 0; i < 4; ++i) w[i] = x[i * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = j * PA_KEYS + ((r + 8 * i) & (PA_KEYS - 1));
+              if (key >= Lk) {
+                x[i * 64] = make_uint4(0, 0, 0, 0);
+              } else if (!(finite_word<F16>(w[i].x) && finite_word<F16>(w[i].y) && finite_word<F16>(w[i].z) && finite_word<F16>(w[i].w))) {
+                uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
+                  if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
                 }
+                x[i * 64] = make_uint4(u[0], u[1], u[2], u[3]);
+                const int k = key - edge * PA_KEYS;
+                if (k < 512) atomicOr(poison + (k >> 5), 1u << (k & 31));
               }
             }
-            const int k = key - edge * PA_KEYS;
-            if (bad && k < 512) atomicOr(poison + (k >> 5), 1u << (k & 31));
           }
         }
         fence_proxy_async_shared();  // the products read shared memory through the async proxy
@@ -430,7 +484,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + C::TM_O + tile * D;
     const float sc = a.scale_log2;
-    const float grow = 8.0f / sc;
+    const float grow = (F16 ? 14.0f : 20.0f) / sc;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < nb; ++j) {
@@ -444,55 +498,92 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
       tmem_ld_wait();
-      if (j >= edge) {
-        const int limit = min(Lk - 1, row + off) - j * PA_KEYS;  // columns behind it are not seen
+      // A block that is seen whole is weighed with the reference that there is, while its largest score is still being looked
+      // for: nothing waits for it. If a score of the warp passes its row's reference by too much (or is NaN), or the block is
+      // an edge, or the first, the block is weighed (again) below.
+      bool again = j >= edge || j == 0;
+      f32x2 sum0 = pair(0.0f, 0.0f), sum1 = sum0;
+      // The weights of the block against the reference, written over S, and their sums. Both callers have the same arithmetic
+      // in the same order, so that a row does not depend on which one its warp needs.
+      auto weigh = [&](float sub, auto any) {  // any: scores that are -infinity (or not seen) or NaN too
+        const f32x2 sc2 = pair(sc, sc), sub2 = pair(-sub, -sub);
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;
-      }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-      for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-      const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool take = mb > m + grow || m == -INFINITY;
-      if (j == 0) {
-        m = mb;
-      } else if (__any_sync(0xffffffffu, take)) {
-        // the next product on O waits for P, the last one is done: it was issued before this S (D = 256: after it)
-        if (C::NQ == 1) {
-          ok = mbar_wait(o_bar, (uint32_t)(j - 1) & 1u, EX_DEVERR_WAIT_MMA);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
+          for (int i = 0; i < 16; ++i) {
+            const f32x2 x = fma2(pair(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), sc2, sub2);
+            float a0, a1, x0, x1;
+            split(x, x0, x1);
+            if ((i & 7) < PA_POLY) {
+              ex2_pair(x, a0, a1);
+              if (decltype(any)::value) {
+                a0 = x0 > -INFINITY ? a0 : ex2(x0);
+                a1 = x1 > -INFINITY ? a1 : ex2(x1);
+              }
+            } else {
+              a0 = ex2(x0);
+              a1 = ex2(x1);
+            }
+            if (i & 1) sum1 = add2(sum1, pair(a0, a1));
+            else sum0 = add2(sum0, pair(a0, a1));
+            p[i] = F16 ? pack2<__half>(a0, a1) : pack_bf16(a0, a1);
+          }
+          tmem_st16(s_addr + c * 16, p);
         }
-        const float mn = take ? fmaxf(m, mb) : m;
-        const float al = m == -INFINITY ? (mn == -INFINITY ? 1.0f : 0.0f) : ex2((m - mn) * sc);
-        m = mn;
-        l *= al;
+      };
+      if (!again) {
+        float mx[2] = {s[0], s[1]};
+#pragma unroll
+        for (int c = 2; c < 126; c += 4) {
+          mx[0] = max3_nan(mx[0], s[c], s[c + 1]);
+          mx[1] = max3_nan(mx[1], s[c + 2], s[c + 3]);
+        }
+        const float mb = max_nan(max3_nan(mx[0], s[126], s[127]), mx[1]);
+        weigh(m * sc, std::false_type{});
+        again = !(mb <= m + grow);
+      }
+      if (__any_sync(0xffffffffu, again)) {
+        if (j >= edge) {
+          const int limit = min(Lk - 1, row + off) - j * PA_KEYS;  // columns behind it are not seen
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+        const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool take = mb > m + grow || m == -INFINITY;
+        if (j == 0) {
+          m = mb;
+        } else if (__any_sync(0xffffffffu, take)) {
+          // the next product on O waits for P, the last one is done: it was issued before this S (D = 256: after it)
+          if (C::NQ == 1) {
+            ok = mbar_wait(o_bar, (uint32_t)(j - 1) & 1u, EX_DEVERR_WAIT_MMA);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          const float mn = take ? fmaxf(m, mb) : m;
+          const float al = m == -INFINITY ? (mn == -INFINITY ? 1.0f : 0.0f) : ex2((m - mn) * sc);
+          m = mn;
+          l *= al;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c, o);
-          tmem_ld_wait();
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c, o);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-          tmem_st32(o_addr + c, o);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+            tmem_st32(o_addr + c, o);
+          }
         }
+        sum0 = sum1 = pair(0.0f, 0.0f);
+        weigh(m == -INFINITY ? 0.0f : m * sc, std::true_type{});
       }
-      const float sub = m == -INFINITY ? 0.0f : m * sc;
-      float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float x = ex2(__fmaf_rn(s[c * 64 + 2 * i], sc, -sub)), y = ex2(__fmaf_rn(s[c * 64 + 2 * i + 1], sc, -sub));
-          sum[0] += x;
-          sum[1] += y;
-          p[i] = F16 ? pack2<__half>(x, y) : pack_bf16(x, y);
-        }
-        tmem_st32(s_addr + c * 32, p);
-      }
-      l += sum[0] + sum[1];
+      float a0, a1;
+      split(add2(sum0, sum1), a0, a1);
+      l += a0 + a1;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_bar + buf);
@@ -505,7 +596,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // nothing seen: zeros; NaN stays NaN
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(q0 + row) * a.so_t + (int64_t)h * a.so_h;
+        // the warp's 32 rows go through shared memory (over its queries), so that a row is written as a whole
+        uint8_t* mine = smem + (tile * 128 + (warp & 3) * 32) * (2 * D);
         bool any = false;
         for (int i = 0; i < 16; ++i) any |= poison[i] != 0;
 #pragma unroll 1
@@ -533,18 +625,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               }
             }
           }
-          if (row < Lq) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t w[4];
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
-                w[k] = F16 ? pack2<__half>(x, y) : pack_bf16(x, y);
-              }
-              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 4; ++k) {
+              const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
+              w[k] = F16 ? pack2<__half>(x, y) : pack_bf16(x, y);
             }
+            *reinterpret_cast<uint4*>(mine + lane * (2 * D) + ((((c + i) >> 3) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+        }
+        __syncwarp();
+        constexpr int PER = D / 8;  // 16-byte pieces of a row
+        const int rows = min(32, Lq - (row - lane));
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(q0 + row - lane) * a.so_t + (int64_t)h * a.so_h;
+#pragma unroll 4
+        for (int i = lane; i < rows * PER; i += 32) {
+          const int r = i / PER, c = i % PER;
+          *reinterpret_cast<uint4*>(dst + r * a.so_t + c * 8) = *reinterpret_cast<const uint4*>(mine + r * (2 * D) + ((c ^ (r & 7)) << 4));
         }
       }
     }

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import check, launch_on, lib
 
 __all__ = ["alloc_q8_cache", "cache_write", "cache_read"]
 
@@ -50,9 +50,8 @@ def _check_cache(key_cache, value_cache, key_scale, value_scale, dev):
         raise ValueError("key and value caches must share strides")
     if st[3] != 1 or ss[2] != 1:
         raise ValueError("the head dimension of codes and the places of scales must be contiguous")
-    for t in (key_cache, value_cache, key_scale, value_scale):
-        if t.device != dev:
-            raise ValueError("the cache must be on the same CUDA device as the other tensors")
+    if not key_cache.get_device() == value_cache.get_device() == key_scale.get_device() == value_scale.get_device() == dev:
+        raise ValueError("the cache must be on the same CUDA device as the other tensors")
     return code
 
 
@@ -73,8 +72,8 @@ def cache_write(key, value, key_cache, value_cache, key_scale, value_scale, slot
 
     key_out, value_out (tokens, KV, D), in key's type: receive the numbers which the rows stand for, so that the prompt
     that is being cached can attend to what later steps will see. Rows with an infinity or a NaN read back as NaN."""
-    dev = key.device
-    if not key.is_cuda or value.device != dev or slot_mapping.device != dev:
+    dev = key.get_device()  # -1: not on a GPU
+    if dev < 0 or value.get_device() != dev or slot_mapping.get_device() != dev:
         raise ValueError("cache_write needs CUDA tensors of one device (there is no CPU fallback)")
     code = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
     nb, BS, KV, D = key_cache.shape
@@ -86,26 +85,27 @@ def cache_write(key, value, key_cache, value_cache, key_scale, value_scale, slot
         raise ValueError("key_out and value_out are given together")
     if key_out is not None:
         _check_rows("key_out and value_out", key_out, value_out, KV, D)
-        if key_out.dtype != key.dtype or key_out.shape[0] != T or key_out.device != dev or value_out.device != dev:
+        if (key_out.dtype != key.dtype or key_out.shape[0] != T or key_out.get_device() != dev
+                or value_out.get_device() != dev):
             raise ValueError("key_out and value_out must be like key")
     slot_mapping = slot_mapping.contiguous()
     sk, sv, sc, ss = key.stride(), value.stride(), key_cache.stride(), key_scale.stride()
-    ko, vo = (key_out, value_out) if key_out is not None else (key, value)
-    with torch.cuda.device(dev):
+    ko, vo, sko, svo = None, None, (0, 0), (0, 0)
+    if key_out is not None:
+        ko, vo, sko, svo = key_out.data_ptr(), value_out.data_ptr(), key_out.stride(), value_out.stride()
+    with launch_on(dev) as stream:
         check("ex_cache_write_q8", lib().ex_cache_write_q8(
             key.data_ptr(), sk[0], sk[1], value.data_ptr(), sv[0], sv[1], _DT[key.dtype], code, key_cache.data_ptr(),
             value_cache.data_ptr(), sc[0], sc[1], sc[2], key_scale.data_ptr(), value_scale.data_ptr(), ss[0], ss[1], nb,
-            BS, slot_mapping.data_ptr(), T, KV, D, None if key_out is None else ko.data_ptr(), ko.stride(0),
-            ko.stride(1), None if key_out is None else vo.data_ptr(), vo.stride(0), vo.stride(1),
-            torch.cuda.current_stream(dev).cuda_stream))
+            BS, slot_mapping.data_ptr(), T, KV, D, ko, sko[0], sko[1], vo, svo[0], svo[1], stream))
 
 
 def cache_read(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, key_out, value_out):
     """Read the first cu_seqlens[b + 1] - cu_seqlens[b] tokens of every sequence b back into rows cu_seqlens[b] .. of
     key_out and value_out (rows, KV, D) bf16 or fp16; block_table (n, pages) int32, cu_seqlens (n + 1) int32. Rows of no
     sequence, behind the block table, or on a page that the cache does not have are left as they were."""
-    dev = key_out.device
-    if not key_out.is_cuda or any(t.device != dev for t in (value_out, block_table, cu_seqlens)):
+    dev = key_out.get_device()  # -1: not on a GPU
+    if dev < 0 or value_out.get_device() != dev or block_table.get_device() != dev or cu_seqlens.get_device() != dev:
         raise ValueError("cache_read needs CUDA tensors of one device (there is no CPU fallback)")
     code = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
     nb, BS, KV, D = key_cache.shape
@@ -118,12 +118,11 @@ def cache_read(key_cache, value_cache, key_scale, value_scale, block_table, cu_s
     if width > 1 and block_table.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
     cu_seqlens = cu_seqlens.contiguous()
-    sc, ss = key_cache.stride(), key_scale.stride()
-    with torch.cuda.device(dev):
+    sc, ss, sk, sv = key_cache.stride(), key_scale.stride(), key_out.stride(), value_out.stride()
+    with launch_on(dev) as stream:
         check("ex_cache_read_q8", lib().ex_cache_read_q8(
             key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0], sc[1], sc[2], key_scale.data_ptr(),
             value_scale.data_ptr(), ss[0], ss[1], nb, BS, block_table.data_ptr(), block_table.stride(0), width,
             cu_seqlens.data_ptr(), n, key_out.shape[0], KV, D, _DT[key_out.dtype], key_out.data_ptr(),
-            key_out.stride(0), key_out.stride(1), value_out.data_ptr(), value_out.stride(0), value_out.stride(1),
-            torch.cuda.current_stream(dev).cuda_stream))
+            sk[0], sk[1], value_out.data_ptr(), sv[0], sv[1], stream))
     return key_out, value_out

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, kv_cache
-from ._lib import check, lib
+from ._lib import check, launch_on, lib
 
 SPLIT = 4096       # keys per segment (fixed per deployment: it sets the reduction order)
 MAX_LEN = 16384    # number of segments = ceil(MAX_LEN / SPLIT); enable() sets it to max_model_len
@@ -94,16 +94,18 @@ def rows_workspace_bytes(tokens: int, H: int, D: int, max_len: int) -> int:
     return lib().ex_paged_rows_workspace_bytes(tokens, H, D, max_len)
 
 
-def _rows_operands(name, query, key_cache, value_cache, block_table, seq_lens, out, n, others):
-    """Checks shared by paged_decode_q8 and tree_attention."""
-    dev = query.device
-    if not query.is_cuda or any(t.device != dev for t in (key_cache, value_cache, block_table, seq_lens, out, *others)):
+def _rows_operands(name, query, key_cache, value_cache, block_table, seq_lens, out, n):
+    """Checks shared by paged_decode_q8 and tree_attention; the index of the device."""
+    dev = query.get_device()  # -1: not on a GPU
+    if (dev < 0 or key_cache.get_device() != dev or value_cache.get_device() != dev or block_table.get_device() != dev
+            or seq_lens.get_device() != dev or out.get_device() != dev):
         raise ValueError(f"{name} needs CUDA tensors of one device (there is no CPU fallback)")
     if query.dtype not in _DT16 or out.dtype != query.dtype:
         raise TypeError(f"{name} expects a bf16 or fp16 query, and out of the same type")
-    if query.dim() != 3 or out.dim() != 3 or key_cache.dim() != 4 or query.shape[2] != key_cache.shape[3]:
+    sq, so = query.shape, out.shape
+    if len(sq) != 3 or len(so) != 3 or key_cache.dim() != 4 or sq[2] != key_cache.shape[3]:
         raise ValueError("query and out must be (tokens, H, D), caches (num_blocks, block_size, KV, D)")
-    if out.shape[0] < query.shape[0] or out.shape[1:] != query.shape[1:]:
+    if so[1] != sq[1] or so[2] != sq[2]:
         raise ValueError("out must have a row for every row of query")
     if query.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("the head dimension must be contiguous")
@@ -113,13 +115,14 @@ def _rows_operands(name, query, key_cache, value_cache, block_table, seq_lens, o
         raise ValueError("block_table (n, pages) and seq_lens (n) need a row for every request")
     if block_table.shape[1] > 1 and block_table.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
+    return dev
 
 
-def _rows_scratch(tokens, H, D, max_len, workspace, dev):
-    nbytes = rows_workspace_bytes(tokens, H, D, max_len)
+def _rows_scratch(tokens, H, D, max_len, workspace, query):
+    nbytes = lib().ex_paged_rows_workspace_bytes(tokens, H, D, max_len)
     if nbytes and (workspace is None or workspace.numel() * workspace.element_size() < nbytes):
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    elif workspace is not None and workspace.device != dev:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    elif workspace is not None and workspace.get_device() != query.get_device():
         raise ValueError("the workspace must be on the query's device")
     return nbytes, workspace
 
@@ -137,22 +140,21 @@ def paged_decode_q8(query, key_cache, value_cache, key_scale, value_scale, block
         return out
     if query.shape[0] < n or out.shape[0] < n:
         raise ValueError("query and out need a row for every request")
-    _rows_operands("paged_decode_q8", query[:n], key_cache, value_cache, block_table, seq_lens, out, n, ())
-    dev = query.device
+    dev = _rows_operands("paged_decode_q8", query, key_cache, value_cache, block_table, seq_lens, out, n)
     code = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
     seq_lens = seq_lens.contiguous()
-    H, D = query.shape[1:]
+    _, H, D = query.shape
     nb, BS, KV, _ = key_cache.shape
     width = block_table.shape[1]
     max_len = width * BS if max_seq_len is None else min(max(0, int(max_seq_len)), width * BS)
-    nbytes, workspace = _rows_scratch(n, H, D, max_len, workspace, dev)
+    nbytes, workspace = _rows_scratch(n, H, D, max_len, workspace, query)
     sq, sc, ss, so = query.stride(), key_cache.stride(), key_scale.stride(), out.stride()
-    with torch.cuda.device(dev):
+    with launch_on(dev) as stream:
         check("ex_paged_decode_q8", lib().ex_paged_decode_q8(
             query.data_ptr(), sq[0], sq[1], _DT16[query.dtype], key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0],
             sc[1], sc[2], key_scale.data_ptr(), value_scale.data_ptr(), ss[0], ss[1], nb, block_table.data_ptr(),
             block_table.stride(0), width, seq_lens.data_ptr(), n, H, KV, D, BS, float(scale), max_len, out.data_ptr(),
-            so[0], so[1], workspace.data_ptr() if nbytes else None, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+            so[0], so[1], workspace.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
@@ -174,14 +176,15 @@ def tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_s
         raise TypeError("query_start_loc must be a 1-D int32 tensor with n + 1 entries")
     if not 1 <= max_query_len <= MAX_DRAFT:
         raise ValueError(f"max_query_len must be 1 to {MAX_DRAFT}")
-    others = (query_start_loc,)
     if tree_mask is not None:
         if tree_mask.dtype != torch.int64 or tree_mask.dim() != 1 or tree_mask.shape[0] < tokens:
             raise TypeError("tree_mask must be a 1-D int64 tensor with a word for every row of query")
         tree_mask = tree_mask.contiguous()
-        others += (tree_mask,)
-    _rows_operands("tree_attention", query, key_cache, value_cache, block_table, seq_lens, out, n, others)
-    dev = query.device
+    dev = _rows_operands("tree_attention", query, key_cache, value_cache, block_table, seq_lens, out, n)
+    if query_start_loc.get_device() != dev or (tree_mask is not None and tree_mask.get_device() != dev):
+        raise ValueError("tree_attention needs CUDA tensors of one device (there is no CPU fallback)")
+    if out.shape[0] < tokens:
+        raise ValueError("out must have a row for every row of query")
     if key_cache.dtype == query.dtype:
         if value_cache.dtype != key_cache.dtype or key_scale is not None or value_scale is not None:
             raise TypeError("a 16-bit cache has query's type and no scales")
@@ -196,19 +199,19 @@ def tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_s
     if n == 0 or tokens == 0:
         return out
     seq_lens, query_start_loc = seq_lens.contiguous(), query_start_loc.contiguous()
-    H, D = query.shape[1:]
+    _, H, D = query.shape
     nb, BS, KV, _ = key_cache.shape
     width = block_table.shape[1]
     max_len = width * BS if max_seq_len is None else min(max(0, int(max_seq_len)), width * BS)
-    nbytes, workspace = _rows_scratch(tokens, H, D, max_len, workspace, dev)
+    nbytes, workspace = _rows_scratch(tokens, H, D, max_len, workspace, query)
     sq, sc, so = query.stride(), key_cache.stride(), out.stride()
-    with torch.cuda.device(dev):
+    with launch_on(dev) as stream:
         check("ex_tree_attention", lib().ex_tree_attention(
             query.data_ptr(), sq[0], sq[1], _DT16[query.dtype], key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0],
             sc[1], sc[2], ks, vs, ss[0], ss[1], nb, block_table.data_ptr(), block_table.stride(0), width,
             seq_lens.data_ptr(), query_start_loc.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), n,
             tokens, max_query_len, H, KV, D, BS, float(scale), max_len, out.data_ptr(), so[0], so[1],
-            workspace.data_ptr() if nbytes else None, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+            workspace.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
