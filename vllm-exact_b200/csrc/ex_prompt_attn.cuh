@@ -215,10 +215,46 @@ __device__ __forceinline__ void ex2_pair(f32x2 x, float& a, float& b) {
   b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
+// Two 16-bit values in a word: a bit (15, 31) for each that is not finite. One more than the largest exponent carries into the
+// place of the sign, and no further.
 template <bool F16>
-__device__ __forceinline__ bool finite_word(uint32_t w) {  // both halves
-  const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-  return (w & e) != e && ((w >> 16) & e) != e;
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return ((w & (F16 ? 0x7c007c00u : 0x7f807f80u)) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {  // zeros for the others
+  const uint32_t n = not_finite<F16>(w);
+  return w & ~((n >> 15) * 0xffffu);
+}
+
+// The 128 values of a slot (`columns` swizzled columns of 64 dims): those from number `live` on become zeros, and so do numbers
+// that are not finite, whose keys are noted. 16 bytes of a key a thread, eight threads along a key's 128 bytes (no bank
+// conflict; with a key a thread a block took 7000 cycles), four keys in flight.
+template <bool F16, int THREADS>
+__device__ __forceinline__ void clean_values(uint8_t* vs, int columns, int t, int live, uint32_t* noted) {
+  constexpr int STEP = THREADS / 8;  // keys side by side
+#pragma unroll 1
+  for (int r = t >> 3; r < 128 * columns; r += 4 * STEP) {
+    uint4* x = reinterpret_cast<uint4*>(vs + r * 128 + (t & 7) * 16);
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 w = x[i * STEP * 8];
+      bad |= not_finite<F16>(w.x) | not_finite<F16>(w.y) | not_finite<F16>(w.z) | not_finite<F16>(w.w);
+    }
+    if (live >= 128 && bad == 0) continue;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const int key = (r + i * STEP) & 127;
+      const uint4 v = x[i * STEP * 8];
+      if (key >= live) {
+        x[i * STEP * 8] = make_uint4(0, 0, 0, 0);
+      } else if (not_finite<F16>(v.x) | not_finite<F16>(v.y) | not_finite<F16>(v.z) | not_finite<F16>(v.w)) {
+        x[i * STEP * 8] = make_uint4(only_finite<F16>(v.x), only_finite<F16>(v.y), only_finite<F16>(v.z), only_finite<F16>(v.w));
+        atomicOr(noted + (key >> 5), 1u << (key & 31));
+      }
+    }
+  }
 }
 
 template <int D, bool F16>
@@ -232,12 +268,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   uint64_t* bar = reinterpret_cast<uint64_t*>(ring + C::SLOTS * C::SLOT);
   uint64_t* full_bar = bar;            // [8] ring slots
   uint64_t* empty_bar = bar + 8;       // [8]
-  uint64_t* q_bar = bar + 16;
-  uint64_t* s_bar = bar + 17;          // [2] S of a tile (D = 256: of a buffer) is there
-  uint64_t* p_bar = bar + 19;          // [2] P of a tile (buffer) is there
-  uint64_t* o_bar = bar + 21;          // D = 256: P V of a block is done
-  uint64_t* end_bar = bar + 22;        // every product is done
-  uint64_t* ask_bar = bar + 23;        // [PA_EDGES] loads of an edge block's values have been issued
+  uint64_t* q_bar = bar + 16;          // [2] the queries of a tile
+  uint64_t* s_bar = bar + 18;          // [2] S of a tile (D = 256: of a buffer) is there
+  uint64_t* p_bar = bar + 20;          // [2] P of a tile (buffer) is there
+  uint64_t* o_bar = bar + 22;          // D = 256: P V of a block is done
+  uint64_t* end_bar = bar + 23;        // every product is done
+  uint64_t* ask_bar = bar + 24;        // [PA_EDGES] loads of an edge block's values have been issued
   uint64_t* fix_bar = ask_bar + PA_EDGES;  // [PA_EDGES] they have been looked at
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix_bar + PA_EDGES);
   uint32_t* poison = tmem_slot + 1;    // [16] edge keys with a value that is not finite
@@ -252,8 +288,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       mbar_init(full_bar + i, 1);
       mbar_init(empty_bar + i, 1);
     }
-    mbar_init(q_bar, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(q_bar + i, 1);
       mbar_init(s_bar + i, 1);
       mbar_init(p_bar + i, 128);
     }
@@ -297,10 +333,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     if (warp == 9) {
       // -------------------------------------------------------------------------------------------- TMA producer
       if (lane == 0 && nmax > 0) {
-        mbar_arrive_expect_tx(q_bar, C::Q_BYTES);
+        auto load_q = [&](int tile) {
+          mbar_arrive_expect_tx(q_bar + tile, C::Q_BYTES / C::NQ);
 #pragma unroll
-        for (int i = 0; i < C::NQ * (D / 64); ++i)
-          tma_load_3d(smem + i * C::SUB, &tm_q, q_bar, (i % (D / 64)) * 64, h, q0 + row0 + (i / (D / 64)) * 128);
+          for (int i = 0; i < D / 64; ++i)
+            tma_load_3d(smem + (tile * (D / 64) + i) * C::SUB, &tm_q, q_bar + tile, i * 64, h, q0 + row0 + tile * 128);
+        };
+        load_q(0);
         int slot = 0, made = 0;
         uint32_t ph = 1;
         bool ok = true;
@@ -318,6 +357,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         };
         // in the order of use: S of a block is issued one block ahead of P V
         load(&tm_k, 0);
+        if (C::NQ == 2) load_q(C::NQ - 1);
         if (C::NQ == 1 && nmax > 1) load(&tm_k, 1);
         for (int j = 0; j < nmax && ok; ++j) {
           load(&tm_v, j);
@@ -325,7 +365,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const int k = j + (C::NQ == 1 ? 2 : 1);
           if (k < nmax) load(&tm_k, k);
         }
-        mbar_wait(q_bar, 0, EX_DEVERR_WAIT_TMA);  // every load has landed before the CTA ends
+        for (int i = 0; i < C::NQ; ++i) mbar_wait(q_bar + i, 0, EX_DEVERR_WAIT_TMA);  // every load has landed before the CTA ends
         for (int i = max(0, made - C::SLOTS); i < made; ++i)
           mbar_wait(full_bar + i % C::SLOTS, (uint32_t)(i / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
       }
@@ -373,6 +413,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             issue_s(0, 0, 0, 0);
             commit(s_bar);
           }
+          mbar_wait(q_bar + 1, 0, EX_DEVERR_WAIT_TMA);
+          __syncwarp();
+          tc_fence_after();
           if (n1 > 0) {
             issue_s(0, 1, 1, 0);
             commit(s_bar + 1);
@@ -444,32 +487,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const int at = C::NQ == 1 ? (min(j + 2, nmax) + j) * C::PARTS + p : 2 * j + 1;
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
           ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
-          // 16 bytes of a key a thread, eight threads along a key's 128 bytes (no bank conflict), four keys in flight
-          const int sub = t & 7;
-#pragma unroll 1
-          for (int r = t >> 3; r < PA_KEYS * (C::SW / 64) && ok; r += 32) {
-            uint4 w[4];
-            uint4* x = reinterpret_cast<uint4*>(vs + r * 128 + sub * 16);  // row r of the slot's columns of 128 keys
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = x[i * 64];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = j * PA_KEYS + ((r + 8 * i) & (PA_KEYS - 1));
-              if (key >= Lk) {
-                x[i * 64] = make_uint4(0, 0, 0, 0);
-              } else if (!(finite_word<F16>(w[i].x) && finite_word<F16>(w[i].y) && finite_word<F16>(w[i].z) && finite_word<F16>(w[i].w))) {
-                uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
-                  if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
-                }
-                x[i * 64] = make_uint4(u[0], u[1], u[2], u[3]);
-                const int k = key - edge * PA_KEYS;
-                if (k < 512) atomicOr(poison + (k >> 5), 1u << (k & 31));
-              }
-            }
-          }
+          if (ok && j - edge < PA_EDGES) clean_values<F16, 64>(vs, C::SW / 64, t, Lk - j * PA_KEYS, poison + (j - edge) * 4);
         }
         fence_proxy_async_shared();  // the products read shared memory through the async proxy
         if (ok) mbar_arrive(fix_bar + (j - edge));

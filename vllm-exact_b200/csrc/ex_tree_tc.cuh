@@ -406,31 +406,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
           ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
           ok = __all_sync(0xffffffffu, ok);
-#pragma unroll 1
-          for (int r = lane; r < 128 && ok; r += 32) {
-            const int key = start + j * 128 + r;
-            bool bad = false;
-#pragma unroll 1
-            for (int c = 0; c < C::SW / 8; ++c) {
-              uint4* x = reinterpret_cast<uint4*>(vs + (c >> 3) * C::SUB + r * 128 + (c & 7) * 16);
-              if (key >= end) {
-                *x = make_uint4(0, 0, 0, 0);
-              } else {
-                const uint4 w = *x;
-                if (!(finite_word<F16>(w.x) && finite_word<F16>(w.y) && finite_word<F16>(w.z) && finite_word<F16>(w.w))) {
-                  bad = true;
-                  uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    if (!finite_word<F16>(u[k] & 0xffffu)) u[k] &= 0xffff0000u;
-                    if (!finite_word<F16>(u[k] & 0xffff0000u)) u[k] &= 0x0000ffffu;
-                  }
-                  *x = make_uint4(u[0], u[1], u[2], u[3]);
-                }
-              }
-            }
-            if (bad) atomicOr(mine + e * 4 + (r >> 5), 1u << (r & 31));
-          }
+          if (ok) clean_values<F16, 32>(vs, C::SW / 64, lane, end - start - j * 128, mine + e * 4);
         }
         fence_proxy_async_shared();  // the products read shared memory through the async proxy
         if (ok) mbar_arrive(fix_bar + (edges & (PTC_EDGES - 1)));
