@@ -133,6 +133,29 @@ def test_cache_write_is_the_rounded_formula(dtype, real, T, KV, D, page):
         assert torch.equal(torch.nan_to_num(back.cpu().float(), nan=-1.5), torch.nan_to_num(want_b.float(), nan=-1.5))
 
 
+@pytest.mark.parametrize("dtype", [I8, E4])
+@pytest.mark.parametrize("real", [BF, FP])
+def test_cache_write_quotients_are_those_of_the_division(dtype, real):
+    """Rows of every magnitude (scales down to the subnormal numbers, where the quotient is taken another way), values
+    over 2^14 below the largest, short mantissas among them, so that quotients lie on ties and next to them."""
+    from vllm_exact import kv_cache as C
+    g = gen(5)
+    T, KV, D, page = 700, 6, 128, 16
+    lo, hi = (-133, 127) if real == BF else (-24, 15)
+    e = torch.randint(lo, hi + 1, (T, 2, KV, 1), generator=g) - torch.randint(0, 15, (T, 2, KV, D), generator=g)
+    m = 1 + torch.randint(0, 256, (T, 2, KV, D), generator=g) / 256.0
+    m = torch.where(torch.rand(T, 2, KV, D, generator=g) < 0.3, 1 + torch.randint(0, 8, m.shape, generator=g) / 8.0, m)
+    x = (torch.ldexp(m.double(), e) * torch.where(torch.rand(m.shape, generator=g) < 0.5, -1.0, 1.0)).to(real)
+    assert bool(torch.isfinite(x).all()) and int((x != 0).sum()) > x.numel() // 2
+    kc, vc, ks, vs = C.alloc_q8_cache(T // page + 1, page, KV, D, dtype, DEV)
+    x = x.to(DEV)
+    C.cache_write(x[:, 0], x[:, 1], kc, vc, ks, vs, torch.arange(T, device=DEV))
+    for i, (codes, scale) in enumerate(((kc, ks), (vc, vs))):
+        q, s = S.quantise(x[:, i], dtype)
+        assert torch.equal(codes.cpu().view(-1, KV, D)[:T].float(), q.float())
+        assert torch.equal(scale.cpu().transpose(1, 2).reshape(-1, KV)[:T], s)
+
+
 def test_cache_write_without_values_and_empty():
     from vllm_exact import kv_cache as C
     kc, vc, ks, vs = C.alloc_q8_cache(4, 16, 8, 128, I8, DEV)
@@ -461,6 +484,19 @@ def test_tree_rows_left_untouched():
     assert not bool((got[:2] == 7.0).any()) and not bool((got[11:14] == 7.0).any())
     short = tree(c, q[:12], T, 0.1, None, most=9)  # the last request's rows are not all in q
     assert bool((short[11:] == 7.0).all()) and not bool((short[:11] == 7.0).any())
+
+
+@pytest.mark.parametrize("dtype", [None, E4])
+def test_tree_padded_batch(dtype):
+    """Rows behind the last request (a captured step of a fixed number of rows): the requests' bits are those of the batch
+    without them, the rows are left as they were."""
+    H, KV, D, most = 32, 8, 128, 8
+    T, lens = [1, 8, 3], [900, 2300, 40]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(most * len(T), H, D, generator=gen(14)).to(BF)
+    want = tree(c, q[:sum(T)], T, 0.1, None, most=most)
+    got = tree(c, q, T, 0.1, None, most=most)
+    assert torch.equal(got[:sum(T)], want) and bool((got[sum(T):] == 7.0).all())
 
 
 # ----------------------------------------------------------------------------------------------------------- prompt

@@ -324,11 +324,9 @@ cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& m
   a.rows_hi = ex::PR_FEW;
   if (rows <= 8) return launch_few_t<D, CODE, F16, 1>(mk, mv, a, per_tile, st);
   if (rows <= ex::PR_FEW) return launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
-  if (a.tokens != (int64_t)a.n * a.max_tokens) {  // else every request has max_tokens rows
-    const cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);
-    if (e != cudaSuccess) return e;
-    a.rows_lo = ex::PR_FEW;
-  }
+  const cudaError_t e = launch_few_t<D, CODE, F16, 2>(mk, mv, a, per_tile, st);  // (how many there are is known on the device)
+  if (e != cudaSuccess) return e;
+  a.rows_lo = ex::PR_FEW;
   a.rows_hi = INT32_MAX;
   using C = ex::PtcCfg<D, CODE>;
   static KernelReady ready;
@@ -442,12 +440,13 @@ cudaError_t launch_cache_write(const void* key, const void* value, int f16, int6
                                int64_t sv_h, const ex::CacheView& c, const int64_t* slots, int64_t tokens, int KV,
                                void* ko, void* vo, int64_t sko_t, int64_t sko_h, int64_t svo_t, int64_t svo_h,
                                cudaStream_t st) {
-  const dim3 grid((unsigned)cdiv(tokens * 2 * KV * (D / 8), ex::CQ_THREADS)), block(ex::CQ_THREADS);
+  const int64_t per_token = cdiv(2 * KV, (32 / (D / 8)) * ex::CQ_PASSES), items = tokens * per_token;  // a warp each
+  const dim3 grid((unsigned)cdiv(items, ex::CQ_THREADS / 32)), block(ex::CQ_THREADS);
   if (f16)
     return ex_launch_pdl(ex::k_cache_write<D, CODE, __half>, grid, block, 0, st, (const __half*)key, (const __half*)value,
-                         sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, (__half*)ko, (__half*)vo, sko_t, sko_h, svo_t, svo_h);
+                         sk_t, sk_h, sv_t, sv_h, c, slots, (uint32_t)items, (uint32_t)per_token, KV, (__half*)ko, (__half*)vo, sko_t, sko_h, svo_t, svo_h);
   return ex_launch_pdl(ex::k_cache_write<D, CODE, __nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16*)key,
-                       (const __nv_bfloat16*)value, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, (__nv_bfloat16*)ko,
+                       (const __nv_bfloat16*)value, sk_t, sk_h, sv_t, sv_h, c, slots, (uint32_t)items, (uint32_t)per_token, KV, (__nv_bfloat16*)ko,
                        (__nv_bfloat16*)vo, sko_t, sko_h, svo_t, svo_h);
 }
 
