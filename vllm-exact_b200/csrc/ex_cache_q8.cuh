@@ -102,14 +102,15 @@ struct CacheView {      // strides in elements
 
 constexpr int CQ_THREADS = 256;
 
-// A warp takes 4 passes of one token's rows (keys' heads, then values'), D / 8 lanes a row and 16 bytes a lane: 4 loads in
+// A warp takes PASSES (4) passes of one token's rows (keys' heads, then values'), D / 8 lanes a row and 16 bytes a lane: 4 loads in
 // flight a lane, and the token's slot looked up once. What bounds it is instructions: the quotients are therefore not
 // divisions but (Markstein, 1990) q = q0 + r (x - q0 s) with r = 1 / s and q0 = x r, all rounded to nearest, which is the
 // correctly rounded x / s as long as x - q0 s is exact: its last bit is at least 2^-46 |q| s, so it is for s >= 2^-80 where
 // |q| is not so small (under 2^-10) that its code is 0 anyway. Smaller scales take the division.
 // 16000 tokens of 8 heads of 128 with values read back, bf16 to e4m3: 34 us, 4.8 TB/s (one pass a warp and a division per value: 56 us).
-constexpr int CQ_PASSES = 4;
-template <int D, int CODE, typename T>
+// PASSES = 1 where all warps run at once even so: it is a chain of latencies then (16 tokens of 8 heads of 128: 2.3 us, with 4
+// passes 3.1 us).
+template <int D, int CODE, typename T, int PASSES>
 __global__ void __launch_bounds__(CQ_THREADS)
     k_cache_write(const T* __restrict__ key, const T* __restrict__ value, int64_t sk_t, int64_t sk_h, int64_t sv_t,
                   int64_t sv_h, CacheView c, const int64_t* __restrict__ slots, uint32_t items, uint32_t per_token, int KV,
@@ -122,12 +123,12 @@ __global__ void __launch_bounds__(CQ_THREADS)
   if (item >= items) return;
   const uint32_t token = item / per_token;
   const int64_t t = token;
-  const int first = (int)(item - token * per_token) * (ROWS * CQ_PASSES) + (threadIdx.x & 31) / LANES;
+  const int first = (int)(item - token * per_token) * (ROWS * PASSES) + (threadIdx.x & 31) / LANES;
   const int lane = threadIdx.x % LANES;
   const int64_t slot = slots[t];
-  uint4 v[CQ_PASSES];
+  uint4 v[PASSES];
 #pragma unroll
-  for (int i = 0; i < CQ_PASSES; ++i) {
+  for (int i = 0; i < PASSES; ++i) {
     const int r = first + i * ROWS;
     v[i] = make_uint4(0, 0, 0, 0);  // (every lane stays for the shuffles)
     if (r < 2 * KV) {
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(CQ_THREADS)
     place = (int)(slot - blk * c.page);
   }
 #pragma unroll
-  for (int i = 0; i < CQ_PASSES; ++i) {
+  for (int i = 0; i < PASSES; ++i) {
     const int r = first + i * ROWS;
     const bool is_v = r >= KV;
     const int h = is_v ? r - KV : r;

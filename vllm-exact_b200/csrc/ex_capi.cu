@@ -435,19 +435,23 @@ int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
                                  ex::PA_THREADS, C::SMEM, st, mq, mk, mv, a));
 }
 
-template <int D, int CODE>
-cudaError_t launch_cache_write(const void* key, const void* value, int f16, int64_t sk_t, int64_t sk_h, int64_t sv_t,
-                               int64_t sv_h, const ex::CacheView& c, const int64_t* slots, int64_t tokens, int KV,
-                               void* ko, void* vo, int64_t sko_t, int64_t sko_h, int64_t svo_t, int64_t svo_h,
-                               cudaStream_t st) {
-  const int64_t per_token = cdiv(2 * KV, (32 / (D / 8)) * ex::CQ_PASSES), items = tokens * per_token;  // a warp each
+template <int D, int CODE, int PASSES, typename T>
+cudaError_t launch_cache_write_t(const void* key, const void* value, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
+                                 const ex::CacheView& c, const int64_t* slots, int64_t tokens, int KV, void* ko, void* vo,
+                                 int64_t sko_t, int64_t sko_h, int64_t svo_t, int64_t svo_h, cudaStream_t st) {
+  const int64_t per_token = cdiv(2 * KV, (32 / (D / 8)) * PASSES), items = tokens * per_token;  // a warp each
   const dim3 grid((unsigned)cdiv(items, ex::CQ_THREADS / 32)), block(ex::CQ_THREADS);
-  if (f16)
-    return ex_launch_pdl(ex::k_cache_write<D, CODE, __half>, grid, block, 0, st, (const __half*)key, (const __half*)value,
-                         sk_t, sk_h, sv_t, sv_h, c, slots, (uint32_t)items, (uint32_t)per_token, KV, (__half*)ko, (__half*)vo, sko_t, sko_h, svo_t, svo_h);
-  return ex_launch_pdl(ex::k_cache_write<D, CODE, __nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16*)key,
-                       (const __nv_bfloat16*)value, sk_t, sk_h, sv_t, sv_h, c, slots, (uint32_t)items, (uint32_t)per_token, KV, (__nv_bfloat16*)ko,
-                       (__nv_bfloat16*)vo, sko_t, sko_h, svo_t, svo_h);
+  return ex_launch_pdl(ex::k_cache_write<D, CODE, T, PASSES>, grid, block, 0, st, (const T*)key, (const T*)value, sk_t, sk_h,
+                       sv_t, sv_h, c, slots, (uint32_t)items, (uint32_t)per_token, KV, (T*)ko, (T*)vo, sko_t, sko_h, svo_t, svo_h);
+}
+template <int D, int CODE, typename T>
+cudaError_t launch_cache_write(const void* key, const void* value, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
+                               const ex::CacheView& c, const int64_t* slots, int64_t tokens, int KV, void* ko, void* vo,
+                               int64_t sko_t, int64_t sko_h, int64_t svo_t, int64_t svo_h, cudaStream_t st) {
+  // one pass a warp while that leaves no warp waiting (64 of an SM run at once)
+  const bool few = tokens * cdiv(2 * KV, 32 / (D / 8)) <= 64 * (int64_t)num_sms();
+  return (few ? launch_cache_write_t<D, CODE, 1, T> : launch_cache_write_t<D, CODE, 4, T>)(
+      key, value, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, ko, vo, sko_t, sko_h, svo_t, svo_h, st);
 }
 
 template <int D, int CODE>
@@ -927,10 +931,10 @@ int ex_cache_write_q8(const void* key, int64_t sk_t, int64_t sk_h, const void* v
   const ex::CacheView c = cache_view(k_cache, v_cache, s_block, s_page, s_head, k_scale, v_scale, ss_block, ss_head, num_blocks, BS);
   cudaStream_t st = (cudaStream_t)stream;
   const int f16 = dtype == EX_DTYPE_F16;
-#define EX_CW(DD, CC)                                                                                              \
-  if (D == DD && code == CC)                                                                                       \
-    return cuda_status(launch_cache_write<DD, CC>(key, value, f16, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV,   \
-                                                  key_out, value_out, sko_t, sko_h, svo_t, svo_h, st));
+#define EX_CW(DD, CC)                                                                                                     \
+  if (D == DD && code == CC)                                                                                              \
+    return cuda_status((f16 ? launch_cache_write<DD, CC, __half> : launch_cache_write<DD, CC, __nv_bfloat16>)(            \
+        key, value, sk_t, sk_h, sv_t, sv_h, c, slots, tokens, KV, key_out, value_out, sko_t, sko_h, svo_t, svo_h, st));
   EX_CW(64, ex::CODE_INT8)
   EX_CW(128, ex::CODE_INT8)
   EX_CW(256, ex::CODE_INT8)
