@@ -389,7 +389,7 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   a.q = q; a.sq_t = sq_t; a.sq_h = sq_h; a.q_is_f16 = q_dtype == EX_DTYPE_F16;
   a.bt = block_table; a.sbt = sbt; a.seq_lens = seq_lens; a.qsl = qsl;
   a.mask = reinterpret_cast<const uint64_t*>(mask);
-  a.n = n; a.H = H; a.G = G; a.KV = KV; a.BS = BS; a.group_log2 = BS % 16 == 0 ? 4 : 3; a.max_tokens = max_tokens;
+  a.n = n; a.H = H; a.G = G; a.g_inv = (65536u + G - 1) / G; a.KV = KV; a.BS = BS; a.group_log2 = BS % 16 == 0 ? 4 : 3; a.max_tokens = max_tokens;
   a.max_keys = (int)max_len; a.blocks = num_blocks; a.tokens = tokens; a.scale_log2 = scale * ex::PR_LOG2E;
   a.k_scale = k_scale; a.v_scale = v_scale; a.ss_block = ss_block; a.ss_head = ss_head; a.NS = NS;
   if (need > 0) {

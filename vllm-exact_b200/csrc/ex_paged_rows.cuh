@@ -19,28 +19,21 @@
 #include "ex_paged_decode.cuh"
 #include "ex_paged_decode_tma.cuh"
 
-#ifndef XSEG_A
-#define XSEG_A 256
-#define XSEG_B 512
-#endif
-#ifndef XTSEG
-#define XTSEG(L) ((L) <= 2048 ? 512 : 2048)
-#endif
-#ifndef XNW
-#define XNW ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 12 : (CODE == CODE_NONE ? 2 : 1) * D <= 256 ? 8 : 4)
-#endif
-#ifndef XMK
-#define XMK ((CODE == CODE_NONE ? 2 : 1) * D <= 128 ? 2 : 1)
-#endif
 namespace ex {
 
 constexpr int PR_MAX_TOKENS = 64;  // drafted tokens of a request (bits of a mask word)
 constexpr float PR_LOG2E = 1.4426950408889634f;
 
-// Keys a segment, by the request's own length; of requests with at most 16 rows a KV head, and with more (whose results take
-// more memory traffic a segment).
-__host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? XSEG_A : XSEG_B; }
-__host__ __device__ inline int pr_segment_many(int64_t L) { return XTSEG(L); }
+// Keys a segment, by the request's own length alone: the order of its sums must not depend on the batch. Short segments spread
+// a request over more SMs; every segment costs its partial results' traffic, and with many rows a CTA's start and end (15000
+// cycles of a 2048-key segment's 45000).
+// At most 16 rows a KV head: 256 up to 2048 keys (256 requests of 1024 keys, e4m3: 120 us; 128: 131; 64: 160; one request of
+// 1000 keys: 19, 16, 16 us), 512 behind (16 requests of 16384 keys, int8: 130 us; 256: 142; 1024: 136; one such request:
+// 31, 31, 44 us).
+__host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? 256 : 512; }
+// More rows: 512, from 2048 keys on 2048 (64 requests of 8192 keys, 16 tokens: 455 us; 1024: 613; 32 requests, D = 256: 212,
+// with 4096: 252 us), from 12288 keys on 4096 (16 requests of 16384 keys, e4m3: 242 us; 2048: 268; 8192: 328).
+__host__ __device__ inline int pr_segment_many(int64_t L) { return L <= 2048 ? 512 : L <= 12288 ? 2048 : 4096; }
 __host__ __device__ inline int pr_segments(int64_t L) {
   const int s = pr_segment(L), n = (int)((L + s - 1) / s);
   return n < 1 ? 1 : n;
@@ -84,6 +77,7 @@ struct PrArgs {
   const float* v_scale;
   int64_t ss_block, ss_head;
   int NS;
+  uint32_t g_inv;            // ceil(2^16 / G): x / G is x g_inv >> 16 for x < 4096 (G <= 16)
   int rows_lo, rows_hi;      // requests with rows_lo < T G <= rows_hi are this kernel's
   float* ws_m;
   float* ws_l;
@@ -223,8 +217,12 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
 // ------------------------------------------------------------------------------------------------------------------
 template <int D, int CODE, int NT>
 struct PfCfg {
-  static constexpr int MK = XMK;                       // 16-key tiles of a block
-  static constexpr int NW = XNW;                       // warps of a CTA, one CTA per SM
+  static constexpr int ROW = (CODE == CODE_NONE ? 2 : 1) * D;  // bytes of a key
+  // 16-key tiles of a block: two where the registers have room for them (256 requests of 1024 keys, e4m3: 119 us, with one 133)
+  static constexpr int MK = ROW <= 128 ? 2 : 1;
+  // Warps of a CTA, one CTA per SM: as many as rings of enough blocks fit in shared memory and results in registers (the same
+  // batch: 12 warps 119 us, 8 124, 4 186; 64 requests of 8192 keys, D = 256: 8 warps 207 us, 4 294)
+  static constexpr int NW = ROW <= 128 ? 12 : ROW <= 256 ? 8 : 4;
   static constexpr int BLK = 16 * MK;
   using R = PrTile<D, CODE, BLK>;
   static constexpr int STAGE = 2 * R::TILE;

@@ -14,7 +14,7 @@
 //   warps 12-15, for codes 9-11   producers: TMA boxes of 8 or 16 tokens through the block table into a ring of slots. Issuing
 //                   a box takes a warp about 75 cycles (its operands are uniform registers), 16 boxes of a 32 KB tile longer
 //                   than HBM takes to deliver it: so several warps share the boxes of every tile.
-//   warp 10         16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
+//   warps 10, 11    16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
 //                   are not finite are zeroed and noted, and added in the end to the rows that see them
 //   warps 12-15     for codes: codes to float16 tiles (exact; keys behind the end to zeros)
 // Bound by reading the cache once: a block of 128 keys of a 16-bit cache is 64 KB (D = 128), 1.5 us of an SM's share of HBM;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     }
     for (int i = 0; i < PTC_EDGES; ++i) {
       mbar_init(ask_bar + i, C::FEEDERS);
-      mbar_init(fix_bar + i, 32);
+      mbar_init(fix_bar + i, 64);
     }
     mbar_init(done_bar, 1);
     mbar_init(q_bar, 256);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     commit(done_bar);
     mbar_wait(done_bar, 0, EX_DEVERR_WAIT_MMA);
     __syncwarp();
-  } else if (warp == 10 && !Q8) {
+  } else if ((warp == 10 || warp == 11) && !Q8) {
     // ---------------------------------------------------------------------------------------------- edge values
     int base = 0;   // slots of the items before
     uint32_t edges = 0;
@@ -394,8 +394,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     while (ok && next()) {
       uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
       if (jedge < nblk) {
-        if (lane < 8) mine[lane] = 0;
-        __syncwarp();
+        if (warp == 10 && lane < 8) mine[lane] = 0;
+        asm volatile("bar.sync 6, 64;" ::: "memory");
       }
       for (int j = jedge; j < nblk && ok; ++j) {
         const int e = j - jedge;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           uint8_t* vs = ring + (at % C::SLOTS) * C::SLOT;
           ok = mbar_wait(full_bar + at % C::SLOTS, (uint32_t)(at / C::SLOTS) & 1u, EX_DEVERR_WAIT_TMA);
           ok = __all_sync(0xffffffffu, ok);
-          if (ok) clean_values<F16, 32>(vs, C::SW / 64, lane, end - start - j * 128, mine + e * 4);
+          if (ok) clean_values<F16, 64>(vs, C::SW / 64, tid & 63, end - start - j * 128, mine + e * 4);
         }
         fence_proxy_async_shared();  // the products read shared memory through the async proxy
         if (ok) mbar_arrive(fix_bar + (edges & (PTC_EDGES - 1)));
@@ -470,8 +470,61 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t phs[2] = {0, 0}, pho = 0, phe = 0, blocks = 0;
     int item = 0;
-    bool ok = true;
-    while (ok && next()) {
+    // The queries of an item: row-major in swizzled columns of 64 dims, D / 8 lanes a row. Up to D = 128 they are loaded (QN
+    // pieces a thread) while the products of the item before still run; codes leave no registers for it (with it 3 % slower).
+    constexpr int LANES = D / 8, QSTEP = 256 / LANES, QN = 128 / QSTEP;
+    constexpr bool AHEAD = D <= 128 && !Q8;
+    const int qc = tid % LANES, qx = tid / LANES;
+    uint4 qv[AHEAD ? QN : 1];
+    auto load_q = [&](int x) {
+      const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1, xl = copies == 1 ? row0 + x : x & (128 / copies - 1);
+      if (xl >= R) return make_uint4(0, 0, 0, 0);
+      const int t = (int)((uint32_t)xl * a.g_inv >> 16);
+      return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + t) * a.sq_t +
+                                             (int64_t)(g * a.G + xl - t * a.G) * a.sq_h + qc * 8);
+    };
+    auto put_q = [&](int x, uint4 v) {
+      if constexpr (Q8) {
+        float f = 1.0f;
+        if (!a.q_is_f16) {
+          float y[8];
+          unpack2<__nv_bfloat16>(v.x, y[0], y[1]);
+          unpack2<__nv_bfloat16>(v.y, y[2], y[3]);
+          unpack2<__nv_bfloat16>(v.z, y[4], y[5]);
+          unpack2<__nv_bfloat16>(v.w, y[6], y[7]);
+          float mq = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mq = fmaxf(mq, fabsf(y[i]));
+#pragma unroll
+          for (int o = LANES / 2; o; o >>= 1) mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, o));
+          const float inv = pr_query_scale(mq, f);
+          v.x = pack2<__half>(y[0] * inv, y[1] * inv);
+          v.y = pack2<__half>(y[2] * inv, y[3] * inv);
+          v.z = pack2<__half>(y[4] * inv, y[5] * inv);
+          v.w = pack2<__half>(y[6] * inv, y[7] * inv);
+        }
+        if (qc == 0) sfac[x] = f * fabsf(a.scale_log2);
+      }
+      if (a.scale_log2 < 0.0f) {  // the largest score is looked for before it is scaled
+        v.x ^= 0x80008000u;
+        v.y ^= 0x80008000u;
+        v.z ^= 0x80008000u;
+        v.w ^= 0x80008000u;
+      }
+      *reinterpret_cast<uint4*>(smem + (qc >> 3) * C::SUB + x * 128 + (((qc & 7) ^ (x & 7)) << 4)) = v;
+    };
+    auto next_item = [&]() {  // the next item and, in registers, its queries
+      const bool more = next();
+      if constexpr (AHEAD) {
+        if (more && nblk > 0) {
+#pragma unroll
+          for (int i = 0; i < QN; ++i) qv[i] = load_q(qx + i * QSTEP);
+        }
+      }
+      return more;
+    };
+    bool more = next_item();
+    while (more) {
       const uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
       // copies of the rows: each weighs W keys of a block
       const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1, rows = 128 / copies, W = 128 / copies;
@@ -480,45 +533,18 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       const bool active = copies > 1 || row0 + (warp & 3) * 32 < R;  // some row of this warp is real
       float m = -INFINITY, l = 0.0f, vref = 0.0f, vinv = 0.0f;
       if (nblk > 0) {
-        // queries: row-major in swizzled columns of 64 dims; D/8 lanes a row
-        constexpr int LANES = D / 8;
-        const int c = tid % LANES;
-        for (int x = tid / LANES; x < 128; x += 256 / LANES) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          const int xl = copies == 1 ? row0 + x : x & (rows - 1);
-          if (xl < R) {
-            const int t = xl / a.G, h = xl % a.G;
-            v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(first + t) * a.sq_t +
-                                                (int64_t)(g * a.G + h) * a.sq_h + c * 8);
-          }
-          if constexpr (Q8) {
-            float f = 1.0f;
-            if (!a.q_is_f16) {
-              float y[8];
-              unpack2<__nv_bfloat16>(v.x, y[0], y[1]);
-              unpack2<__nv_bfloat16>(v.y, y[2], y[3]);
-              unpack2<__nv_bfloat16>(v.z, y[4], y[5]);
-              unpack2<__nv_bfloat16>(v.w, y[6], y[7]);
-              float mq = 0.0f;
+        if constexpr (AHEAD) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) mq = fmaxf(mq, fabsf(y[i]));
+          for (int i = 0; i < QN; ++i) put_q(qx + i * QSTEP, qv[i]);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < QN; i += 4) {
+            uint4 v[4];
 #pragma unroll
-              for (int o = LANES / 2; o; o >>= 1) mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, o));
-              const float inv = pr_query_scale(mq, f);
-              v.x = pack2<__half>(y[0] * inv, y[1] * inv);
-              v.y = pack2<__half>(y[2] * inv, y[3] * inv);
-              v.z = pack2<__half>(y[4] * inv, y[5] * inv);
-              v.w = pack2<__half>(y[6] * inv, y[7] * inv);
-            }
-            if (c == 0) sfac[x] = f * fabsf(a.scale_log2);
+            for (int k = 0; k < 4; ++k) v[k] = load_q(qx + (i + k) * QSTEP);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) put_q(qx + (i + k) * QSTEP, v[k]);
           }
-          if (a.scale_log2 < 0.0f) {  // the largest score is looked for before it is scaled
-            v.x ^= 0x80008000u;
-            v.y ^= 0x80008000u;
-            v.z ^= 0x80008000u;
-            v.w ^= 0x80008000u;
-          }
-          *reinterpret_cast<uint4*>(smem + (c >> 3) * C::SUB + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
         }
         fence_proxy_async_shared();
         tc_fence_before();  // the last item's O has been read
@@ -528,7 +554,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       const float fac = Q8 ? sfac[r] : fabsf(a.scale_log2);
       uint64_t word = 0;
       if (rl < R) {
-        const int t = rl / a.G;
+        const int t = (int)((uint32_t)rl * a.g_inv >> 16);
         word = (a.mask ? a.mask[first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - T));  // (T >= 1)
       }
       const uint32_t all_good = (uint32_t)((1ull << (128 >> a.group_log2)) - 1ull);
@@ -571,7 +597,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           }
           // One step of 32 or 64 columns keeps its scores; more are read twice. Blocks that are not seen whole take a loop of
           // their own, in steps of 32.
-          float x[64];
+          constexpr int STEP = Q8 ? 32 : 64;
+          float x[STEP];
           auto masked = [&](int q) {
             float (&y)[32] = reinterpret_cast<float (&)[32]>(x);
             ptc_scores<Q8>(s_addr + col + q * 32, ks + col + q * 32, y);
@@ -592,8 +619,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             mb = ptc_max(reinterpret_cast<float (&)[32]>(x));
           } else {
 #pragma unroll 1
-            for (int q = W / 64 - 1; q >= 0; --q) {  // (the first 64 last: they are kept)
-              ptc_scores<Q8>(s_addr + col + q * 64, ks + col + q * 64, x);
+            for (int q = W / STEP - 1; q >= 0; --q) {  // (the first step last: it is kept)
+              ptc_scores<Q8>(s_addr + col + q * STEP, ks + col + q * STEP, x);
               mb = fmaxf(mb, ptc_max(x));
             }
           }
@@ -647,9 +674,9 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             l += ptc_weights<Q8, MF16>(p_addr, vs, fac, sub, vinv, reinterpret_cast<float (&)[32]>(x));
           } else {
 #pragma unroll 1
-            for (int q = 0; q < W / 64; ++q) {
-              if (q > 0) ptc_scores<Q8>(s_addr + col + q * 64, ks + col + q * 64, x);
-              l += ptc_weights<Q8, MF16>(p_addr + q * 32, vs + q * 64, fac, sub, vinv, x);
+            for (int q = 0; q < W / STEP; ++q) {
+              if (q > 0) ptc_scores<Q8>(s_addr + col + q * STEP, ks + col + q * STEP, x);
+              l += ptc_weights<Q8, MF16>(p_addr + q * (STEP / 2), vs + q * STEP, fac, sub, vinv, x);
             }
           }
           if (copies > 1) {  // no weight of this copy for the other keys
@@ -663,10 +690,13 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         tc_fence_before();
         mbar_arrive(p_bar + buf);
       }
+      // the item as the results need it; the next one is looked up, and its queries are loaded, while the last products run
+      struct { int b, first, T, L, g, s, row0, R, start, end, ctx, nblk, jedge; } const w = {b, first, T, L, g, s, row0, R, start, end, ctx, nblk, jedge};
+      more = next_item();
       // the streams and copies of each row, CD dims at a time through shared memory (over the queries); four warps each
       // take every other piece of the head dimension
-      if (nblk > 0 && !mbar_wait(end_bar, phe, EX_DEVERR_WAIT_MMA)) *sfail = 1;
-      if (nblk > 0) phe ^= 1;
+      if (w.nblk > 0 && !mbar_wait(end_bar, phe, EX_DEVERR_WAIT_MMA)) *sfail = 1;
+      if (w.nblk > 0) phe ^= 1;
       asm volatile("bar.sync 2, 256;" ::: "memory");  // (every product is done: the queries may be written over)
       if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
       tc_fence_after();
@@ -675,8 +705,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       sm[256 + wg * 128 + r] = l;
       sm[512 + wg * 128 + r] = vref;
       asm volatile("bar.sync 2, 256;" ::: "memory");
-      pho += nblk;
-      blocks += nblk;
+      pho += w.nblk;
+      blocks += w.nblk;
       float mall = -INFINITY, lall = 0.0f, f[2];
       for (int k = 0; k < copies; ++k) {
         const int x = copies == 1 ? r : (r & (rows - 1)) + k * rows;
@@ -690,10 +720,10 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         f[i] = sm[i * 128 + r] == -INFINITY ? 0.0f : ex2(sm[i * 128 + r] - sub) * (Q8 ? sm[512 + i * 128 + r] : 1.0f);
-      const bool have1 = C::STREAMS == 2 && nblk > 1;
-      const bool single = pr_segments_many(pr_keys(a, L)) == 1;
+      const bool have1 = C::STREAMS == 2 && w.nblk > 1;
+      const bool single = pr_segments_many(pr_keys(a, w.L)) == 1;
       bool any = false;
-      if (!Q8 && jedge < nblk)
+      if (!Q8 && w.jedge < w.nblk)
         for (int i = 0; i < 8; ++i) any |= mine[i] != 0;
       const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
       asm volatile("bar.sync 2, 256;" ::: "memory");  // sm has been read
@@ -702,56 +732,50 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
 #pragma unroll 1
       for (int c = wg * CD; c < D; c += 2 * CD) {
         if (active) {
-          uint32_t u[CD];
-          float o[CD];
-#pragma unroll
-          for (int i = 0; i < CD; ++i) o[i] = 0.0f;
-          if (nblk > 0) {
-            tmem_ld_n<CD>(tmem + lanes + TM_O + c, u);
+#pragma unroll 1
+          for (int k = 0; k < CD; k += 16) {
+            uint32_t u[16] = {}, v[16] = {};
+            if (w.nblk > 0) tmem_ld16(tmem + lanes + TM_O + c + k, u);
+            if (have1) tmem_ld16(tmem + lanes + TM_O + D + c + k, v);
             tmem_ld_wait();
+            float o[16];
 #pragma unroll
-            for (int i = 0; i < CD; ++i) o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
+            for (int i = 0; i < 16; ++i) {
+              o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
+              o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(v[i]) * f[1];
+              if (single) o[i] *= inv;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(piece + r * CD + ((((k + i) >> 2) ^ (r & (CD / 4 - 1))) << 2)) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
-          if (have1) {
-            tmem_ld_n<CD>(tmem + lanes + TM_O + D + c, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < CD; ++i) o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[1];
-          }
-          if (single) {
-#pragma unroll
-            for (int i = 0; i < CD; ++i) o[i] *= inv;
-          }
-#pragma unroll
-          for (int i = 0; i < CD; i += 4)
-            *reinterpret_cast<float4*>(piece + r * CD + (((i >> 2) ^ (r & (CD / 4 - 1))) << 2)) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
         if (wg == 0) asm volatile("bar.sync 4, 128;" ::: "memory");
         else asm volatile("bar.sync 5, 128;" ::: "memory");
-        const int real = copies == 1 ? min(128, R - row0) : R;
-        for (int i = t2; i < real * (CD / 4); i += 128) {
-          const int x = i / (CD / 4), q = i % (CD / 4);
+        const int real = copies == 1 ? min(128, w.R - w.row0) : w.R, q = t2 % (CD / 4), d0 = c + q * 4;
+#pragma unroll 2
+        for (int x = t2 / (CD / 4); x < real; x += 128 / (CD / 4)) {
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           for (int k = 0; k < copies; ++k) {
             const int y = x + k * rows;
-            const float4 w = *reinterpret_cast<const float4*>(piece + y * CD + ((q ^ (y & (CD / 4 - 1))) << 2));
-            v.x += w.x;
-            v.y += w.y;
-            v.z += w.z;
-            v.w += w.w;
+            const float4 z = *reinterpret_cast<const float4*>(piece + y * CD + ((q ^ (y & (CD / 4 - 1))) << 2));
+            v.x += z.x;
+            v.y += z.y;
+            v.z += z.z;
+            v.w += z.w;
           }
-          const int row = row0 + x, t = row / a.G, h = g * a.G + row % a.G, d0 = c + q * 4;
+          const int row = w.row0 + x, t = (int)((uint32_t)row * a.g_inv >> 16), h = w.g * a.G + row - t * a.G;
           if (any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
-            const uint64_t rw = (a.mask ? a.mask[first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - T));
+            const uint64_t rw = (a.mask ? a.mask[w.first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - w.T));
 #pragma unroll 1
             for (int k = 0; k < 256; ++k) {
               if (!((mine[k >> 5] >> (k & 31)) & 1u)) continue;
-              const int key = start + jedge * 128 + k, d = key - ctx;
-              if (key >= end || (d >= 0 && !((rw >> d) & 1ull))) continue;
-              const int page = a.bt[(int64_t)b * a.sbt + key / a.BS];
+              const int key = w.start + w.jedge * 128 + k, d = key - w.ctx;
+              if (key >= w.end || (d >= 0 && !((rw >> d) & 1ull))) continue;
+              const int page = a.bt[(int64_t)w.b * a.sbt + key / a.BS];
               if (page < 0 || page >= a.blocks) continue;
               const uint16_t* e = reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
-                                  (int64_t)(key % a.BS) * s_page + (int64_t)g * s_head + d0;
+                                  (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0;
               float y[4];
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
@@ -766,19 +790,20 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           }
           if (single) {
             const bool f16 = Q8 ? a.q_is_f16 != 0 : F16;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)(first + t) * a.so_t +
+            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)(w.first + t) * a.so_t +
                                                         (int64_t)h * a.so_h + d0);
             dst[0] = f16 ? pack2<__half>(v.x, v.y) : pack_bf16(v.x, v.y);
             dst[1] = f16 ? pack2<__half>(v.z, v.w) : pack_bf16(v.z, v.w);
           } else {
-            *reinterpret_cast<float4*>(a.ws_acc + (((int64_t)(first + t) * a.H + h) * a.NS + s) * D + d0) = v;
+            *reinterpret_cast<float4*>(a.ws_acc + (((int64_t)(w.first + t) * a.H + h) * a.NS + w.s) * D + d0) = v;
           }
         }
         if (wg == 0) asm volatile("bar.sync 4, 128;" ::: "memory");
         else asm volatile("bar.sync 5, 128;" ::: "memory");
       }
-      if (wg == 0 && !single && rl < R && (copies == 1 || r < rows)) {
-        const int64_t pi = ((int64_t)(first + rl / a.G) * a.H + g * a.G + rl % a.G) * a.NS + s;
+      if (wg == 0 && !single && rl < w.R && (copies == 1 || r < rows)) {
+        const int rt = (int)((uint32_t)rl * a.g_inv >> 16);
+        const int64_t pi = ((int64_t)(w.first + rt) * a.H + w.g * a.G + rl - rt * a.G) * a.NS + w.s;
         a.ws_m[pi] = mall;
         a.ws_l[pi] = lall;
       }
