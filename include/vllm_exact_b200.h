@@ -310,6 +310,7 @@ size_t ex_paged_rows_workspace_bytes(int64_t tokens, int H, int D, int64_t max_l
  *   - tokens behind max_len or behind the block table (n x width), and tokens on pages outside [0, num_blocks), are
  *     not seen
  *   - scales must start on 16 bytes, their strides be multiples of 4
+ *   - scale: finite and not 0 (EX_ERR_ARG)
  */
 int ex_paged_decode_q8(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
                        int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,
@@ -340,7 +341,8 @@ int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, co
  * key rows cu_k[b] .. cu_k[b + 1] of k and v (keys x KV x D), all bf16 or all fp16; its last query is its last key's
  * token, so query i sees keys j <= i + Lk - Lq (the keys may start before the queries: a continued conversation). A
  * query that sees no key gives zeros. Rows of no sequence are left untouched; a sequence whose offsets leave the
- * arrays is skipped. scale must be positive. A row's bits depend on its own sequence alone.
+ * arrays is skipped. scale must be positive and finite. A row's bits depend on its own query and on the keys and values of its
+ * sequence that it sees, alone: a prompt in pieces, each over all keys so far, gives the bits of the whole.
  */
 int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
                         const void* v, int64_t sv_t, int64_t sv_h, int dtype, const int32_t* cu_q, const int32_t* cu_k,

@@ -620,7 +620,71 @@ def test_prompt_attention_graph():
     del g
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_attention_in_pieces(D):
+    """A prompt whose last queries come by themselves, over all keys so far, has the bits of the whole."""
+    H, KV, L = 4, 2, 700
+    g = gen(12)
+    q = torch.randn(L, H, D, generator=g).to(BF).to(DEV)
+    k, v = (torch.randn(L, KV, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    q[650] *= 30  # a row whose largest score grows late, with its neighbours'
+    whole = prompt(q, k, v, [L], [L], 0.2)
+    for lo, hi in ((0, 130), (130, 500), (500, 501), (501, 700)):
+        assert torch.equal(prompt(q[lo:hi], k[:hi], v[:hi], [hi - lo], [hi], 0.2), whole[lo:hi]), (lo, hi)
+
+
 # ---------------------------------------------------------------------------------------------------------- together
+def test_calls_on_two_streams_at_once():
+    """Prompt, decode and draft calls of two streams, each with its own outputs and workspaces, in flight together."""
+    from vllm_exact import paged_attn as P, prompt_attn as A
+    H, KV, D = 16, 4, 128
+    g = gen(13)
+    T, lens = [20, 3], [3000, 700]
+    caches = [Cache(lens, 16, KV, D, E4), Cache(lens, 16, KV, D, None)]
+    q = torch.randn(600, H, D, generator=g).to(BF).to(DEV)
+    kv = torch.randn(600, 2, KV, D, generator=g).to(BF).to(DEV)
+    cq, ct = cu([400, 200]), cu(T)
+
+    def run():
+        a, b, c, d = (torch.empty_like(x) for x in (q, q[:2], q[:23], q[:23]))
+        A.prompt_attention(q, kv[:, 0], kv[:, 1], cq, cq, 0.1, out=a)
+        P.paged_decode_q8(q[:2], caches[0].dk, caches[0].dv, *caches[0].ds, caches[0].dt, caches[0].dl, 0.1, b, 2)
+        for x, o in zip(caches, (c, d)):
+            P.tree_attention(q[:23], x.dk, x.dv, x.dt, x.dl, ct, 0.1, o, 20, key_scale=x.ds[0], value_scale=x.ds[1])
+        return a, b, c, d
+
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for x in got:
+        assert all(torch.equal(y, w) for y, w in zip(x, want))
+
+
+def test_calls_without_work():
+    from vllm_exact import kv_cache as C, paged_attn as P, prompt_attn as A
+    c = Cache([20], 16, 2, 64, E4)
+    q = torch.ones(3, 4, 64, dtype=BF, device=DEV)
+    kv = torch.ones(3, 2, 64, dtype=BF, device=DEV)
+    out = torch.full_like(q, 7.0)
+    none = cu([])
+    A.prompt_attention(q, kv, kv, none, none, 0.1, out=out)
+    assert A.prompt_attention(q[:0], kv, kv, cu([0]), cu([3]), 0.1).shape == (0, 4, 64)
+    P.paged_decode_q8(q, c.dk, c.dv, *c.ds, c.dt, c.dl, 0.1, out, 0)
+    P.tree_attention(q, c.dk, c.dv, c.dt[:0], c.dl[:0], none, 0.1, out, 4, key_scale=c.ds[0], value_scale=c.ds[1])
+    P.tree_attention(q, c.dk, c.dv, c.dt, c.dl, cu([0]), 0.1, out, 4, key_scale=c.ds[0], value_scale=c.ds[1])
+    rows = torch.full((3, 2, 64), 7.0, dtype=BF, device=DEV)
+    C.cache_read(c.dk, c.dv, *c.ds, c.dt[:0], none, rows, rows)
+    C.cache_read(c.dk, c.dv, *c.ds, c.dt, cu([0]), rows, rows)
+    C.cache_read(c.dk, c.dv, *c.ds, c.dt, cu([3]), rows[:0], rows[:0])
+    assert bool((out == 7.0).all()) and bool((rows == 7.0).all())
+
+
 @pytest.mark.parametrize("dtype", [I8, E4])
 def test_a_served_conversation(dtype):
     """A prompt is cached and attended to with the numbers the cache stands for, one token is decoded, a draft is

@@ -101,6 +101,29 @@ def test_prompt_refusals(X):
         refuse(f, PROMPT, status, **change)
 
 
+@pytest.mark.parametrize("scale", [0.0, float("inf"), float("nan"), 3e38])
+def test_scales_that_are_refused(X, scale):
+    """0 and what is not finite (3e38 times log2 e is not); prompts take positive scales only."""
+    L = X.lib()
+    for f, base in ((L.ex_paged_decode_q8, DECODE), (L.ex_tree_attention, TREE), (L.ex_prompt_attention, PROMPT)):
+        refuse(f, base, X.EX_ERR_ARG, scale=scale)
+    refuse(L.ex_prompt_attention, PROMPT, X.EX_ERR_ARG, scale=-0.1)
+
+
+def test_launch_on_restores_the_current_device(X, monkeypatch):
+    now = [1]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: now.__setitem__(0, d))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+    with X.launch_on(1) as stream:
+        assert stream == 101 and now == [1]
+    with pytest.raises(KeyError):
+        with X.launch_on(3) as stream:
+            assert stream == 103 and now == [3]
+            raise KeyError
+    assert now == [1]
+
+
 def test_python_refusals(X):
     """CPU tensors and wrong types raise (there is no CPU path)."""
     from vllm_exact import kv_cache as C, paged_attn as A, prompt_attn as Q

@@ -359,6 +359,8 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   if (n < 0 || tokens < 0 || tokens > INT32_MAX || H <= 0 || KV <= 0 || H % KV != 0 || BS <= 0 || width < 0 || max_len < 0)
     return EX_ERR_ARG;
   if (code < ex::CODE_NONE || code > ex::CODE_E4M3 || max_tokens < 1) return EX_ERR_ARG;
+  // (0 times the -infinity of a key that is not seen would be NaN)
+  if (!(fabsf(scale) > 0.0f && fabsf(scale * ex::PR_LOG2E) < INFINITY)) return EX_ERR_ARG;
   if (!half_dtype(q_dtype)) return EX_ERR_DTYPE;
   const int G = H / KV;
   if (G > 16 || !head_size_ok(D) || BS % 8 != 0 || max_tokens > ex::PR_MAX_TOKENS) return EX_ERR_UNSUPPORTED;
@@ -886,7 +888,7 @@ int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k
   if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(out, 16) || sq_t % 8 != 0 ||
       sq_h % 8 != 0 || sk_t % 8 != 0 || sk_h % 8 != 0 || sv_t % 8 != 0 || sv_h % 8 != 0 || so_t % 8 != 0 || so_h % 8 != 0)
     return EX_ERR_ALIGN;
-  if (!(scale > 0.0f && scale < INFINITY)) return EX_ERR_ARG;
+  if (!(scale > 0.0f && scale * ex::PR_LOG2E < INFINITY)) return EX_ERR_ARG;
   if (!ex::device_is_sm100()) return EX_ERR_UNSUPPORTED;
   if (keys == 0) {  // nothing to map: any rows do, none of them is read
     k = v = q;

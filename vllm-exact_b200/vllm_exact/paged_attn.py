@@ -135,7 +135,7 @@ def paged_decode_q8(query, key_cache, value_cache, key_scale, value_scale, block
 
     max_seq_len: no request is longer (a bound for the workspace; default: what the block table holds). Tokens behind
     it, and tokens on pages that the cache does not have, are not seen. A request of length 0 gives zeros. workspace: as
-    in paged_decode (rows_workspace_bytes), not to be shared by calls that may run at the same time."""
+    in paged_decode (rows_workspace_bytes), not to be shared by calls that may run at the same time. scale: finite, not 0."""
     if n <= 0:
         return out
     if query.shape[0] < n or out.shape[0] < n:

@@ -1,6 +1,7 @@
 """Causal attention of packed prompts on B200 (the reference leaves prompts to vLLM, src/vllm_exact/paged_attn.py:156).
 
-A row's bits depend on its own sequence alone, never on the other sequences of the batch, as in decode attention.
+A row's bits depend on its own query and the keys and values that it sees, never on the other sequences of the batch, as in
+decode attention: a prompt in pieces, each over all keys so far, gives the bits of the whole.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, scale, out=N
     rows cu_seqlens_k[b] .. cu_seqlens_k[b + 1] (int32, n + 1 entries each). Its last query is its last key's token:
     query i sees the keys j <= i + Lk - Lq, so keys may start before the queries (a continued conversation, its cached
     beginning read with kv_cache.cache_read). A query that sees no key gives zeros. Query head h reads KV head
-    h // (H / KV). Returns out (like query; made if not given); its rows of no sequence are left as they were."""
+    h // (H / KV). scale is positive. Returns out (like query; made if not given); its rows of no sequence are left as they were."""
     dev = query.get_device()  # -1: not on a GPU
     if (dev < 0 or key.get_device() != dev or value.get_device() != dev or cu_seqlens_q.get_device() != dev
             or cu_seqlens_k.get_device() != dev):
