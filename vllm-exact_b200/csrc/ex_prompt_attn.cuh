@@ -17,6 +17,10 @@
 //                   another sequence or to nobody, are zeroed, since 0 * NaN would reach O; values that are not finite
 //                   are zeroed and noted, and the rows that see such a key get it added at the end.
 // D = 256: one query tile and two S buffers (tensor memory holds no more), S of the next block issued before P V.
+// Bound by the products and the exponentials together, at the clock that the board's power leaves (1.6 to 1.7 GHz under this
+// load): a prompt of 16384 tokens (32 heads of 128 over 8) takes 1740 to 1890 us, 1.16 to 1.26 PFLOP/s; without its softmax it
+// would take 1554, without its products 1352 us. Steps of 64 keys with two S buffers a tile, so that no softmax waits for its
+// S: 1810 to 1980 us (a product of 64 columns reads Q as often as one of 128). Two threads a row: no faster, and spills.
 #pragma once
 #include "ex_paged_rows.cuh"
 
@@ -72,25 +76,34 @@ __device__ __forceinline__ uint64_t make_sw128_desc_n(uint32_t smem_addr, uint32
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// Products of one tile, issued by one lane of a warp that is here as a whole. Where every operand is uniform over the warp
-// (and the compiler can see it: see warp_uniform), they are in uniform registers from the start; a single lane's copies
-// would be moved there one by one, 80 cycles a product of 64.
+// Products of one tile, issued by a warp that is here as a whole and does not branch: one lane is elected in the instruction's
+// own predicate. Where every operand is uniform over the warp (and the compiler can see it: see warp_uniform), operands are
+// then made and held in uniform registers; in a branch of one lane each would be moved there, 50 to 80 cycles a product
+// of 64.
 // D[tmem] (+)= A B^T over 64 elements of K, operands in shared memory: low words of the descriptors (the high words, 1024
 // bytes between groups of 8 rows, version 1, 128-byte swizzle, are the same for every operand here).
 constexpr uint32_t SW128_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ void tc_mma_16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 r;\n\telect.sync r|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(SW128_DESC_HI)
       : "memory");
 }
 // the same with A in tensor memory
 __device__ __forceinline__ void tc_mma_16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t.reg .b32 r;\n\telect.sync r|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(SW128_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_warp(uint64_t* bar) {  // tc_commit by one lane of a whole warp
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b32 r;\n\telect.sync r|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(ex_smem_u32(bar))
       : "memory");
 }
 // The value that every lane has, in a register the compiler knows to be uniform.
@@ -379,7 +392,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       uint32_t slot = 0, ph = 0;  // next slot to be used
       // S (buffer) = Q (tile) K^T over the dims of the slot
       auto issue_s = [&](uint32_t at, int tile, int buf, int part) {
-        if (elect_one()) {
+        {
 #pragma unroll
           for (int x = 0; x < C::SW / 64; ++x)
 #pragma unroll
@@ -389,14 +402,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       };
       auto issue_o = [&](uint32_t at, int tile, int buf, int part, uint32_t acc) {
-        if (elect_one()) {
+        {
 #pragma unroll
           for (int k = 0; k < PA_KEYS / 16; ++k)
             tc_mma_16_ta(tm + C::TM_O + tile * D + part * C::SW, tm + C::TM_S + buf * 128 + k * 8,
                          dv + at * (C::SLOT >> 4) + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
         }
       };
-      auto commit = [&](uint64_t* b) { if (elect_one()) tc_commit(b); };
+      auto commit = [&](uint64_t* b) { tc_commit_warp(b); };
       auto wait_full = [&](uint32_t at, uint32_t p) {
         mbar_wait(full_bar + at, p, EX_DEVERR_WAIT_TMA);
         __syncwarp();
@@ -495,6 +508,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
     const int tile = warp >> 2;
     const int nb = nblk[tile & 1];
+    const int whole = max(0, min(Lk, row0 + (tile & (C::NQ - 1)) * 128 + off + 1)) / PA_KEYS;  // blocks before it are seen by every row of the tile
     const int row = row0 + tile * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + C::TM_O + tile * D;
@@ -516,7 +530,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       // A block that is seen whole is weighed with the reference that there is, while its largest score is still being looked
       // for: nothing waits for it. If a score of the warp passes its row's reference by too much (or is NaN), or the block is
       // an edge, or the first, the block is weighed (again) below.
-      bool again = j >= edge || j == 0;
+      bool again = j >= whole || j == 0;
       f32x2 sum0 = pair(0.0f, 0.0f), sum1 = sum0;
       // The weights of the block against the reference, written over S, and their sums. Both callers have the same arithmetic
       // in the same order, so that a row does not depend on which one its warp needs.
@@ -559,7 +573,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         again = !(mb <= m + grow);
       }
       if (__any_sync(0xffffffffu, again)) {
-        if (j >= edge) {
+        if (j >= whole) {
           const int limit = min(Lk - 1, row + off) - j * PA_KEYS;  // columns behind it are not seen
 #pragma unroll
           for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;

@@ -333,7 +333,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
                    dr = warp_uniform((uint32_t)make_sw128_desc(ex_smem_u32(ring))),
                    dv = warp_uniform((uint32_t)make_sw128_desc_n(ex_smem_u32(ring), C::SUB)), tm = warp_uniform(tmem);
     uint32_t slot = 0, ph = 0, php = 0, phq = 0, edges = 0;
-    auto commit = [&](uint64_t* b) { if (elect_one()) tc_commit(b); };
+    auto commit = [&](uint64_t* b) { tc_commit_warp(b); };
     while (next()) {
       const int nb = (int)warp_uniform((uint32_t)nblk), je = (int)warp_uniform((uint32_t)jedge);
       if (nb == 0) continue;
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           mbar_wait(full_bar + slot, ph, EX_DEVERR_WAIT_TMA);
           __syncwarp();
           tc_fence_after();
-          if (elect_one()) {
+          {
             if (is_v) {
               const uint32_t d = tm + TM_O + (C::STREAMS == 2 ? (j & 1) * D : p * C::SW), db = dv + slot * (C::SLOT >> 4);
               const uint32_t acc = j >= C::STREAMS ? 1u : 0u;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
                   tc_mma_16(sbuf, dq + (p * (C::SW / 64) + x) * (C::SUB >> 4) + 2 * k, db + x * (C::SUB >> 4) + 2 * k, id_s,
                             (p | x | k) != 0);
             }
-            tc_commit(empty_bar + slot);
+            commit(empty_bar + slot);
           }
           if (++slot == C::SLOTS) slot = 0, ph ^= 1u;
         }
