@@ -29,7 +29,8 @@ def attend(q, k, v, seen, scale, dtype, q8=False):
         float16 weight is below the normal numbers (q8: every weight is float16);
       * float32 sums over D and over the keys (2^-23 a step, truncating tensor cores included), the rescalings of the
         blocks and segments, and 2^x to 2^-22 with its argument rounded to 2^-23 of |x|; an error d of the
-        scores changes a normalised weight by at most 2 d of itself;
+        scores changes a normalised weight by at most 2 d of itself (prompts: an eighth of the weights by a polynomial of
+        relative error 2.7e-6; twice that is 46 steps, among the 128 that are added to the L of the sums);
       * q8: query elements below 2^-14 of their row's largest keep 2^-25 of it."""
     q, k, v = q.detach().cpu().double(), k.detach().cpu().double(), v.detach().cpu().double()
     seen = seen.cpu()

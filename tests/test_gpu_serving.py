@@ -486,6 +486,33 @@ def test_tree_rows_left_untouched():
     assert bool((short[11:] == 7.0).all()) and not bool((short[:11] == 7.0).any())
 
 
+def test_tree_many_empty_requests_between():
+    """Values that are not finite belong to their own request, however many requests without keys lie between two that have
+    some (a CTA takes every so many-th item)."""
+    from vllm_exact import paged_attn as P
+    H, KV, D, T = 16, 1, 128, 2
+    step = 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    n = 2 * step + 1
+    c = Cache([20, 30, 40], 16, KV, D, None)
+    lens = torch.zeros(n, dtype=torch.int32, device=DEV)
+    table = torch.zeros(n, c.dt.shape[1], dtype=torch.int32, device=DEV)
+    for i, b in enumerate((0, step, 2 * step)):
+        lens[b], table[b] = c.lens[i], c.dt[i]
+        c.dv[int(c.table[i, 0]), 3, 0, 5 + i] = float("inf")
+    q = torch.randn(T, H, D, generator=gen(21)).to(BF).to(DEV).repeat(n, 1, 1)
+    out = torch.full_like(q, 7.0)
+    P.tree_attention(q, c.dk, c.dv, table, lens, cu([T] * n), 0.1, out, T)
+    out = out.view(n, T, H, D)
+    some = torch.tensor([0, step, 2 * step], device=DEV)
+    empty = torch.ones(n, dtype=torch.bool, device=DEV)
+    empty[some] = False
+    assert bool((out[empty] == 0).all())
+    want = torch.zeros(3, T, H, D, dtype=torch.bool, device=DEV)
+    for i in range(3):
+        want[i, :, :, 5 + i] = True
+    assert torch.equal(out[some] == float("inf"), want) and torch.equal(~torch.isfinite(out[some]), want)
+
+
 @pytest.mark.parametrize("dtype", [None, E4])
 def test_tree_padded_batch(dtype):
     """Rows behind the last request (a captured step of a fixed number of rows): the requests' bits are those of the batch

@@ -214,6 +214,9 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
 // only when a score passes it by more than 6 (a factor of 64; p stays small enough for float16), and the reference of
 // the value scales when one is 64 times it: the common path has two votes and no shuffles. Both are decided for
 // every row (every key) alone.
+// Bound by the cache's bytes where there are many requests (64 of 8192 keys, int8: 209 us, 5.3 TB/s of 6.56 measured; 256 of
+// 1024, e4m3: 119 us, 4.7 TB/s; 16-bit, 4 tokens: 411 us, 5.2 TB/s), and before that by the instructions that make float16
+// of codes and weights of scores; one request of 1000 keys takes 19 us, most of it two launches and first uses of code.
 // ------------------------------------------------------------------------------------------------------------------
 template <int D, int CODE, int NT>
 struct PfCfg {

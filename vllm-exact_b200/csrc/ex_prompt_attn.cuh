@@ -207,7 +207,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
 // quarter of what a block of scores asks for) has none: x = i + f with i the nearest integer (1.5 2^23 leaves no bits behind the
 // point), 2^f by a polynomial, i into the exponent. The polynomial is the least-maximum-error one of degree 4 on
 // [-0.5, 0.5], fitted by iteratively reweighted least squares (Lawson's method): relative error 2.7e-6 = 2^-18.5 in
-// float32, a hundredth of a rounding step of float16. Below 2^-126 it stays there.
+// float32, a hundredth of a rounding step of float16. Below 2^-126 it stays there: next to the largest weight (at least 1 when
+// it was made the reference) that is nothing, and keys that are not seen have weight 0 from elsewhere.
 __device__ __forceinline__ void ex2_pair(f32x2 x, float& a, float& b) {
   float x0, x1;
   split(x, x0, x1);

@@ -17,8 +17,13 @@
 //   warps 10, 11    16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
 //                   are not finite are zeroed and noted, and added in the end to the rows that see them
 //   warps 12-15     for codes: codes to float16 tiles (exact; keys behind the end to zeros)
-// Bound by reading the cache once: a block of 128 keys of a 16-bit cache is 64 KB (D = 128), 1.5 us of an SM's share of HBM;
-// its products take 0.55 us and the 128 exponentials of a row 0.55 us on every scheduler that has rows.
+// 16-bit: bound by reading the cache once (a block of 128 keys is 64 KB for D = 128, 1.5 us of an SM's share of HBM) and by an
+// item's start and end, when only as much is read as the ring holds: queries 600 cycles (their loads run during the last
+// products), first scores 1400, last products 3000, results 8000, of 45000 for 2048 keys. 64 requests of 8192 keys with 16
+// tokens: 455 us, 4.7 TB/s.
+// Codes: bound by shared memory's bandwidth, 1800 cycles a block of 128 keys (S reads both operands, 512; P V 256; the
+// converters 768; TMA 256) of the 2650 that it takes; four converter warps more change nothing. 16 requests of 16384 keys,
+// 7 tokens: 242 us, 2.3 TB/s.
 #pragma once
 #include "ex_paged_rows.cuh"
 #include "ex_prompt_attn.cuh"
@@ -107,7 +112,8 @@ __device__ __forceinline__ float ptc_weights(uint32_t p_addr, const float* vs, f
 }
 
 constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
-constexpr int PTC_POISON = 8;  // items whose notes of values that are not finite are kept (the ring runs ahead of the rows)
+constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values that are not finite are kept (the ring, of at most
+                               // 8 slots, runs ahead of the rows)
 
 // The tiles of a segment of nblk blocks in the order of use, K0 K1 V0 K2 V1 .. (S of a block is made one block ahead of its
 // P V): tile n of 2 nblk is block j's values or keys.
@@ -392,8 +398,9 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     int item = 0;
     bool ok = true;
     while (ok && next()) {
-      uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
+      uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
       if (jedge < nblk) {
+        ++item;
         if (warp == 10 && lane < 8) mine[lane] = 0;
         asm volatile("bar.sync 6, 64;" ::: "memory");
       }
@@ -525,7 +532,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     };
     bool more = next_item();
     while (more) {
-      const uint32_t* mine = poison + (item++ & (PTC_POISON - 1)) * 8;
+      const uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
+      if (jedge < nblk) ++item;
       // copies of the rows: each weighs W keys of a block
       const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1, rows = 128 / copies, W = 128 / copies;
       const int rl = copies == 1 ? row0 + r : r & (rows - 1);  // row of the request (at least R: none)

@@ -34,16 +34,18 @@ def alloc_q8_cache(num_blocks: int, block_size: int, KV: int, D: int, dtype=torc
 
 
 def _check_cache(key_cache, value_cache, key_scale, value_scale, dev):
-    """Types, shapes, strides and device of the four tensors of an 8-bit cache; its code as the library names it."""
-    code = CODES.get(key_cache.dtype)
-    if code is None or value_cache.dtype != key_cache.dtype:
+    """Types, shapes, strides and device of the four tensors of an 8-bit cache; its code as the library names it, its shape
+    and the strides of its codes and scales."""
+    kind = key_cache.dtype
+    code = CODES.get(kind)
+    if code is None or value_cache.dtype != kind:
         raise TypeError("an 8-bit cache holds int8 or float8_e4m3fn codes, the same for keys and values")
     if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
         raise TypeError("the scales of an 8-bit cache are float32")
-    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+    shape, scales = key_cache.shape, key_scale.shape
+    if len(shape) != 4 or value_cache.shape != shape:
         raise ValueError("codes must be (num_blocks, block_size, KV, D), the same for keys and values")
-    nb, BS, KV, _ = key_cache.shape
-    if key_scale.shape != (nb, KV, BS) or value_scale.shape != (nb, KV, BS):
+    if len(scales) != 3 or (shape[0], shape[2], shape[1]) != scales or value_scale.shape != scales:
         raise ValueError("scales must be (num_blocks, KV, block_size)")
     st, ss = key_cache.stride(), key_scale.stride()
     if value_cache.stride() != st or value_scale.stride() != ss:
@@ -52,16 +54,22 @@ def _check_cache(key_cache, value_cache, key_scale, value_scale, dev):
         raise ValueError("the head dimension of codes and the places of scales must be contiguous")
     if not key_cache.get_device() == value_cache.get_device() == key_scale.get_device() == value_scale.get_device() == dev:
         raise ValueError("the cache must be on the same CUDA device as the other tensors")
-    return code
+    return code, shape, st, ss
 
 
 def _check_rows(name, a, b, KV, D):
-    if a.dtype not in _DT or b.dtype != a.dtype:
+    """Types, shapes and head dimensions of keys and values as packed rows; their type as the library names it, their number
+    and strides."""
+    kind, shape = a.dtype, a.shape
+    dtype = _DT.get(kind)
+    if dtype is None or b.dtype != kind:
         raise TypeError(f"{name} must be bf16 or fp16, the same for keys and values")
-    if a.dim() != 3 or a.shape != b.shape or a.shape[1] != KV or a.shape[2] != D:
+    if len(shape) != 3 or b.shape != shape or shape[1] != KV or shape[2] != D:
         raise ValueError(f"{name} must be (tokens, {KV}, {D}), the same for keys and values")
-    if a.stride(2) != 1 or b.stride(2) != 1:
+    sa, sb = a.stride(), b.stride()
+    if sa[2] != 1 or sb[2] != 1:
         raise ValueError(f"the head dimension of {name} must be contiguous")
+    return dtype, shape[0], sa, sb
 
 
 def cache_write(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping, key_out=None, value_out=None):
@@ -75,27 +83,22 @@ def cache_write(key, value, key_cache, value_cache, key_scale, value_scale, slot
     dev = key.get_device()  # -1: not on a GPU
     if dev < 0 or value.get_device() != dev or slot_mapping.get_device() != dev:
         raise ValueError("cache_write needs CUDA tensors of one device (there is no CPU fallback)")
-    code = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
-    nb, BS, KV, D = key_cache.shape
-    _check_rows("key and value", key, value, KV, D)
-    T = key.shape[0]
+    code, (nb, BS, KV, D), sc, ss = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+    dtype, T, sk, sv = _check_rows("key and value", key, value, KV, D)
     if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] != T:
         raise ValueError("slot_mapping must be a 1-D int64 tensor with a slot for every token")
     if (key_out is None) != (value_out is None):
         raise ValueError("key_out and value_out are given together")
-    if key_out is not None:
-        _check_rows("key_out and value_out", key_out, value_out, KV, D)
-        if (key_out.dtype != key.dtype or key_out.shape[0] != T or key_out.get_device() != dev
-                or value_out.get_device() != dev):
-            raise ValueError("key_out and value_out must be like key")
-    slot_mapping = slot_mapping.contiguous()
-    sk, sv, sc, ss = key.stride(), value.stride(), key_cache.stride(), key_scale.stride()
     ko, vo, sko, svo = None, None, (0, 0), (0, 0)
     if key_out is not None:
-        ko, vo, sko, svo = key_out.data_ptr(), value_out.data_ptr(), key_out.stride(), value_out.stride()
+        dtype_out, T_out, sko, svo = _check_rows("key_out and value_out", key_out, value_out, KV, D)
+        if dtype_out != dtype or T_out != T or key_out.get_device() != dev or value_out.get_device() != dev:
+            raise ValueError("key_out and value_out must be like key")
+        ko, vo = key_out.data_ptr(), value_out.data_ptr()
+    slot_mapping = slot_mapping.contiguous()
     with launch_on(dev) as stream:
         check("ex_cache_write_q8", lib().ex_cache_write_q8(
-            key.data_ptr(), sk[0], sk[1], value.data_ptr(), sv[0], sv[1], _DT[key.dtype], code, key_cache.data_ptr(),
+            key.data_ptr(), sk[0], sk[1], value.data_ptr(), sv[0], sv[1], dtype, code, key_cache.data_ptr(),
             value_cache.data_ptr(), sc[0], sc[1], sc[2], key_scale.data_ptr(), value_scale.data_ptr(), ss[0], ss[1], nb,
             BS, slot_mapping.data_ptr(), T, KV, D, ko, sko[0], sko[1], vo, svo[0], svo[1], stream))
 
@@ -107,9 +110,8 @@ def cache_read(key_cache, value_cache, key_scale, value_scale, block_table, cu_s
     dev = key_out.get_device()  # -1: not on a GPU
     if dev < 0 or value_out.get_device() != dev or block_table.get_device() != dev or cu_seqlens.get_device() != dev:
         raise ValueError("cache_read needs CUDA tensors of one device (there is no CPU fallback)")
-    code = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
-    nb, BS, KV, D = key_cache.shape
-    _check_rows("key_out and value_out", key_out, value_out, KV, D)
+    code, (nb, BS, KV, D), sc, ss = _check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+    dtype, rows, sk, sv = _check_rows("key_out and value_out", key_out, value_out, KV, D)
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or cu_seqlens.dtype != torch.int32:
         raise TypeError("block_table (n, pages) and cu_seqlens must be int32")
     n, width = block_table.shape
@@ -118,11 +120,10 @@ def cache_read(key_cache, value_cache, key_scale, value_scale, block_table, cu_s
     if width > 1 and block_table.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
     cu_seqlens = cu_seqlens.contiguous()
-    sc, ss, sk, sv = key_cache.stride(), key_scale.stride(), key_out.stride(), value_out.stride()
     with launch_on(dev) as stream:
         check("ex_cache_read_q8", lib().ex_cache_read_q8(
             key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0], sc[1], sc[2], key_scale.data_ptr(),
             value_scale.data_ptr(), ss[0], ss[1], nb, BS, block_table.data_ptr(), block_table.stride(0), width,
-            cu_seqlens.data_ptr(), n, key_out.shape[0], KV, D, _DT[key_out.dtype], key_out.data_ptr(),
+            cu_seqlens.data_ptr(), n, rows, KV, D, dtype, key_out.data_ptr(),
             sk[0], sk[1], value_out.data_ptr(), sv[0], sv[1], stream))
     return key_out, value_out

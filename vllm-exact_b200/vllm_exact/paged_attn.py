@@ -141,14 +141,13 @@ def paged_decode_q8(query, key_cache, value_cache, key_scale, value_scale, block
     if query.shape[0] < n or out.shape[0] < n:
         raise ValueError("query and out need a row for every request")
     dev = _rows_operands("paged_decode_q8", query, key_cache, value_cache, block_table, seq_lens, out, n)
-    code = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+    code, (nb, BS, KV, _), sc, ss = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
     seq_lens = seq_lens.contiguous()
     _, H, D = query.shape
-    nb, BS, KV, _ = key_cache.shape
     width = block_table.shape[1]
     max_len = width * BS if max_seq_len is None else min(max(0, int(max_seq_len)), width * BS)
     nbytes, workspace = _rows_scratch(n, H, D, max_len, workspace, query)
-    sq, sc, ss, so = query.stride(), key_cache.stride(), key_scale.stride(), out.stride()
+    sq, so = query.stride(), out.stride()
     with launch_on(dev) as stream:
         check("ex_paged_decode_q8", lib().ex_paged_decode_q8(
             query.data_ptr(), sq[0], sq[1], _DT16[query.dtype], key_cache.data_ptr(), value_cache.data_ptr(), code, sc[0],
@@ -194,8 +193,8 @@ def tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_s
     else:
         if key_scale is None or value_scale is None:
             raise TypeError("the cache must be in query's type, or 8-bit with key_scale and value_scale")
-        code = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
-        ks, vs, ss = key_scale.data_ptr(), value_scale.data_ptr(), key_scale.stride()
+        code, _, _, ss = kv_cache._check_cache(key_cache, value_cache, key_scale, value_scale, dev)
+        ks, vs = key_scale.data_ptr(), value_scale.data_ptr()
     if n == 0 or tokens == 0:
         return out
     seq_lens, query_start_loc = seq_lens.contiguous(), query_start_loc.contiguous()
