@@ -27,6 +27,7 @@
 #pragma once
 #include "ex_paged_rows.cuh"
 #include "ex_prompt_attn.cuh"
+#include "ex_tree_ring.h"
 
 namespace ex {
 
@@ -35,7 +36,8 @@ struct PtcCfg {
   static constexpr bool Q8 = CODE != CODE_NONE;
   static constexpr int STREAMS = D == 256 ? 1 : 2;
   static constexpr int THREADS = 512;
-  static constexpr int FEEDERS = Q8 ? 3 : 4;         // producer warps
+  static constexpr int FEEDERS = ptc_feeders(Q8);    // producer warps
+  static constexpr int LOADED = ptc_loaded_count(Q8);  // arrivals on a loaded tile
   // registers a thread: at launch, of the softmax warps and of the others, which give theirs up
   static constexpr int REGS = 128, REGS_SOFTMAX = 168, REGS_OTHER = 88;
   static_assert(256 * REGS_SOFTMAX + (THREADS - 256) * REGS_OTHER <= THREADS * REGS, "register shares");
@@ -115,14 +117,6 @@ constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of th
 constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values that are not finite are kept (the ring, of at most
                                // 8 slots, runs ahead of the rows)
 
-// The tiles of a segment of nblk blocks in the order of use, K0 K1 V0 K2 V1 .. (S of a block is made one block ahead of its
-// P V): tile n of 2 nblk is block j's values or keys.
-__device__ __forceinline__ bool ptc_tile(int n, int nblk, int& j) {
-  const bool v = n == 2 * nblk - 1 || (n > 0 && !(n & 1));
-  j = n == 2 * nblk - 1 ? nblk - 1 : v ? (n >> 1) - 1 : (n + 1) >> 1;
-  return v;
-}
-
 template <int D, int CODE, bool F16>
 __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     k_tree_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -162,9 +156,9 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   if (tid == 0) {
     *sfail = 0;
     for (int i = 0; i < 8; ++i) {
-      mbar_init(full_bar + i, Q8 ? 128 : 1);
+      mbar_init(full_bar + i, Q8 ? 128 : C::LOADED);
       mbar_init(empty_bar + i, 1);
-      mbar_init(rfull_bar + i, 33);  // every producer lane's copies of scales, and the codes
+      mbar_init(rfull_bar + i, C::LOADED);
       mbar_init(rempty_bar + i, 128);
     }
     for (int i = 0; i < 2; ++i) {
@@ -301,6 +295,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
                           po, pg);
           }
           __syncwarp();
+          // every producer arrives on every tile (feeder 0 has; the last one for codes with its copies of scales): see ptc_arrivals
+          if (feeder != 0 && !(Q8 && feeder == C::FEEDERS - 1) && lane == 0) mbar_arrive(fulls + slot);
           if constexpr (Q8) {
             if (feeder == C::FEEDERS - 1) {
               if (!is_v && p == 0) {  // both scales come with the keys: the weights need them before the values
