@@ -72,6 +72,7 @@ def paged_decode(query, key_cache, value_cache, block_table, seq_lens, scale, ou
     BS, KV = key_cache.shape[1], key_cache.shape[2]
     split = split or SPLIT
     nbytes = workspace_bytes(n, H, D, MAX_LEN, split)
+    _check_workspace(workspace, query)
     if workspace is None or workspace.numel() < nbytes:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
     with torch.cuda.device(query.device):
@@ -118,12 +119,17 @@ def _rows_operands(name, query, key_cache, value_cache, block_table, seq_lens, o
     return dev
 
 
+def _check_workspace(workspace, query):
+    """A caller's workspace is written as one run of bytes: a strided or expanded view would have others' memory between."""
+    if workspace is not None and (workspace.get_device() != query.get_device() or not workspace.is_contiguous()):
+        raise ValueError("the workspace must be contiguous and on the query's device")
+
+
 def _rows_scratch(tokens, H, D, max_len, workspace, query):
+    _check_workspace(workspace, query)
     nbytes = lib().ex_paged_rows_workspace_bytes(tokens, H, D, max_len)
     if nbytes and (workspace is None or workspace.numel() * workspace.element_size() < nbytes):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-    elif workspace is not None and workspace.get_device() != query.get_device():
-        raise ValueError("the workspace must be on the query's device")
     return nbytes, workspace
 
 
@@ -135,7 +141,7 @@ def paged_decode_q8(query, key_cache, value_cache, key_scale, value_scale, block
 
     max_seq_len: no request is longer (a bound for the workspace; default: what the block table holds). Tokens behind
     it, and tokens on pages that the cache does not have, are not seen. A request of length 0 gives zeros. workspace: as
-    in paged_decode (rows_workspace_bytes), not to be shared by calls that may run at the same time. scale: finite, not 0."""
+    in paged_decode (rows_workspace_bytes; contiguous), not to be shared by calls that may run at the same time. scale: finite, not 0."""
     if n <= 0:
         return out
     if query.shape[0] < n or out.shape[0] < n:
