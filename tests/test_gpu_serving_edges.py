@@ -29,3 +29,40 @@ def test_tree_many_tiles_of_one_box(dtype, H, KV, D):
     made = [words(t, "chain", None) for t in T]
     got = tree(c, q, T, D ** -0.5, None)
     tree_check(c, q, T, [s for _, s in made], got, D ** -0.5, BF)
+
+
+# rows a KV head: 8 and 16 are the few-row kernel's, 24 and 64 stand in the tile in copies, 68 and 132 do not
+DRAFTS = [2, 4, 6, 16, 17, 33]
+
+
+# ---- value rows that are not finite
+@pytest.mark.parametrize("dtype", [I8, E4])
+@pytest.mark.parametrize("T", DRAFTS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_tree_value_rows_written_from_numbers_that_are_not_finite(dtype, T, D, bad):
+    """All value rows of one head of a request, and those of a last block that begins with the drafted tokens, were written
+    from infinities or NaN: every row that sees one is NaN there, the other head and request keep their bits."""
+    from vllm_exact import kv_cache as C
+    H, KV = 8, 2
+    lens = [100, 128 + T, 1000, 100]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(len(lens) * T, H, D, generator=gen(5)).to(BF)
+    clean = tree(c, q, [T] * 4, 0.1, None)
+    for b, lo in ((0, 0), (1, 128), (2, 0)):
+        pos = torch.arange(lo, lens[b])
+        slots = c.table[b].long()[pos // 16] * 16 + pos % 16
+        x = torch.randn(len(pos), KV, D, generator=gen(7)).to(BF).to(DEV)
+        v = c.seq(1, b)[lo:].float().to(BF).to(DEV)
+        v[:, 1, 3] = bad
+        keep = [t.clone() for t in (c.dk, c.ds[0])]
+        before = [c.dv.clone(), c.ds[1].clone()]
+        C.cache_write(x, v, c.dk, c.dv, *c.ds, slots.to(DEV))
+        c.dk.copy_(keep[0])
+        c.ds[0].copy_(keep[1])
+        blk, off = c.table[b].long()[pos // 16].to(DEV), (pos % 16).to(DEV)
+        c.dv.view(torch.uint8)[blk, off, 0] = before[0].view(torch.uint8)[blk, off, 0]  # head 0 as it was
+        c.ds[1][blk, 0, off] = before[1][blk, 0, off]
+    got = tree(c, q, [T] * 4, 0.1, None)
+    assert bool(torch.isnan(got[:3 * T, 4:]).all())
+    assert torch.equal(got[:, :4], clean[:, :4]) and torch.equal(got[3 * T:], clean[3 * T:])

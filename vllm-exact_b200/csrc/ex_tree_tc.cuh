@@ -721,9 +721,12 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         const int x = copies == 1 ? r : (r & (rows - 1)) + k * rows;
         lall += sm[256 + x] * ex2(sm[x] - sub) + sm[256 + 128 + x] * ex2(sm[128 + x] - sub);
       }
+      bool some[2];  // (a stream that weighed nothing may hold anything; one with a factor of 0 may hold NaN, which stays)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        f[i] = sm[i * 128 + r] == -INFINITY ? 0.0f : ex2(sm[i * 128 + r] - sub) * (Q8 ? sm[512 + i * 128 + r] : 1.0f);
+      for (int i = 0; i < 2; ++i) {
+        some[i] = sm[i * 128 + r] > -INFINITY;
+        f[i] = some[i] ? ex2(sm[i * 128 + r] - sub) * (Q8 ? sm[512 + i * 128 + r] : 1.0f) : 0.0f;
+      }
       const bool have1 = C::STREAMS == 2 && w.nblk > 1;
       const bool single = pr_segments_many(pr_keys(a, w.L)) == 1;
       bool any = false;
@@ -745,8 +748,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             float o[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              o[i] = f[0] == 0.0f ? 0.0f : __uint_as_float(u[i]) * f[0];
-              o[i] += f[1] == 0.0f ? 0.0f : __uint_as_float(v[i]) * f[1];
+              o[i] = some[0] ? __uint_as_float(u[i]) * f[0] : 0.0f;
+              o[i] += some[1] ? __uint_as_float(v[i]) * f[1] : 0.0f;
               if (single) o[i] *= inv;
             }
 #pragma unroll
