@@ -66,3 +66,114 @@ def test_tree_value_rows_written_from_numbers_that_are_not_finite(dtype, T, D, b
     got = tree(c, q, [T] * 4, 0.1, None)
     assert bool(torch.isnan(got[:3 * T, 4:]).all())
     assert torch.equal(got[:, :4], clean[:, :4]) and torch.equal(got[3 * T:], clean[3 * T:])
+
+
+def close(q, k, v, seen, scale, dtype, q8):
+    """(out, bound) as serving_ref.attend, but with a bound made of what the row sees and weighs alone: hidden keys, and keys
+    of next to no weight, do not widen it. Element by element:
+      * the output to its type (below bf16's normal numbers half of 2^-133; below float16's of 2^-24);
+      * weights and sums: A (the sum of p |v|) times half a step of 16 bits, twice the scores' error and the float32 sums';
+      * float16 weights below the normal numbers (q8, float16): at most half a step, 2^-25, of the reference each, on a
+        code of at most Q. The reference is at most the largest weight times value scale of the row, which times Q is the
+        largest weight times largest |v| of its key;
+      * q8: the reference is at least 2^-126 (2^-25 2^-126 448 a key), products of weight and scale below the normal
+        numbers are rounded to 2^-149 (half of it times 448)."""
+    q, k, v = q.detach().cpu().double(), k.detach().cpu().double(), v.detach().cpu().double()
+    T, H, D = q.shape
+    G = H // k.shape[1]
+    kh, vh = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    hide = ~seen.cpu()[None]
+    s = (torch.einsum("thd,lhd->htl", q, kh) * scale).masked_fill(hide, -torch.inf)
+    s_abs = (torch.einsum("thd,lhd->htl", q.abs(), kh.abs()) * abs(scale)).masked_fill(hide, 0.0)
+    m = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(m > -torch.inf, m, torch.zeros_like(m))).masked_fill(hide, 0.0)
+    l = p.sum(-1, keepdim=True)
+    p = torch.where(l > 0, p / l.clamp(min=1e-300), torch.zeros_like(p))
+    out = torch.einsum("htl,lhd->thd", p, vh)
+    A = torch.einsum("htl,lhd->thd", p, vh.abs())
+    # the scores of keys with a weight that counts (2^-160 and more of the largest); of the others nothing is left
+    counts = p > 2.0 ** -160
+    ds = s_abs.masked_fill(~counts, 0.0).amax(-1) * ((D + 8) * 2.0 ** -23) + 2.0 ** -21
+    if q8:
+        kmax = kh.abs().amax(-1).T[:, None].expand_as(p).masked_fill(~counts, 0.0).amax(-1)  # (H, T)
+        ds = ds + D * 2.0 ** -25 * q.abs().amax(-1).T * kmax * abs(scale) * 2
+    n = seen.double().sum(-1)[:, None, None]
+    half = S.HALF_STEP[FP if q8 else dtype]
+    bound = S.HALF_STEP[dtype] * out.abs() + A * (half + 2 * ds.T[..., None] + (k.shape[0] + 128) * 2.0 ** -23) * 1.01
+    if q8 or dtype == FP:
+        heaviest = (p * vh.abs().amax(-1).T[:, None]).amax(-1).T[..., None]  # (T, H, 1)
+        bound = bound + n * 2.0 ** -25 * heaviest * 1.01
+    bound = bound + (2.0 ** -25 if dtype == FP else 2.0 ** -134)
+    if q8:
+        bound = bound + n * (2.0 ** -142 + 2.0 ** -141)
+    return out, bound
+
+
+def put_value(c, b, pos, codes, scale):
+    """The value row of token `pos` of sequence b of an 8-bit cache, and what it then stands for."""
+    blk, off = int(c.table[b, pos // c.page]), pos % c.page
+    c.dv.view(torch.uint8)[blk, off] = codes.view(torch.uint8).to(DEV)
+    c.ds[1][blk, :, off] = scale.to(DEV)
+    c.real[1][blk, off] = S.values(codes, scale)
+
+
+# ---- value scales
+@pytest.mark.parametrize("dtype", [I8, E4])
+@pytest.mark.parametrize("T", DRAFTS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tree_hidden_value_scales(dtype, T, D):
+    """What the value row of a drafted token holds, an ordinary row or one of 1e30, does not change a bit of the rows that do
+    not see it; those that see it are right."""
+    H, KV = 8, 2
+    lens = [100, 700]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(2 * T, H, D, generator=gen(5)).to(BF)
+    w, see = words(T, "tree", gen(9))
+    hidden = T // 2
+    see[:, hidden] &= torch.arange(T) % 2 == hidden % 2
+    w = [sum(1 << j for j in range(T) if see[i, j]) for i in range(T)]
+    w = [x - (1 << 64) if x >> 63 else x for x in w]
+    clean = tree(c, q, [T, T], 0.1, w * 2)
+    other = torch.randn(KV, D, generator=gen(8))
+    for factor in (1.0, 2.0 ** 14, 1e30):
+        codes, scale = S.quantise(other, dtype)
+        for b in range(2):
+            put_value(c, b, lens[b] - T + hidden, codes, scale * factor)
+        got = tree(c, q, [T, T], 0.1, w * 2)
+        blind = (~see[:, hidden]).repeat(2).to(DEV)
+        assert torch.equal(got[blind], clean[blind]), factor
+        for b in range(2):
+            seen = torch.cat([torch.ones(T, lens[b] - T, dtype=torch.bool), see], 1)
+            want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 0.1, BF, True)
+            check(got[b * T:b * T + T], want, bound, (factor, b))
+
+
+@pytest.mark.parametrize("dtype", [I8, E4])
+@pytest.mark.parametrize("T", [1, 4, 6, 33])
+@pytest.mark.parametrize("bits,ratio", [(144, 14), (144, 26), (144, 100), (60, 40), (60, 60), (60, 58), (30, 40), (3, 20)])
+def test_value_scales_of_keys_with_little_weight(dtype, T, bits, ratio):
+    """One key with values 2^ratio times the others' and a weight of about 2^-bits: the result is the weighted sum, whichever
+    of the two wins, wherever the key lies."""
+    H, KV, D, lens = 8, 2, 128, [1000, 90, 300]
+    scale = 0.125
+    c = Cache(lens, 16, KV, D, dtype)
+    u = torch.sign(torch.randn(KV, D, generator=gen(3)))
+    q = torch.randn(len(lens) * T, KV, H // KV, D, generator=gen(4)) * 0.05 + u[:, None]
+    q = q.reshape(-1, H, D).to(BF)
+    for b, pos in enumerate((3, 50, 290 - T)):
+        blk, off = int(c.table[b, pos // 16]), pos % 16
+        codes, s = S.quantise(-u, dtype)  # the score of u on it: -D a scale
+        s = s * (bits * 0.6931 / (D * scale))
+        c.dk.view(torch.uint8)[blk, off] = codes.view(torch.uint8).to(DEV)
+        c.ds[0][blk, :, off] = s.to(DEV)
+        c.real[0][blk, off] = S.values(codes, s)
+        codes, s = S.quantise(torch.randn(KV, D, generator=gen(6)), dtype)
+        put_value(c, b, pos, codes, s * 2.0 ** ratio)
+    if T == 1:
+        got = decode(c, q.to(DEV), scale)
+    else:
+        got = tree(c, q, [T] * len(lens), scale, None)
+    for b, L in enumerate(lens):
+        seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+        want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, scale, BF, True)
+        check(got[b * T:b * T + T], want, bound, b)

@@ -11,8 +11,10 @@
 // sync), dealt out in turn: neighbouring items share keys' pages. Requests of at most 16 rows a KV head are k_paged_few's,
 // the others k_tree_tc's (ex_tree_tc.cuh), by their own number of rows.
 //
-// 8-bit codes become float16 (exact). The key scale multiplies the score; the value scale goes into P, divided by the
-// largest value scale so far, which multiplies O in the end: float16 P keeps 11 bits of every weight that counts.
+// 8-bit codes become float16 (exact). The key scale multiplies the score; the value scale goes into P: P is p_j vs_j over a
+// reference of the row's own, the largest p_j vs_j of the keys that it sees so far, taken up like m and carried along when m
+// is; it multiplies O in the end. So float16 P keeps 11 bits of every product that counts, and what a hidden key or one of
+// next to no weight has for a value scale is nothing to the row.
 // Queries are brought to float16 by a power of two per row, exact for all elements above 2^-14 of the row's largest.
 #pragma once
 #include "ex_cache_q8.cuh"
@@ -212,8 +214,8 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
 // Every warp streams its own items: it loads blocks of 16 MK keys into its own ring, S blocks ahead and on into its next
 // item, and computes S^T = K Q^T, P and O^T += V^T P^T on what has arrived. No thread waits for another warp. m is taken up
 // only when a score passes it by more than 6 (a factor of 64; p stays small enough for float16), and the reference of
-// the value scales when one is 64 times it: the common path has two votes and no shuffles. Both are decided for
-// every row (every key) alone.
+// weights times value scales when one is 64 times it: the common path has two votes and no shuffles. Both are decided for
+// every row alone.
 // Bound by the cache's bytes where there are many requests (64 of 8192 keys, int8: 209 us, 5.3 TB/s of 6.56 measured; 256 of
 // 1024, e4m3: 119 us, 4.7 TB/s; 16-bit, 4 tokens: 411 us, 5.2 TB/s), and before that by the instructions that make float16
 // of codes and weights of scores; one request of 1000 keys takes 19 us, most of it two launches and first uses of code.
@@ -406,11 +408,12 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
       fac[i] = Q8 ? __shfl_sync(0xffffffffu, qs[i >> 1], (qc + (i & 1)) * 4) * a.scale_log2 : a.scale_log2;
 
     float m[2 * NT], l[2 * NT], o[KT][NT][4];
-    float vref = 0.0f, vinv = 0.0f;
+    float vref[2 * NT], vinv[2 * NT];  // codes: O is the sum of p vs c over vref; 1 / vref
 #pragma unroll
     for (int i = 0; i < 2 * NT; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.0f;
+      vref[i] = vinv[i] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i)
@@ -531,7 +534,8 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
         top[x] = v;
         need |= v > m[x] + 6.0f;
       }
-      if (__any_sync(0xffffffffu, need)) {
+      const bool moved = __any_sync(0xffffffffu, need);
+      if (moved) {
 #pragma unroll
         for (int x = 0; x < 2 * NT; ++x) {
           float v = top[x];
@@ -542,62 +546,85 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             const float al = ex2(m[x] - v);
             m[x] = v;
             l[x] *= al;
+            if constexpr (Q8) {
+              vref[x] *= al;  // (O stays: it is over the reference)
+            } else {
 #pragma unroll
-            for (int mt = 0; mt < KT; ++mt) {
-              o[mt][x >> 1][x & 1] *= al;
-              o[mt][x >> 1][2 + (x & 1)] *= al;
+              for (int mt = 0; mt < KT; ++mt) {
+                o[mt][x >> 1][x & 1] *= al;
+                o[mt][x >> 1][2 + (x & 1)] *= al;
+              }
             }
           }
         }
       }
-      if constexpr (Q8) {
-        float v = 0.0f;
+      // weights; for codes times the keys' value scales (of a key that is not seen it may be anything)
 #pragma unroll
-        for (int i = 0; i < MK; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) v = fmaxf(v, vsc[i][e] < INFINITY ? vsc[i][e] : 0.0f);  // (NaN: 0)
-        if (__any_sync(0xffffffffu, v > 64.0f * vref)) {
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          const bool tiny = v < 1.2e-38f;  // such values are zero next to any output type's smallest step
-          const float be = tiny ? 1.0f : __fdividef(vref, v);
-          vinv = tiny ? 0.0f : __frcp_rn(v);
-          vref = v;
-#pragma unroll
-          for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[mt][j][e] *= be;
-        }
-      }
-      uint32_t pb[MK][NT][2];
-#pragma unroll
-      for (int i = 0; i < MK; ++i) {
+      for (int i = 0; i < MK; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float ref = m[2 * j + (e & 1)];
-            p[e] = ex2(sc[i][j][e] - (ref == -INFINITY ? 0.0f : ref));
+            sc[i][j][e] = ex2(sc[i][j][e] - (ref == -INFINITY ? 0.0f : ref));
           }
-          l[2 * j] += p[0] + p[2];
-          l[2 * j + 1] += p[1] + p[3];
+          l[2 * j] += sc[i][j][0] + sc[i][j][2];
+          l[2 * j + 1] += sc[i][j][1] + sc[i][j][3];
           if constexpr (Q8) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] *= vsc[i][e >> 1] * vinv;
-            if (!whole) {  // a key that is not seen has a scale that may be anything
+            for (int e = 0; e < 4; ++e) sc[i][j][e] *= vsc[i][e >> 1];
+            if (!whole) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if ((hidden >> ((i * NT + j) * 4 + e)) & 1u) p[e] = 0.0f;
+                if ((hidden >> ((i * NT + j) * 4 + e)) & 1u) sc[i][j][e] = 0.0f;
             }
           }
-          pb[i][j][0] = movmatrix_t(MF16 ? pack2<__half>(p[0], p[1]) : pack_bf16(p[0], p[1]));
-          pb[i][j][1] = movmatrix_t(MF16 ? pack2<__half>(p[2], p[3]) : pack_bf16(p[2], p[3]));
         }
+      if constexpr (Q8) {
+        float high[2 * NT];
+        bool rise = moved;
+#pragma unroll
+        for (int x = 0; x < 2 * NT; ++x) {
+          float v = fmaxf(sc[0][x >> 1][x & 1], sc[0][x >> 1][2 + (x & 1)]);  // (NaN: left out)
+#pragma unroll
+          for (int i = 1; i < MK; ++i) v = fmaxf(v, fmaxf(sc[i][x >> 1][x & 1], sc[i][x >> 1][2 + (x & 1)]));
+          high[x] = v;
+          rise |= v > 64.0f * vref[x];
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+          for (int x = 0; x < 2 * NT; ++x) {
+            float v = high[x] < INFINITY ? high[x] : 0.0f;
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            const float to = v > 64.0f * vref[x] ? v : vref[x];
+            const bool tiny = to < 1.2e-38f;  // such values are zero next to any output type's smallest step
+            vinv[x] = tiny ? 0.0f : __frcp_rn(to);
+            const float be = to == vref[x] ? 1.0f : vref[x] * vinv[x];
+            vref[x] = to;
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt) {
+              o[mt][x >> 1][x & 1] *= be;
+              o[mt][x >> 1][2 + (x & 1)] *= be;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MK; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[i][j][e] *= vinv[2 * j + (e & 1)];
       }
+      uint32_t pb[MK][NT][2];
+#pragma unroll
+      for (int i = 0; i < MK; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          pb[i][j][0] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][0], sc[i][j][1]) : pack_bf16(sc[i][j][0], sc[i][j][1]));
+          pb[i][j][1] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][2], sc[i][j][3]) : pack_bf16(sc[i][j][2], sc[i][j][3]));
+        }
       const int mi = lane >> 3;
       if (!Q8 && slow) {
         // one product at a time: a weight of 0 leaves a value out that is not finite
@@ -669,7 +696,7 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
       const int c = (x >> 1) * 8 + qc + (x & 1);
       if (c >= R) continue;
       const int t = c / a.G, h = g * a.G + c % a.G;
-      const float up = Q8 ? vref : 1.0f;
+      const float up = Q8 ? vref[x] : 1.0f;
       // 16 dims a tile: codes 2 qr, 2 qr + 1; 16-bit qr, qr + 8
       if (single) {
         const float inv = lx > 0.0f ? up / lx : (lx == 0.0f ? 0.0f : lx);  // nothing seen: zeros; NaN stays NaN

@@ -82,8 +82,17 @@ __device__ __forceinline__ float ptc_max(const float (&x)[N]) {
   for (int i = 4; i < N; ++i) m[i & 3] = fmaxf(m[i & 3], x[i]);
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
+// The largest x fac + log2 of the value scale: what a row's reference has to reach. (NaN, and keys that are not seen: left out.)
+template <int N>
+__device__ __forceinline__ float ptc_high(const float (&x)[N], const float* vs, float fac) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, __fmaf_rn(x[i], fac, __log2f(vs[i])));
+  return m;
+}
 // Their weights 2^(x fac - sub) in 16 bits to tensor memory at p_addr (over scores that have been read); returns the weights'
-// sum. Codes: times the values' scales over their reference.
+// sum. Codes: times the values' scales over the row's reference (the scale times the weight first: neither that over the
+// reference nor the scale over it need be a number).
 template <bool Q8, bool MF16, int N>
 __device__ __forceinline__ float ptc_weights(uint32_t p_addr, const float* vs, float fac, float sub, float vinv, float (&x)[N]) {
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -100,10 +109,10 @@ __device__ __forceinline__ float ptc_weights(uint32_t p_addr, const float* vs, f
       }
       if constexpr (Q8) {
         const float4 v = *reinterpret_cast<const float4*>(vs + c + i);
-        w[0] *= v.x * vinv;
-        w[1] *= v.y * vinv;
-        w[2] *= v.z * vinv;
-        w[3] *= v.w * vinv;
+        w[0] = w[0] * v.x * vinv;
+        w[1] = w[1] * v.y * vinv;
+        w[2] = w[2] * v.z * vinv;
+        w[3] = w[3] * v.w * vinv;
       }
       p[i / 2] = MF16 ? pack2<__half>(w[0], w[1]) : pack_bf16(w[0], w[1]);
       p[i / 2 + 1] = MF16 ? pack2<__half>(w[2], w[3]) : pack_bf16(w[2], w[3]);
@@ -535,7 +544,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       const int rl = copies == 1 ? row0 + r : r & (rows - 1);  // row of the request (at least R: none)
       const int col = copies == 1 ? 0 : r / rows * W;
       const bool active = copies > 1 || row0 + (warp & 3) * 32 < R;  // some row of this warp is real
-      float m = -INFINITY, l = 0.0f, vref = 0.0f, vinv = 0.0f;
+      // codes: O is the sum of the weights times value scales times codes over 2^(vtop - m); vinv = 2^(m - vtop)
+      float m = -INFINITY, l = 0.0f, vtop = -INFINITY, vinv = 0.0f;
       if (nblk > 0) {
         if constexpr (AHEAD) {
 #pragma unroll
@@ -585,20 +595,6 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               if ((good >> (((col + 32 * q) >> a.group_log2) + i)) & 1u) pages |= ((1u << (1 << a.group_log2)) - 1u) << (i << a.group_log2);
             return v & pages;
           };
-          float vmax = 0.0f;
-          if constexpr (Q8) {  // the largest finite value scale of the block's readable keys: lane l looks at 4 l ..
-            const float4 v = *reinterpret_cast<const float4*>(ks + 128 + lane * 4);
-            const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if ((whole || (kb + lane * 4 + k < end && ((good >> ((lane * 4 + k) >> a.group_log2)) & 1u))) && x[k] < INFINITY)
-                vmax = fmaxf(vmax, x[k]);
-            vmax = __any_sync(0xffffffffu, vmax > 64.0f * vref) ? vmax : 0.0f;
-            if (__any_sync(0xffffffffu, vmax > 0.0f)) {
-#pragma unroll
-              for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-            }
-          }
           // One step of 32 or 64 columns keeps its scores; more are read twice. Blocks that are not seen whole take a loop of
           // their own, in steps of 32.
           constexpr int STEP = Q8 ? 32 : 64;
@@ -611,12 +607,14 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             for (int i = 0; i < 32; ++i)
               if (!((v >> i) & 1u)) y[i] = -INFINITY;
           };
-          float mb = -INFINITY;
+          float mb = -INFINITY, vb = -INFINITY;  // the largest score, and the largest with the value scale in it
+          const float* vs = ks + 128 + col;
           if (!whole) {
 #pragma unroll 1
             for (int q = 0; q < W / 32; ++q) {
               masked(q);
               mb = fmaxf(mb, ptc_max(reinterpret_cast<float (&)[32]>(x)));
+              if constexpr (Q8) vb = fmaxf(vb, ptc_high(reinterpret_cast<float (&)[32]>(x), vs + q * 32, fac));
             }
           } else if (W == 32) {
             ptc_scores<Q8>(s_addr + col, ks + col, reinterpret_cast<float (&)[32]>(x));
@@ -629,19 +627,43 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             }
           }
           mb *= fac;
-          const bool grows = mb > m + 8.0f;  // (m = -inf: any finite score)
-          const bool vgrows = Q8 && vmax > 64.0f * vref;
-          if (__any_sync(0xffffffffu, grows) || vgrows) {
+          if constexpr (Q8) {
+            // No product passes the largest score with the largest scale (but for roundings, hence 5.9): the products are looked at
+            // only if that would matter. Whether they are may depend on the warp's other rows, what is then decided does not.
+            if (whole) {
+              const float4 v = *reinterpret_cast<const float4*>(ks + 128 + lane * 4);
+              const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
+              const int d = __float_as_int(mb - vtop);  // (as whole numbers, negative ones turned round, floats are in order)
+              const int far = __reduce_max_sync(0xffffffffu, d ^ ((d >> 31) & 0x7fffffff));
+              if (!(__int_as_float(far ^ ((far >> 31) & 0x7fffffff)) + __log2f(__uint_as_float(most)) <= 5.9f)) {
+                if (W == 32) {
+                  vb = ptc_high(x, vs, fac);
+                } else {
+#pragma unroll 1
+                  for (int q = W / STEP - 1; q >= 0; --q) {
+                    ptc_scores<Q8>(s_addr + col + q * STEP, ks + col + q * STEP, x);
+                    vb = fmaxf(vb, ptc_high(x, vs + q * STEP, fac));
+                  }
+                }
+              }
+            }
+          }
+          // (m = -inf: any finite score; codes: a weight of 2^6 times a value scale of at most 2^121 is a number)
+          const bool grows = mb > m + (Q8 ? 6.0f : 8.0f);
+          const bool vgrows = Q8 && vb > vtop + 6.0f;
+          if (__any_sync(0xffffffffu, grows || vgrows)) {
             const float mn = grows ? mb : m;
             float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
             m = mn;
             l *= al;
-            if (vgrows) {
-              if (vmax >= 1.2e-38f) al *= __fdividef(vref, vmax);
-              vref = vmax;
-              vinv = vref >= 1.2e-38f ? __frcp_rn(vref) : 0.0f;
+            if constexpr (Q8) {  // O stays where only m has grown: it is over the reference
+              const float to = vgrows ? vb : vtop;
+              al = to == -INFINITY ? 1.0f : ex2(vtop - to);
+              vtop = to;
+              const float half = ex2(0.5f * (m - vtop));  // (2^(m - vtop) may be below the normal numbers)
+              vinv = vtop > m - 126.0f ? half * half : 0.0f;
             }
-            if (j >= C::STREAMS) {  // (else nothing is on O yet)
+            if (j >= C::STREAMS && (!Q8 || __any_sync(0xffffffffu, al != 1.0f))) {  // (else nothing is on O yet)
               // the last product on this O is done: it was issued before this S (D = 256: after it)
               if (C::STREAMS == 1) {
                 if (!mbar_wait(o_bar, (pho + j - 1) & 1u, EX_DEVERR_WAIT_MMA)) *sfail = 1;
@@ -661,7 +683,6 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           }
           const float sub = m == -INFINITY ? 0.0f : m;
           const uint32_t p_addr = s_addr + (col >> 1);
-          const float* vs = ks + 128 + col;
           if (!whole) {
 #pragma unroll 1
             for (int q = 0; q < W / 32; ++q) {
@@ -704,10 +725,10 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       asm volatile("bar.sync 2, 256;" ::: "memory");  // (every product is done: the queries may be written over)
       if (*sfail) break;  // the same for every thread here: the flag is only set before the barrier
       tc_fence_after();
-      float* sm = reinterpret_cast<float*>(smem);  // [2 streams][128]: m, then l, then the references of the value scales
+      float* sm = reinterpret_cast<float*>(smem);  // [2 streams][128]: m, then l, then 2^(vtop - m)
       sm[wg * 128 + r] = m;
       sm[256 + wg * 128 + r] = l;
-      sm[512 + wg * 128 + r] = vref;
+      if constexpr (Q8) sm[512 + wg * 128 + r] = vtop > -INFINITY ? ex2(vtop - m) : 0.0f;
       asm volatile("bar.sync 2, 256;" ::: "memory");
       pho += w.nblk;
       blocks += w.nblk;
