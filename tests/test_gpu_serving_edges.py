@@ -177,3 +177,24 @@ def test_value_scales_of_keys_with_little_weight(dtype, T, bits, ratio):
         seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
         want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, scale, BF, True)
         check(got[b * T:b * T + T], want, bound, b)
+
+
+# ---- tiny values
+@pytest.mark.parametrize("dtype", [I8, E4])
+@pytest.mark.parametrize("T", [1, 4, 6, 33])
+@pytest.mark.parametrize("down", [100, 118, 122, 126, 132])
+def test_values_next_to_the_smallest_numbers(dtype, T, down):
+    """Values of 2^-down: their scales are below float32's normal numbers, what they stand for is not below bf16's."""
+    H, KV, D, lens = 8, 2, 128, [300, 2600]
+    c = Cache(lens, 16, KV, D, dtype, garbage=False)
+    c.ds[1].mul_(2.0 ** -down)
+    small = c.ds[1].cpu().double()
+    c.real[1] = c.codes[1].float().double() * small.transpose(1, 2).unsqueeze(-1)
+    q = torch.randn(len(lens) * T, H, D, generator=gen(4)).to(BF)
+    got = decode(c, q.to(DEV), 0.1) if T == 1 else tree(c, q, [T] * len(lens), 0.1, None)
+    for b, L in enumerate(lens):
+        seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+        want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 0.1, BF, True)
+        # the bound tells them from zeros (at 2^-126 and 2600 keys it is a tenth of them)
+        assert down > 122 or float(want.abs().max()) > 16 * float(bound.min())
+        check(got[b * T:b * T + T], want, bound, b)

@@ -598,9 +598,10 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            const float to = v > 64.0f * vref[x] ? v : vref[x];
-            const bool tiny = to < 1.2e-38f;  // such values are zero next to any output type's smallest step
-            vinv[x] = tiny ? 0.0f : __frcp_rn(to);
+            // At least 2^-126, so that its reciprocal is a number: products down to 2^-149 are then above 2^-24, and what they
+            // lose (2^-25 times 2^-126 times a code) is below bf16's smallest step.
+            const float to = fmaxf(v > 64.0f * vref[x] ? v : vref[x], 0x1p-126f);
+            vinv[x] = __frcp_rn(to);
             const float be = to == vref[x] ? 1.0f : vref[x] * vinv[x];
             vref[x] = to;
 #pragma unroll

@@ -657,11 +657,11 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             m = mn;
             l *= al;
             if constexpr (Q8) {  // O stays where only m has grown: it is over the reference
-              const float to = vgrows ? vb : vtop;
+              const float to = fmaxf(vgrows ? vb : vtop, m - 126.0f);  // (what it is divided by stays a normal number)
               al = to == -INFINITY ? 1.0f : ex2(vtop - to);
               vtop = to;
               const float half = ex2(0.5f * (m - vtop));  // (2^(m - vtop) may be below the normal numbers)
-              vinv = vtop > m - 126.0f ? half * half : 0.0f;
+              vinv = vtop > -INFINITY ? half * half : 0.0f;
             }
             if (j >= C::STREAMS && (!Q8 || __any_sync(0xffffffffu, al != 1.0f))) {  // (else nothing is on O yet)
               // the last product on this O is done: it was issued before this S (D = 256: after it)
@@ -728,7 +728,10 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       float* sm = reinterpret_cast<float*>(smem);  // [2 streams][128]: m, then l, then 2^(vtop - m)
       sm[wg * 128 + r] = m;
       sm[256 + wg * 128 + r] = l;
-      if constexpr (Q8) sm[512 + wg * 128 + r] = vtop > -INFINITY ? ex2(vtop - m) : 0.0f;
+      if constexpr (Q8) {
+        const float half = ex2(0.5f * (vtop - m));
+        sm[512 + wg * 128 + r] = vtop > -INFINITY ? half * half : 0.0f;
+      }
       asm volatile("bar.sync 2, 256;" ::: "memory");
       pho += w.nblk;
       blocks += w.nblk;
