@@ -198,3 +198,25 @@ def test_values_next_to_the_smallest_numbers(dtype, T, down):
         # the bound tells them from zeros (at 2^-126 and 2600 keys it is a tenth of them)
         assert down > 122 or float(want.abs().max()) > 16 * float(bound.min())
         check(got[b * T:b * T + T], want, bound, b)
+
+
+def test_prompt_attention_scores_of_minus_infinity():
+    """Keys whose scores are -infinity, whole blocks of them and the first ones, have no weight."""
+    from vllm_exact import prompt_attn as A
+    for D, real in ((64, BF), (128, BF), (128, FP), (256, BF)):
+        H, KV, L, gone = 4, 2, 1100, 300
+        g = gen(D)
+        q = torch.randn(L, H, D, generator=g)
+        q[..., 0] = q[..., 0].abs() + 0.5
+        q = q.to(real)
+        k, v = (torch.randn(L, KV, D, generator=g).to(real) for _ in range(2))
+        k[:gone, :, 0] = -float("inf")
+        got = A.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu([L]), cu([L]), 0.1)
+        k[:gone, :, 0] = 0
+        seen = torch.ones(L, L, dtype=torch.bool).tril()
+        seen[:, :gone] = False
+        want, bound = S.attend(q, k, v, seen, 0.1, real)
+        check(got[gone:], want[gone:], bound[gone:], (D, real))
+        k[:gone, :, 0] = -float("inf")
+        for lo, hi in ((256, 420), (700, 1100)):  # and with other rows in the tiles
+            assert torch.equal(A.prompt_attention(q[lo:hi].to(DEV), k[:hi].to(DEV), v[:hi].to(DEV), cu([hi - lo]), cu([hi]), 0.1)[gone - min(lo, gone):], got[max(lo, gone):hi])

@@ -529,8 +529,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
       tmem_ld_wait();
       // A block that is seen whole is weighed with the reference that there is, while its largest score is still being looked
-      // for: nothing waits for it. If a score of the warp passes its row's reference by too much (or is NaN), or the block is
-      // an edge, or the first, the block is weighed (again) below.
+      // for: nothing waits for it. If a score of the warp passes its row's reference by too much (or is NaN), or a row has none
+      // yet (every score so far was -infinity), or the block is an edge, or the first, the block is weighed (again) below.
       bool again = j >= whole || j == 0;
       f32x2 sum0 = pair(0.0f, 0.0f), sum1 = sum0;
       // The weights of the block against the reference, written over S, and their sums. Both callers have the same arithmetic
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         const float mb = max_nan(max3_nan(mx[0], s[126], s[127]), mx[1]);
         weigh(m * sc, std::false_type{});
-        again = !(mb <= m + grow);
+        again = !(mb <= m + grow) || m == -INFINITY;  // (no reference yet: the weights just made are not numbers)
       }
       if (__any_sync(0xffffffffu, again)) {
         if (j >= whole) {
