@@ -340,8 +340,8 @@ int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, co
  * Causal attention of packed prompts: sequence b < n has query rows cu_q[b] .. cu_q[b + 1] of q (tokens x H x D) and
  * key rows cu_k[b] .. cu_k[b + 1] of k and v (keys x KV x D), all bf16 or all fp16; its last query is its last key's
  * token, so query i sees keys j <= i + Lk - Lq (the keys may start before the queries: a continued conversation). A
- * query that sees no key gives zeros. Rows of no sequence are left untouched; a sequence whose offsets leave the
- * arrays is skipped. scale must be positive and finite. A row's bits depend on its own query and on the keys and values of its
+ * query that sees no key gives zeros. Rows of no sequence are left untouched; a sequence whose offsets (of
+ * queries or of keys) leave the arrays or run backwards is skipped. scale must be positive and finite. A row's bits depend on its own query and on the keys and values of its
  * sequence that it sees, alone: a prompt in pieces, each over all keys so far, gives the bits of the whole.
  */
 int ex_prompt_attention(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,

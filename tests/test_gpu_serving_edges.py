@@ -220,3 +220,28 @@ def test_prompt_attention_scores_of_minus_infinity():
         k[:gone, :, 0] = -float("inf")
         for lo, hi in ((256, 420), (700, 1100)):  # and with other rows in the tiles
             assert torch.equal(A.prompt_attention(q[lo:hi].to(DEV), k[:hi].to(DEV), v[:hi].to(DEV), cu([hi - lo]), cu([hi]), 0.1)[gone - min(lo, gone):], got[max(lo, gone):hi])
+
+
+def test_prompt_attention_offsets_that_are_not_followed():
+    """Sequences whose offsets leave the arrays, of queries or of keys, or run backwards: their rows are left as they were."""
+    from vllm_exact import prompt_attn as A
+    H, KV, D = 4, 2, 64
+    g = gen(1)
+    q = torch.randn(400, H, D, generator=g).to(BF).to(DEV)
+    k, v = (torch.randn(500, KV, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    alone = A.prompt_attention(q[:100], k[:120], v[:120], cu([100]), cu([120]), 0.1)
+    for cq, ck in ((i32(0, 100, 350), i32(0, 120, 501)), (i32(0, 100, 350), i32(0, 120, 2 ** 31 - 1)),
+                   (i32(0, 100, 401), i32(0, 120, 400)), (i32(0, 100, 350), i32(0, 120, 100)),
+                   (i32(0, 100, 350), i32(0, 120, -(2 ** 31)))):
+        out = torch.full_like(q, 7.0)
+        A.prompt_attention(q, k, v, cq, ck, 0.1, out=out)
+        assert torch.equal(out[:100], alone) and bool((out[100:] == 7.0).all()), (cq, ck)
+    out = torch.full_like(q, 7.0)
+    A.prompt_attention(q, k, v, i32(0, 100, 350), i32(0, 120, 120), 0.1, out=out)  # no keys: zeros
+    assert torch.equal(out[:100], alone) and bool((out[100:350] == 0).all()) and bool((out[350:] == 7.0).all())
+    # sequences behind such a one are served
+    want = A.prompt_attention(q[100:350], k[200:500], v[200:500], cu([250]), cu([300]), 0.1)
+    out = torch.full_like(q, 7.0)
+    A.prompt_attention(q, k, v, i32(0, 100, 10 ** 9, 100, 350), i32(0, 120, 120, 200, 500), 0.1, out=out)
+    assert torch.equal(out[:100], alone) and torch.equal(out[100:350], want) and bool((out[350:] == 7.0).all())

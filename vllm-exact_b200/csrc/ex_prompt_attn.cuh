@@ -143,7 +143,8 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 }
 
 // The tile'th tile of `rows` queries over all sequences: its first query in its sequence, and that sequence's first query
-// and key and numbers of both (offsets that leave the arrays, or run backwards, are not followed); false if there is none.
+// and key and numbers of both (a sequence whose offsets leave the arrays or run backwards, of queries or of keys, is taken to
+// have no tiles: nothing of it is read or written); false if there is none.
 // Every offset is loaded in the one pass: a second, dependent round of loads would cost 700 cycles.
 __device__ __forceinline__ bool pa_find_tile(const PaArgs& a, int rows, int tile, int& row0, int& q0, int& Lq, int& k0, int& Lk) {
   const int lane = threadIdx.x & 31;
@@ -155,7 +156,7 @@ __device__ __forceinline__ bool pa_find_tile(const PaArgs& a, int rows, int tile
       qb = a.cu_q[base + lane + 1];
       ka = a.cu_k[base + lane];
       kb = a.cu_k[base + lane + 1];
-      c = (int)((max((int64_t)0, (int64_t)qb - qa) + rows - 1) / rows);
+      if (qa >= 0 && qa <= qb && qb <= a.tokens && ka >= 0 && ka <= kb && kb <= a.keys) c = (int)(((int64_t)qb - qa + rows - 1) / rows);
     }
     int incl = c;
 #pragma unroll
@@ -169,9 +170,8 @@ __device__ __forceinline__ bool pa_find_tile(const PaArgs& a, int rows, int tile
       row0 = (tile - seen - __shfl_sync(0xffffffffu, incl - c, l)) * rows;
       q0 = __shfl_sync(0xffffffffu, qa, l);
       k0 = __shfl_sync(0xffffffffu, ka, l);
-      const int64_t q1 = __shfl_sync(0xffffffffu, qb, l), k1 = __shfl_sync(0xffffffffu, kb, l);
-      Lq = q0 >= 0 && q1 <= a.tokens ? (int)max((int64_t)0, q1 - q0) : 0;
-      Lk = k0 >= 0 && k1 <= a.keys ? (int)max((int64_t)0, k1 - k0) : 0;
+      Lq = __shfl_sync(0xffffffffu, qb, l) - q0;
+      Lk = __shfl_sync(0xffffffffu, kb, l) - k0;
       return true;
     }
     seen += __shfl_sync(0xffffffffu, incl, 31);

@@ -21,7 +21,8 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, scale, out=N
     rows cu_seqlens_k[b] .. cu_seqlens_k[b + 1] (int32, n + 1 entries each). Its last query is its last key's token:
     query i sees the keys j <= i + Lk - Lq, so keys may start before the queries (a continued conversation, its cached
     beginning read with kv_cache.cache_read). A query that sees no key gives zeros. Query head h reads KV head
-    h // (H / KV). scale is positive. Returns out (like query; made if not given); its rows of no sequence are left as they were."""
+    h // (H / KV). scale is positive. Returns out (like query; made if not given); its rows of no sequence, and those of a
+    sequence whose offsets leave the arrays or run backwards, are left as they were."""
     dev = query.get_device()  # -1: not on a GPU
     if (dev < 0 or key.get_device() != dev or value.get_device() != dev or cu_seqlens_q.get_device() != dev
             or cu_seqlens_k.get_device() != dev):
