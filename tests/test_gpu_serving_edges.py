@@ -245,3 +245,20 @@ def test_prompt_attention_offsets_that_are_not_followed():
     out = torch.full_like(q, 7.0)
     A.prompt_attention(q, k, v, i32(0, 100, 10 ** 9, 100, 350), i32(0, 120, 120, 200, 500), 0.1, out=out)
     assert torch.equal(out[:100], alone) and torch.equal(out[100:350], want) and bool((out[350:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [None, I8, E4])
+@pytest.mark.parametrize("T", [2, 6, 33])
+def test_tree_scales_that_leave_no_score(dtype, T):
+    """A softmax scale of 1e-30, queries of zeros and next to zeros: every key that is seen weighs the same."""
+    H, KV, D, lens = 8, 2, 128, [100, 700]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(2 * T, H, D, generator=gen(5)).to(BF)
+    q[0] = 0
+    q[1] = q[1] * 1e-38
+    q[T] = 0
+    got = tree(c, q, [T, T], 1e-30, None)
+    for b, L in enumerate(lens):
+        seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+        want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 1e-30, BF, dtype is not None)
+        check(got[b * T:b * T + T], want, bound, b)

@@ -515,7 +515,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
           v.z = pack2<__half>(y[4] * inv, y[5] * inv);
           v.w = pack2<__half>(y[6] * inv, y[7] * inv);
         }
-        if (qc == 0) sfac[x] = f * fabsf(a.scale_log2);
+        if (qc == 0) sfac[x] = fmaxf(f * fabsf(a.scale_log2), 1e-45f);  // (0 times the -infinity of a hidden key would be NaN)
       }
       if (a.scale_log2 < 0.0f) {  // the largest score is looked for before it is scaled
         v.x ^= 0x80008000u;
