@@ -262,3 +262,35 @@ def test_tree_scales_that_leave_no_score(dtype, T):
         seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
         want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 1e-30, BF, dtype is not None)
         check(got[b * T:b * T + T], want, bound, b)
+
+
+@pytest.mark.parametrize("real", [BF, FP])
+@pytest.mark.parametrize("T", DRAFTS + [8])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tree_infinities_in_the_context(real, T, D):
+    """An infinite value that every row sees makes its own element infinite, in every row, and no other; infinities of both
+    signs, or one and a NaN, make NaN."""
+    H, KV, L = 8, 2, 900
+    c = Cache([L, 300], 16, KV, D, None, real=real)
+    for pos in (5, 40, 70, 200, 300, 301, 700):  # a score of 0: some weight in 16 bits
+        c.dk[int(c.table[0, pos // 16]), pos % 16] = 0
+    q = torch.randn(2 * T, H, D, generator=gen(5)).to(real)
+    clean = tree(c, q, [T, T], 0.1, None)
+    inf = float("inf")
+
+    def put(pos, head, d, x):
+        c.dv[int(c.table[0, pos // 16]), pos % 16, head, d] = x
+
+    put(5, 0, 3, inf)
+    put(200, 0, 3, inf)
+    put(70, 0, 9, -inf)
+    put(300, 1, D - 1, inf)
+    put(301, 1, D - 1, -inf)
+    put(40, 1, 0, -inf)
+    put(700, 1, 0, float("nan"))
+    got = tree(c, q, [T, T], 0.1, None)
+    bad = torch.zeros(2 * T, H, D, dtype=torch.bool, device=DEV)
+    bad[:T, :4, 3] = bad[:T, :4, 9] = bad[:T, 4:, D - 1] = bad[:T, 4:, 0] = True
+    assert torch.equal(got[~bad], clean[~bad])
+    assert bool((got[:T, :4, 3] == inf).all()) and bool((got[:T, :4, 9] == -inf).all())
+    assert bool(torch.isnan(got[:T, 4:, D - 1]).all()) and bool(torch.isnan(got[:T, 4:, 0]).all())

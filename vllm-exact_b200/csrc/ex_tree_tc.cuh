@@ -758,6 +758,39 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         for (int i = 0; i < 8; ++i) any |= mine[i] != 0;
       const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
       asm volatile("bar.sync 2, 256;" ::: "memory");  // sm has been read
+      // Values of the context that are not finite, where a row stands in the tile more than once: a copy's weights of 0 for the
+      // other copies' keys have made NaN of them. Dims d0 .. of the keys that every row sees (those of edge blocks have
+      // been taken out) are looked at again: an element that is not finite because of them becomes the sum of the copy's own.
+      auto context_infinities = [&](float (&o)[16], int d0) {
+        float own[16] = {};
+        uint32_t others = 0;
+#pragma unroll 1
+        for (int x = 0; x < w.jedge * 128; ++x) {
+          const int key = w.start + x, page = a.bt[(int64_t)w.b * a.sbt + key / a.BS];
+          if (page < 0 || page >= a.blocks) continue;
+          const uint4* e = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
+                                                          (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0);
+          const uint4 lo = e[0], hi = e[1];
+          const uint32_t z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          uint32_t some = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) some |= not_finite<F16>(z[i]);
+          if (some == 0) continue;
+          const bool mine = (x & 127) >= col && (x & 127) < col + W;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint16_t h = (uint16_t)(z[i >> 1] >> (16 * (i & 1)));
+            const float y = F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
+            if (!(fabsf(y) < INFINITY)) {
+              if (mine) own[i] += y;
+              else others |= 1u << i;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(fabsf(o[i]) < INFINITY) && (own[i] != 0.0f || ((others >> i) & 1u))) o[i] = own[i];
+      };
       float* piece = reinterpret_cast<float*>(smem) + wg * 128 * CD;  // [128][CD], 4 floats a chunk, swizzled
       const int t2 = tid & 127;
 #pragma unroll 1
@@ -774,7 +807,18 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             for (int i = 0; i < 16; ++i) {
               o[i] = some[0] ? __uint_as_float(u[i]) * f[0] : 0.0f;
               o[i] += some[1] ? __uint_as_float(v[i]) * f[1] : 0.0f;
-              if (single) o[i] *= inv;
+            }
+            if constexpr (!Q8) {
+              if (copies > 1 && lall < INFINITY) {  // (NaN weights are NaN whatever the values)
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) bad |= !(fabsf(o[i]) < INFINITY);
+                if (bad) context_infinities(o, c + k);
+              }
+            }
+            if (single) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= inv;
             }
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
