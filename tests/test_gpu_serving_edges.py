@@ -294,3 +294,55 @@ def test_tree_infinities_in_the_context(real, T, D):
     assert torch.equal(got[~bad], clean[~bad])
     assert bool((got[:T, :4, 3] == inf).all()) and bool((got[:T, :4, 9] == -inf).all())
     assert bool(torch.isnan(got[:T, 4:, D - 1]).all()) and bool(torch.isnan(got[:T, 4:, 0]).all())
+
+
+# ---- values that are not finite and that a row may not see
+@pytest.mark.parametrize("kind", [BF, FP, E4])
+@pytest.mark.parametrize("T", DRAFTS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tree_hidden_values_that_are_not_finite_change_no_bit(kind, T, D):
+    """NaN, infinities (16-bit) and NaN codes (e4m3) in a drafted token's values: element by element in the rows that see it,
+    not a bit in the others. A row that sees it sees it however small its weight is."""
+    H, KV = 8, 2
+    lens = [100, 700]
+    c = Cache(lens, 16, KV, D, E4 if kind == E4 else None, real=BF if kind == E4 else kind)
+    q = torch.randn(2 * T, H, D, generator=gen(5))
+    q[..., 1] = q[..., 1].abs() + 4
+    q = q.to(BF if kind == E4 else kind)
+    w, see = words(T, "tree", gen(9))
+    bad = T // 2
+    see[:, bad] &= torch.arange(T) % 2 == bad % 2
+    w = [sum(1 << j for j in range(T) if see[i, j]) for i in range(T)]
+    w = [x - (1 << 64) if x >> 63 else x for x in w]
+    for b in range(2):  # a score of about -500: no weight at all in float32
+        pos = lens[b] - T + bad
+        blk, off = int(c.table[b, pos // 16]), pos % 16
+        if kind == E4:
+            c.dk.view(torch.uint8)[blk, off, :, 1] = 0xfe  # -448
+            c.ds[0][blk, :, off] = 4.0
+        else:
+            c.dk[blk, off, :, 1] = -2000.0
+    clean = tree(c, q, [T, T], 0.1, w * 2)
+    for b in range(2):
+        pos = lens[b] - T + bad
+        blk, off = int(c.table[b, pos // 16]), pos % 16
+        if kind == E4:
+            c.dv.view(torch.uint8)[blk, off, 0, 3] = 0x7f
+            c.dv.view(torch.uint8)[blk, off, 1, D - 1] = 0xff
+        else:
+            c.dv[blk, off, 0, 3] = float("nan")
+            c.dv[blk, off, 1, D - 1] = float("inf")
+            c.dv[blk, off, 1, 16] = -float("inf")
+    got = tree(c, q, [T, T], 0.1, w * 2)
+    hit = torch.zeros(2 * T, H, D, dtype=torch.bool, device=DEV)
+    sees = see[:, bad].repeat(2).to(DEV)
+    hit[sees, :4, 3] = True
+    hit[sees, 4:, D - 1] = True
+    if kind != E4:
+        hit[sees, 4:, 16] = True
+    assert torch.equal(got[~hit], clean[~hit]) and bool(torch.isfinite(clean).all())
+    assert bool(torch.isnan(got[sees][:, :4, 3]).all())
+    if kind == E4:
+        assert bool(torch.isnan(got[sees][:, 4:, D - 1]).all())
+    else:
+        assert bool((got[sees][:, 4:, D - 1] == float("inf")).all()) and bool((got[sees][:, 4:, 16] == -float("inf")).all())

@@ -193,6 +193,19 @@ __device__ __forceinline__ float pr_query_scale(float m, float& f) {
   return __uint_as_float((uint32_t)(254 - e) << 23);
 }
 
+// Two 16-bit values or four codes in a word: a bit (15, 31; e4m3 7, 15, 23, 31) for each that is not finite. One more than the
+// largest exponent (e4m3: than the NaN code, which is all ones) carries into the place of the sign, and no further.
+template <int CODE, bool F16>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (CODE == CODE_E4M3) return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return ((w & (F16 ? 0x7c007c00u : 0x7f807f80u)) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+template <int CODE, bool F16>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {  // zeros for the others
+  const uint32_t n = not_finite<CODE, F16>(w);
+  return w & ~(CODE == CODE_E4M3 ? (n >> 7) * 0xffu : (n >> 15) * 0xffffu);
+}
+
 // a word of the transposing load: dims 2x, 2x + 1 of two keys, as the two keys' dim 2x and their dim 2x + 1
 template <int CODE>
 __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
@@ -477,10 +490,10 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             sc[i][j][2 * e + 1] *= Q8 ? fac[2 * j + 1] * ksc : fac[2 * j + 1];
           }
         }
-      bool slow = false;  // 16-bit: a value that is not finite and that some row may not see
+      bool odd = false;  // a value that is not finite and that some row may not see
       uint32_t hidden = 0;  // bit ((i NT + j) 4 + e): the row does not see the key
       if (!whole) {
-        int bad = 0;
+        uint32_t bad = 0;
 #pragma unroll
         for (int i = 0; i < MK; ++i) {
 #pragma unroll
@@ -511,17 +524,14 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(i, c));
             if (none) {
               *x = make_uint4(0, 0, 0, 0);  // values that may not be read: 0 * NaN would reach O
-            } else if constexpr (!Q8) {
-              const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-              const uint32_t w[4] = {x->x, x->y, x->z, x->w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || ((w[k] >> 16) & e) == e;
+            } else if constexpr (CODE != CODE_INT8) {
+              bad |= not_finite<CODE, F16>(x->x) | not_finite<CODE, F16>(x->y) | not_finite<CODE, F16>(x->z) | not_finite<CODE, F16>(x->w);
             }
           }
         }
         fence_proxy_async_shared();  // the ring slot is written by TMA next
         __syncwarp();
-        if constexpr (!Q8) slow = __any_sync(0xffffffffu, bad);
+        if constexpr (CODE != CODE_INT8) odd = __any_sync(0xffffffffu, bad != 0);
       }
       // references: taken up for the rows that need it
       float top[2 * NT];
@@ -626,60 +636,69 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
           pb[i][j][0] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][0], sc[i][j][1]) : pack_bf16(sc[i][j][0], sc[i][j][1]));
           pb[i][j][1] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][2], sc[i][j][3]) : pack_bf16(sc[i][j][2], sc[i][j][3]));
         }
-      const int mi = lane >> 3;
-      if (!Q8 && slow) {
-        // one product at a time: a weight of 0 leaves a value out that is not finite
+      if (CODE != CODE_INT8 && odd) {
+        // Added as they are (their weight is positive, however small) to the rows that see them, then taken out: 0 times one of
+        // them would reach the others. Dims of a lane: 16-bit qr, qr + 8 of every 16, codes 2 qr, 2 qr + 1.
 #pragma unroll 1
         for (int kk = 0; kk < 16 * MK; ++kk) {
+          const int d = kb + kk - ctx;
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // weight of (row 8 j + qc + e, key kk): in pb[kk / 16][j][kk / 8 % 2] of lane (qc + e) * 4 + kk % 8 / 2
-              uint32_t w = 0;
+            for (int u = 0; u < 2; ++u) {
+              const uint8_t* at = vs + (Q8 ? pr_at<C::PITCH, C::HALF>(kk, mt) + 2 * qr + u : pr_at<C::PITCH, C::HALF>(kk, 2 * mt + u) + 2 * qr);
+              float v;
+              if constexpr (Q8) {
+                v = (*at & 0x7f) == 0x7f ? NAN : 0.0f;
+              } else {
+                const uint16_t w = *reinterpret_cast<const uint16_t*>(at);
+                v = F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+              }
+              if (fabsf(v) < INFINITY) continue;
 #pragma unroll
-              for (int x = 0; x < 2 * MK; ++x)
-                if ((kk >> 3) == x) w = pb[x >> 1][j][x & 1];
-              w = __shfl_sync(0xffffffffu, w, (qc + e) * 4 + ((kk & 7) >> 1));
-              const uint32_t w16 = (kk & 1) ? w >> 16 : w & 0xffffu;
-              const float p = F16 ? __half2float(__ushort_as_half((uint16_t)w16)) : __uint_as_float(w16 << 16);
-#pragma unroll
-              for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  const int d = mt * 16 + qr + 8 * u;
-                  const uint16_t vr = *reinterpret_cast<const uint16_t*>(vs + pr_at<C::PITCH, C::HALF>(kk, d >> 3) + (d & 7) * 2);
-                  const float v = F16 ? __half2float(__ushort_as_half(vr)) : __uint_as_float((uint32_t)vr << 16);
-                  if (p != 0.0f) o[mt][j][2 * u + e] += p * v;
-                }
+              for (int x = 0; x < 2 * NT; ++x) {
+                const int r = (x >> 1) * 8 + qc + (x & 1), t = r / a.G;
+                if (r >= R) continue;
+                if (d >= 0 && !(((a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull)) >> d) & 1ull)) continue;
+                o[mt][x >> 1][2 * u + (x & 1)] += v;
+              }
             }
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < MK; ++i) {
-          const uint32_t vbase = ex_smem_u32(vs) +
-                                 (Q8 ? pr_at<C::PITCH, C::HALF>(16 * i + (mi & 1) * 8 + (lane & 7), mi >> 1)
-                                     : pr_at<C::PITCH, C::HALF>(16 * i + (mi >> 1) * 8 + (lane & 7), mi & 1));
-#pragma unroll
-          for (int mt = 0; mt < KT; mt += (Q8 ? 2 : 1)) {
-            const int c = Q8 ? mt : 2 * mt;
-            uint32_t va[2][4], w[4];  // codes: keys 0-7 | 8-15 of a 16-byte chunk (16 dims), then of the next
-            ldsm_x4_t((vbase ^ ((c & 7) << 4)) + (c >> 3) * C::HALF, w);
-            if constexpr (Q8) {
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                transposed_to_f16<CODE>(w[2 * u], va[u][0], va[u][1]);
-                transposed_to_f16<CODE>(w[2 * u + 1], va[u][2], va[u][3]);
-              }
-            } else {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) va[0][x] = w[x];
-            }
-#pragma unroll
-            for (int u = 0; u < (Q8 ? 2 : 1); ++u)
-#pragma unroll
-              for (int j = 0; j < NT; ++j) mma_16816<MF16>(o[mt + u][j], va[u], pb[i][j][0], pb[i][j][1]);
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < 16 * MK; ++i)
+          for (int c = lane; c < C::ROW / 16; c += 32) {
+            uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(i, c));
+            *x = make_uint4(only_finite<CODE, F16>(x->x), only_finite<CODE, F16>(x->y), only_finite<CODE, F16>(x->z), only_finite<CODE, F16>(x->w));
           }
+        fence_proxy_async_shared();
+        __syncwarp();
+      }
+      const int mi = lane >> 3;
+#pragma unroll
+      for (int i = 0; i < MK; ++i) {
+        const uint32_t vbase = ex_smem_u32(vs) +
+                               (Q8 ? pr_at<C::PITCH, C::HALF>(16 * i + (mi & 1) * 8 + (lane & 7), mi >> 1)
+                                   : pr_at<C::PITCH, C::HALF>(16 * i + (mi >> 1) * 8 + (lane & 7), mi & 1));
+#pragma unroll
+        for (int mt = 0; mt < KT; mt += (Q8 ? 2 : 1)) {
+          const int c = Q8 ? mt : 2 * mt;
+          uint32_t va[2][4], w[4];  // codes: keys 0-7 | 8-15 of a 16-byte chunk (16 dims), then of the next
+          ldsm_x4_t((vbase ^ ((c & 7) << 4)) + (c >> 3) * C::HALF, w);
+          if constexpr (Q8) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              transposed_to_f16<CODE>(w[2 * u], va[u][0], va[u][1]);
+              transposed_to_f16<CODE>(w[2 * u + 1], va[u][2], va[u][3]);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) va[0][x] = w[x];
+          }
+#pragma unroll
+          for (int u = 0; u < (Q8 ? 2 : 1); ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_16816<MF16>(o[mt + u][j], va[u], pb[i][j][0], pb[i][j][1]);
         }
       }
       __syncwarp();

@@ -226,18 +226,6 @@ __device__ __forceinline__ void ex2_pair(f32x2 x, float& a, float& b) {
   b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
-// Two 16-bit values in a word: a bit (15, 31) for each that is not finite. One more than the largest exponent carries into the
-// place of the sign, and no further.
-template <bool F16>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  return ((w & (F16 ? 0x7c007c00u : 0x7f807f80u)) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t only_finite(uint32_t w) {  // zeros for the others
-  const uint32_t n = not_finite<F16>(w);
-  return w & ~((n >> 15) * 0xffffu);
-}
-
 // The 128 values of a slot (`columns` swizzled columns of 64 dims): those from number `live` on become zeros, and so do numbers
 // that are not finite, whose keys are noted. 16 bytes of a key a thread, eight threads along a key's 128 bytes (no bank
 // conflict; with a key a thread a block took 7000 cycles), four keys in flight.
@@ -251,7 +239,7 @@ __device__ __forceinline__ void clean_values(uint8_t* vs, int columns, int t, in
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 w = x[i * STEP * 8];
-      bad |= not_finite<F16>(w.x) | not_finite<F16>(w.y) | not_finite<F16>(w.z) | not_finite<F16>(w.w);
+      bad |= not_finite<CODE_NONE, F16>(w.x) | not_finite<CODE_NONE, F16>(w.y) | not_finite<CODE_NONE, F16>(w.z) | not_finite<CODE_NONE, F16>(w.w);
     }
     if (live >= 128 && bad == 0) continue;
 #pragma unroll 1
@@ -260,8 +248,8 @@ __device__ __forceinline__ void clean_values(uint8_t* vs, int columns, int t, in
       const uint4 v = x[i * STEP * 8];
       if (key >= live) {
         x[i * STEP * 8] = make_uint4(0, 0, 0, 0);
-      } else if (not_finite<F16>(v.x) | not_finite<F16>(v.y) | not_finite<F16>(v.z) | not_finite<F16>(v.w)) {
-        x[i * STEP * 8] = make_uint4(only_finite<F16>(v.x), only_finite<F16>(v.y), only_finite<F16>(v.z), only_finite<F16>(v.w));
+      } else if (not_finite<CODE_NONE, F16>(v.x) | not_finite<CODE_NONE, F16>(v.y) | not_finite<CODE_NONE, F16>(v.z) | not_finite<CODE_NONE, F16>(v.w)) {
+        x[i * STEP * 8] = make_uint4(only_finite<CODE_NONE, F16>(v.x), only_finite<CODE_NONE, F16>(v.y), only_finite<CODE_NONE, F16>(v.z), only_finite<CODE_NONE, F16>(v.w));
         atomicOr(noted + (key >> 5), 1u << (key & 31));
       }
     }

@@ -16,7 +16,8 @@
 //                   than HBM takes to deliver it: so several warps share the boxes of every tile.
 //   warps 10, 11    16-bit: blocks with drafted tokens or the request's end; values behind the end are zeroed, values that
 //                   are not finite are zeroed and noted, and added in the end to the rows that see them
-//   warps 12-15     for codes: codes to float16 tiles (exact; keys behind the end to zeros)
+//   warps 12-15     for codes: codes to float16 tiles (exact; values behind the end to zeros, and in blocks with drafted tokens or
+//                   the end codes that are NaN, noted as 10 and 11 do)
 // 16-bit: bound by reading the cache once (a block of 128 keys is 64 KB for D = 128, 1.5 us of an SM's share of HBM) and by an
 // item's start and end, when only as much is read as the ring holds: queries 600 cycles (their loads run during the last
 // products), first scores 1400, last products 3000, results 8000, of 45000 for 2048 keys. 64 requests of 8192 keys with 16
@@ -122,6 +123,42 @@ __device__ __forceinline__ float ptc_weights(uint32_t p_addr, const float* vs, f
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// 16-bit values of the context that are not finite, where a row stands in the tile more than once: a copy's weights of 0 for
+// the other copies' keys have made NaN of them. The first `keys` keys from `start` on, which every row sees (values of edge
+// blocks have been taken out), are looked at again: an element of the 16 in o that is not finite because of them becomes the
+// sum of the copy's own, those of columns col .. col + W of a block.
+template <bool F16>
+__device__ __noinline__ void ptc_context_infinities(float* o, const int32_t* pages, int BS, int64_t blocks, const uint16_t* values,
+                                                    int64_t s_block, int64_t s_page, int start, int keys, int col, int W) {
+  float own[16] = {};
+  uint32_t others = 0;
+#pragma unroll 1
+  for (int x = 0; x < keys; ++x) {
+    const int key = start + x, page = pages[key / BS];
+    if (page < 0 || page >= blocks) continue;
+    const uint4* e = reinterpret_cast<const uint4*>(values + (int64_t)page * s_block + (int64_t)(key % BS) * s_page);
+    const uint4 lo = e[0], hi = e[1];
+    const uint32_t z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    uint32_t some = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) some |= not_finite<CODE_NONE, F16>(z[i]);
+    if (some == 0) continue;
+    const bool mine = (x & 127) >= col && (x & 127) < col + W;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint16_t h = (uint16_t)(z[i >> 1] >> (16 * (i & 1)));
+      const float y = F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
+      if (!(fabsf(y) < INFINITY)) {
+        if (mine) own[i] += y;
+        else others |= 1u << i;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (!(fabsf(o[i]) < INFINITY) && (own[i] != 0.0f || ((others >> i) & 1u))) o[i] = own[i];
+}
+
 constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
 constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values that are not finite are kept (the ring, of at most
                                // 8 slots, runs ahead of the rows)
@@ -133,6 +170,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   using C = PtcCfg<D, CODE>;
   constexpr bool Q8 = C::Q8;
   constexpr bool MF16 = Q8 || F16;
+  constexpr bool NOTES = CODE != CODE_INT8;  // some values may not be finite
   constexpr int ESZ = Q8 ? 1 : 2;
   constexpr int TM_S = 0, TM_O = 256;
   constexpr int CD = D == 64 ? 16 : 32;  // dims of a piece of the results: two pieces of 128 rows fit where Q was
@@ -432,8 +470,15 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       const int t = tid - 384;
       int rslot = 0, slot = 0;
       uint32_t rph = 0, ph = 1;
+      int item = 0;
       bool ok = true;
       while (ok && next()) {
+        uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
+        if (NOTES && jedge < nblk) {
+          ++item;
+          if (t < 8) mine[t] = 0;
+          asm volatile("bar.sync 6, 128;" ::: "memory");
+        }
 #pragma unroll 1
         for (int n = 0; n < 2 * nblk && ok; ++n) {
           int j;
@@ -443,7 +488,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             ok = mbar_wait(rfull_bar + rslot, rph, EX_DEVERR_WAIT_TMA) && mbar_wait(empty_bar + slot, ph, EX_DEVERR_WAIT_SLOT);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const uint8_t* src = raw + rslot * C::RAW;
+            uint8_t* src = raw + rslot * C::RAW;
             uint8_t* dst = ring + slot * C::SLOT;
             // 8 lanes take the same 16 codes of 8 keys (no bank twice), then the keys STEP on: the swizzle stays the same
             constexpr int CH = C::SW / 16, STEP = 128 / CH;
@@ -451,11 +496,25 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             src += C::SW == 128 ? r0 * 128 + ((c ^ (r0 & 7)) << 4) : r0 * 64 + ((c ^ ((r0 >> 1) & 3)) << 4);
             dst += (c >> 2) * C::SUB + r0 * 128;
             const int d0 = (c2 ^ (r0 & 7)) << 4, d1 = ((c2 + 1) ^ (r0 & 7)) << 4;
-            const int left = is_v ? end - (start + j * 128 + r0) : 128;  // values behind the end: zeros
+            if (is_v && j >= jedge) {  // values behind the end: zeros; codes that are NaN: zeros, noted
+              const int left = end - (start + j * 128 + r0);
+#pragma unroll 1
+              for (int i = 0; i < CH; ++i) {
+                uint4* x = reinterpret_cast<uint4*>(src + i * STEP * C::SW);
+                if (i * STEP >= left) {
+                  *x = make_uint4(0, 0, 0, 0);
+                } else if constexpr (NOTES) {
+                  const uint4 w = *x;
+                  if ((not_finite<CODE, F16>(w.x) | not_finite<CODE, F16>(w.y) | not_finite<CODE, F16>(w.z) | not_finite<CODE, F16>(w.w)) == 0) continue;
+                  *x = make_uint4(only_finite<CODE, F16>(w.x), only_finite<CODE, F16>(w.y), only_finite<CODE, F16>(w.z), only_finite<CODE, F16>(w.w));
+                  const int key = r0 + i * STEP;
+                  atomicOr(mine + (j - jedge) * 4 + (key >> 5), 1u << (key & 31));
+                }
+              }
+            }
 #pragma unroll 4
             for (int i = 0; i < CH; ++i) {
-              uint4 w = *reinterpret_cast<const uint4*>(src + i * STEP * C::SW);
-              if (i * STEP >= left) w = make_uint4(0, 0, 0, 0);
+              const uint4 w = *reinterpret_cast<const uint4*>(src + i * STEP * C::SW);
               uint32_t o[8];
               codes_to_f16<CODE>(w.x, o[0], o[1]);
               codes_to_f16<CODE>(w.y, o[2], o[3]);
@@ -754,43 +813,10 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       const bool have1 = C::STREAMS == 2 && w.nblk > 1;
       const bool single = pr_segments_many(pr_keys(a, w.L)) == 1;
       bool any = false;
-      if (!Q8 && w.jedge < w.nblk)
+      if (NOTES && w.jedge < w.nblk)
         for (int i = 0; i < 8; ++i) any |= mine[i] != 0;
       const float inv = lall > 0.0f ? 1.0f / lall : (lall == 0.0f ? 0.0f : lall);  // nothing seen: zeros; NaN stays NaN
       asm volatile("bar.sync 2, 256;" ::: "memory");  // sm has been read
-      // Values of the context that are not finite, where a row stands in the tile more than once: a copy's weights of 0 for the
-      // other copies' keys have made NaN of them. Dims d0 .. of the keys that every row sees (those of edge blocks have
-      // been taken out) are looked at again: an element that is not finite because of them becomes the sum of the copy's own.
-      auto context_infinities = [&](float (&o)[16], int d0) {
-        float own[16] = {};
-        uint32_t others = 0;
-#pragma unroll 1
-        for (int x = 0; x < w.jedge * 128; ++x) {
-          const int key = w.start + x, page = a.bt[(int64_t)w.b * a.sbt + key / a.BS];
-          if (page < 0 || page >= a.blocks) continue;
-          const uint4* e = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
-                                                          (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0);
-          const uint4 lo = e[0], hi = e[1];
-          const uint32_t z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          uint32_t some = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) some |= not_finite<F16>(z[i]);
-          if (some == 0) continue;
-          const bool mine = (x & 127) >= col && (x & 127) < col + W;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint16_t h = (uint16_t)(z[i >> 1] >> (16 * (i & 1)));
-            const float y = F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
-            if (!(fabsf(y) < INFINITY)) {
-              if (mine) own[i] += y;
-              else others |= 1u << i;
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!(fabsf(o[i]) < INFINITY) && (own[i] != 0.0f || ((others >> i) & 1u))) o[i] = own[i];
-      };
       float* piece = reinterpret_cast<float*>(smem) + wg * 128 * CD;  // [128][CD], 4 floats a chunk, swizzled
       const int t2 = tid & 127;
 #pragma unroll 1
@@ -810,10 +836,19 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             }
             if constexpr (!Q8) {
               if (copies > 1 && lall < INFINITY) {  // (NaN weights are NaN whatever the values)
-                bool bad = false;
+                float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) bad |= !(fabsf(o[i]) < INFINITY);
-                if (bad) context_infinities(o, c + k);
+                for (int i = 0; i < 16; i += 2) top = max3_nan(top, fabsf(o[i]), fabsf(o[i + 1]));
+                if (!(top < INFINITY)) {
+                  float y[16];
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) y[i] = o[i];
+                  ptc_context_infinities<F16>(y, a.bt + (int64_t)w.b * a.sbt, a.BS, a.blocks,
+                                              reinterpret_cast<const uint16_t*>(vcache) + (int64_t)w.g * s_head + c + k, s_block,
+                                              s_page, w.start, w.jedge * 128, col, W);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = y[i];
+                }
               }
             }
             if (single) {
@@ -840,7 +875,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
             v.w += z.w;
           }
           const int row = w.row0 + x, t = (int)((uint32_t)row * a.g_inv >> 16), h = w.g * a.G + row - t * a.G;
-          if (any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
+          if (NOTES && any) {  // values that were taken out: added as they are (their weight is positive) to the rows that see them
             const uint64_t rw = (a.mask ? a.mask[w.first + t] : ~0ull >> (63 - min(t, 63))) & (~0ull >> (64 - w.T));
 #pragma unroll 1
             for (int k = 0; k < 256; ++k) {
@@ -849,13 +884,17 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               if (key >= w.end || (d >= 0 && !((rw >> d) & 1ull))) continue;
               const int page = a.bt[(int64_t)w.b * a.sbt + key / a.BS];
               if (page < 0 || page >= a.blocks) continue;
-              const uint16_t* e = reinterpret_cast<const uint16_t*>(vcache) + (int64_t)page * s_block +
-                                  (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0;
+              const int64_t at = (int64_t)page * s_block + (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0;
               float y[4];
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
-                y[n] = F16 ? __half2float(__ushort_as_half(e[n])) : __uint_as_float((uint32_t)e[n] << 16);
-                if (fabsf(y[n]) < INFINITY) y[n] = 0.0f;
+                if constexpr (Q8) {
+                  y[n] = (reinterpret_cast<const uint8_t*>(vcache)[at + n] & 0x7f) == 0x7f ? NAN : 0.0f;
+                } else {
+                  const uint16_t e = reinterpret_cast<const uint16_t*>(vcache)[at + n];
+                  y[n] = F16 ? __half2float(__ushort_as_half(e)) : __uint_as_float((uint32_t)e << 16);
+                  if (fabsf(y[n]) < INFINITY) y[n] = 0.0f;
+                }
               }
               v.x += y[0];
               v.y += y[1];
