@@ -346,3 +346,86 @@ def test_tree_hidden_values_that_are_not_finite_change_no_bit(kind, T, D):
         assert bool(torch.isnan(got[sees][:, 4:, D - 1]).all())
     else:
         assert bool((got[sees][:, 4:, D - 1] == float("inf")).all()) and bool((got[sees][:, 4:, 16] == -float("inf")).all())
+
+
+# ---- further calls that the documentation allows
+@pytest.mark.parametrize("dtype", [None, I8, E4])
+@pytest.mark.parametrize("T", [3, 6, 33])
+def test_tree_pages_that_do_not_exist(dtype, T):
+    """Tokens on pages outside the cache are not seen: single pages, a whole block of keys, the first page and the last."""
+    H, KV, D, lens = 8, 2, 128, [90, 1200, 640]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(3 * T, H, D, generator=gen(5)).to(BF)
+    gone = {0: [1], 1: [3, 20] + list(range(32, 48)), 2: [0] + [39]}
+    for b, pages in gone.items():
+        for i, x in enumerate(pages):
+            c.dt[b, x] = (-1, c.dk.shape[0], 2 ** 31 - 1, -(2 ** 31))[i % 4]
+    got = tree(c, q, [T] * 3, 0.1, None)
+    for b, L in enumerate(lens):
+        seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+        for x in gone[b]:
+            seen[:, x * 16:(x + 1) * 16] = False
+        want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 0.1, BF, dtype is not None)
+        check(got[b * T:b * T + T], want, bound, b)
+
+
+@pytest.mark.parametrize("dtype", [None, I8, E4])
+@pytest.mark.parametrize("T", [1, 4, 6, 33])
+def test_negative_softmax_scales(dtype, T):
+    H, KV, D, lens = 8, 2, 64, [90, 700, 2100]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(3 * T, H, D, generator=gen(5)).to(BF)
+    calls = [tree(c, q, [T] * 3, -0.1, None)]
+    if dtype is not None and T == 1:
+        calls.append(decode(c, q.to(DEV), -0.1))
+    for got in calls:
+        for b, L in enumerate(lens):
+            seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+            want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, -0.1, BF, dtype is not None)
+            check(got[b * T:b * T + T], want, bound, b)
+
+
+@pytest.mark.parametrize("dtype", [None, I8, E4])
+@pytest.mark.parametrize("T", [1, 4, 6, 33])
+@pytest.mark.parametrize("most", [0, 1, 300, 2050])
+def test_requests_longer_than_max_seq_len(dtype, T, most):
+    """Tokens behind max_seq_len are not seen, the drafted ones among them; the others keep their places."""
+    H, KV, D, lens = 8, 2, 128, [90, 700, 2100]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(3 * T, H, D, generator=gen(5)).to(BF)
+    calls = [tree(c, q, [T] * 3, 0.1, None, max_seq_len=most)]
+    if dtype is not None and T == 1:
+        calls.append(decode(c, q.to(DEV), 0.1, max_seq_len=most))
+    for got in calls:
+        for b, L in enumerate(lens):
+            seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+            seen[:, most:] = False
+            want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 0.1, BF, dtype is not None)
+            check(got[b * T:b * T + T], want, bound, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("T", [4, 20])
+def test_tree_offsets_beyond_32_bits(dtype, T):
+    """Caches of more than 2^32 bytes a tensor (and, 8-bit, codes beyond 2^32 elements), a sequence in the last pages."""
+    from vllm_exact import paged_attn as P
+    KV, D, H, page, L = 8, 256, 32, 16, 1000
+    c = Cache([L], page, KV, D, E4 if dtype == E4 else None)
+    q = torch.randn(T, H, D, generator=gen(7)).to(BF).to(DEV)
+    want = tree(c, q, [T], 0.1, None)
+    blocks = 2 ** 32 // (KV * D * page) // (1 if dtype == E4 else 2) + 70
+    wide = c.dt.shape[1]
+    to = torch.arange(blocks - wide, blocks, device=DEV)
+    big = []
+    for x in (c.dk, c.dv):
+        y = torch.zeros(blocks, page, KV, D, dtype=torch.uint8 if dtype == E4 else BF, device=DEV)
+        y[to] = (x.view(torch.uint8) if dtype == E4 else x)[c.dt[0].long()]
+        big.append(y.view(E4) if dtype == E4 else y)
+    scales = [None, None]
+    if dtype == E4:
+        for i, s in enumerate(c.ds):
+            scales[i] = torch.zeros(blocks, KV, page, device=DEV)
+            scales[i][to] = s[c.dt[0].long()]
+    out = torch.empty_like(q)
+    P.tree_attention(q, *big, to.view(1, -1).to(torch.int32), c.dl, cu([T]), 0.1, out, T, key_scale=scales[0], value_scale=scales[1])
+    assert torch.equal(out, want)
