@@ -429,3 +429,23 @@ def test_tree_offsets_beyond_32_bits(dtype, T):
     out = torch.empty_like(q)
     P.tree_attention(q, *big, to.view(1, -1).to(torch.int32), c.dl, cu([T]), 0.1, out, T, key_scale=scales[0], value_scale=scales[1])
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [None, E4])
+@pytest.mark.parametrize("T", [4, 6, 33])
+def test_tree_lengths_around_the_segments(dtype, T):
+    """Requests as long as the lengths at which the segments change, one shorter and one longer; each has its bits alone."""
+    from vllm_exact import paged_attn as P
+    H, KV, D = 4, 1, 64
+    lens = [x + d for x in (512, 2048, 8192, 10000, 16384) for d in (-1, 0, 1)]
+    c = Cache(lens, 16, KV, D, dtype)
+    q = torch.randn(len(lens) * T, H, D, generator=gen(5)).to(BF)
+    got = tree(c, q, [T] * len(lens), 0.1, None)
+    for b, L in enumerate(lens):
+        seen = torch.ones(T, L, dtype=torch.bool).tril(L - T)
+        want, bound = close(q[b * T:b * T + T], c.seq(0, b), c.seq(1, b), seen, 0.1, BF, dtype is not None)
+        check(got[b * T:b * T + T], want, bound, L)
+        one = torch.empty(T, H, D, dtype=BF, device=DEV)
+        P.tree_attention(q[b * T:b * T + T].to(DEV), c.dk, c.dv, c.dt[b:b + 1], c.dl[b:b + 1], cu([T]), 0.1, one, T,
+                         key_scale=c.ds[0], value_scale=c.ds[1], max_seq_len=L)
+        assert torch.equal(one, got[b * T:b * T + T]), L

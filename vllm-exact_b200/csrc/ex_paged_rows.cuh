@@ -27,15 +27,22 @@ constexpr int PR_MAX_TOKENS = 64;  // drafted tokens of a request (bits of a mas
 constexpr float PR_LOG2E = 1.4426950408889634f;
 
 // Keys a segment, by the request's own length alone: the order of its sums must not depend on the batch. Short segments spread
-// a request over more SMs; every segment costs its partial results' traffic, and with many rows a CTA's start and end (15000
-// cycles of a 2048-key segment's 45000).
+// a request over more SMs; every segment costs its partial results' traffic, and with many rows a CTA's start and end.
 // At most 16 rows a KV head: 256 up to 2048 keys (256 requests of 1024 keys, e4m3: 120 us; 128: 131; 64: 160; one request of
 // 1000 keys: 19, 16, 16 us), 512 behind (16 requests of 16384 keys, int8: 130 us; 256: 142; 1024: 136; one such request:
 // 31, 31, 44 us).
 __host__ __device__ inline int pr_segment(int64_t L) { return L <= 2048 ? 256 : 512; }
-// More rows: 512, from 2048 keys on 2048 (64 requests of 8192 keys, 16 tokens: 455 us; 1024: 613; 32 requests, D = 256: 212,
-// with 4096: 252 us), from 12288 keys on 4096 (16 requests of 16384 keys, e4m3: 242 us; 2048: 268; 8192: 328).
-__host__ __device__ inline int pr_segment_many(int64_t L) { return L <= 2048 ? 512 : L <= 12288 ? 2048 : 4096; }
+// More rows: 512 up to 2048 keys, behind them equal quarters of the request in whole blocks of 128 keys, of at least 2048 and at
+// most 4096. Long segments cost a batch least, short ones spread a single request. 32 heads over 8 of 128, 16 tokens,
+// bf16 | e4m3, microseconds with segments of 512, 1024, 2048, 4096 keys:
+//   one request of  2500 keys   25   27   36   43 |  29   33   48   55      64 of 8192   729  532  458  411 | 973  709  577  504
+//                   4096        24   28   37   56 |  30   36   49   72      32 of 3000   171  141  137  127 | 216  174  162  139
+//                   16384       49   37   46   63 |  55   42   54   78      4 of 16384   121   99   82   67 | 150  118   98   83
+//                   65536      155  116   89   71 | 178  133  104   86
+__host__ __device__ inline int pr_segment_many(int64_t L) {
+  const int quarter = L < 16384 ? (int)((L + 511) >> 9) << 7 : 4096;
+  return L <= 2048 ? 512 : quarter < 2048 ? 2048 : quarter;
+}
 __host__ __device__ inline int pr_segments(int64_t L) {
   const int s = pr_segment(L), n = (int)((L + s - 1) / s);
   return n < 1 ? 1 : n;
