@@ -310,15 +310,10 @@ cudaError_t launch_few_t(const CUtensorMap& mk, const CUtensorMap& mv, const ex:
   return launch_smem(ex::k_paged_few<D, CODE, F16, NT>, ready, 0, dim3(grid), 32 * C::NW, C::SMEM, st, mk, mv, a);
 }
 
-struct CacheStrides {
-  const void* v;
-  int64_t block, page, head;
-};
-
 // Requests of at most 16 rows a KV head go to k_paged_few, the others to k_tree_tc: by their own number of rows, so that
 // a request's bits do not depend on the longest one of the batch.
 template <int D, int CODE, bool F16>
-cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const CacheStrides& c, ex::PrArgs a,
+cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& mv, ex::PrArgs a,
                            int64_t per_tile, cudaStream_t st) {
   a.rows_lo = 0;
   a.rows_hi = ex::PR_FEW;
@@ -331,18 +326,17 @@ cudaError_t launch_rows_nt(int rows, const CUtensorMap& mk, const CUtensorMap& m
   using C = ex::PtcCfg<D, CODE>;
   static KernelReady ready;
   const int grid = (int)std::min<int64_t>(per_tile * cdiv(rows, 128), num_sms());
-  return launch_smem(ex::k_tree_tc<D, CODE, F16>, ready, C::REGS, dim3(grid), C::THREADS, C::SMEM, st, mk, mv, a, c.v,
-                     c.block, c.page, c.head);
+  return launch_smem(ex::k_tree_tc<D, CODE, F16>, ready, C::REGS, dim3(grid), C::THREADS, C::SMEM, st, mk, mv, a);
 }
 
 template <int D>
 cudaError_t launch_rows_d(int code, int q_dtype, int rows, const CUtensorMap& mk, const CUtensorMap& mv,
-                          const CacheStrides& c, const ex::PrArgs& a, int64_t per_tile, cudaStream_t st) {
+                          const ex::PrArgs& a, int64_t per_tile, cudaStream_t st) {
   cudaError_t e;
-  if (code == ex::CODE_INT8) e = launch_rows_nt<D, ex::CODE_INT8, true>(rows, mk, mv, c, a, per_tile, st);
-  else if (code == ex::CODE_E4M3) e = launch_rows_nt<D, ex::CODE_E4M3, true>(rows, mk, mv, c, a, per_tile, st);
-  else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, c, a, per_tile, st);
-  else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, c, a, per_tile, st);
+  if (code == ex::CODE_INT8) e = launch_rows_nt<D, ex::CODE_INT8, true>(rows, mk, mv, a, per_tile, st);
+  else if (code == ex::CODE_E4M3) e = launch_rows_nt<D, ex::CODE_E4M3, true>(rows, mk, mv, a, per_tile, st);
+  else if (q_dtype == EX_DTYPE_F16) e = launch_rows_nt<D, ex::CODE_NONE, true>(rows, mk, mv, a, per_tile, st);
+  else e = launch_rows_nt<D, ex::CODE_NONE, false>(rows, mk, mv, a, per_tile, st);
   if (e != cudaSuccess || a.NS == 1) return e;
   const dim3 grid((unsigned)cdiv(a.tokens * a.H * (D / 64), 4)), block(128);
   if (q_dtype == EX_DTYPE_F16) return ex_launch_pdl(ex::k_paged_rows_merge<D, true>, grid, block, 0, st, a);
@@ -394,6 +388,7 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   a.n = n; a.H = H; a.G = G; a.g_inv = (65536u + G - 1) / G; a.KV = KV; a.BS = BS; a.group_log2 = BS % 16 == 0 ? 4 : 3; a.max_tokens = max_tokens;
   a.max_keys = (int)max_len; a.blocks = num_blocks; a.tokens = tokens; a.scale_log2 = scale * ex::PR_LOG2E;
   a.k_scale = k_scale; a.v_scale = v_scale; a.ss_block = ss_block; a.ss_head = ss_head; a.NS = NS;
+  a.v = v_cache; a.sv_block = s_block; a.sv_page = s_page; a.sv_head = s_head;
   if (need > 0) {
     char* w = reinterpret_cast<char*>(workspace);
     a.ws_m = reinterpret_cast<float*>(w);
@@ -406,11 +401,10 @@ int paged_rows(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const voi
   if (!encode_rows_map(&mk, k_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box) ||
       !encode_rows_map(&mv, v_cache, esz, D, KV, BS, num_blocks, s_head, s_page, s_block, pitch, box))
     return EX_ERR_UNSUPPORTED;
-  const CacheStrides c = {v_cache, s_block, s_page, s_head};
   cudaError_t e;
-  if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
-  else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
-  else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, c, a, per_tile, st);
+  if (D == 64) e = launch_rows_d<64>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  else if (D == 128) e = launch_rows_d<128>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
+  else e = launch_rows_d<256>(code, q_dtype, per_tile_rows, mk, mv, a, per_tile, st);
   return rows_status(e);
 }
 

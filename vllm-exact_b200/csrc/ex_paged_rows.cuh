@@ -12,9 +12,12 @@
 // the others k_tree_tc's (ex_tree_tc.cuh), by their own number of rows.
 //
 // 8-bit codes become float16 (exact). The key scale multiplies the score; the value scale goes into P: P is p_j vs_j over a
-// reference of the row's own, the largest p_j vs_j of the keys that it sees so far, taken up like m and carried along when m
-// is; it multiplies O in the end. So float16 P keeps 11 bits of every product that counts, and what a hidden key or one of
-// next to no weight has for a value scale is nothing to the row.
+// reference of the row's own, the largest p_j vs_j of the keys that it sees so far. So float16 P keeps 11 bits of every product
+// that counts, and what a hidden key or one of next to no weight has for a value scale is nothing to the row.
+//
+// P is rounded to the 16 bits of V (codes: to float16), since one product takes both in one type: half a step, 2^-8 of a weight
+// over bf16, 2^-11 over float16 and codes, with sums of unrounded weights below it. ex_paged_decode holds P as two bf16 numbers,
+// which costs a second product for V: its results are the finer ones, and other bits than these.
 // Queries are brought to float16 by a power of two per row, exact for all elements above 2^-14 of the row's largest.
 #pragma once
 #include "ex_cache_q8.cuh"
@@ -88,6 +91,8 @@ struct PrArgs {
   int NS;
   uint32_t g_inv;            // ceil(2^16 / G): x / G is x g_inv >> 16 for x < 4096 (G <= 16)
   int rows_lo, rows_hi;      // requests with rows_lo < T G <= rows_hi are this kernel's
+  const void* v;             // the values as the tensor map reads them, for those that are not finite
+  int64_t sv_block, sv_page, sv_head;
   float* ws_m;
   float* ws_l;
   float* ws_acc;
@@ -147,6 +152,12 @@ struct PrWalk {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {  // (-infinity for what is below the normal numbers)
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -232,10 +243,9 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
 // At most 16 rows of a KV head: a decode step, or a few drafted tokens.
 //
 // Every warp streams its own items: it loads blocks of 16 MK keys into its own ring, S blocks ahead and on into its next
-// item, and computes S^T = K Q^T, P and O^T += V^T P^T on what has arrived. No thread waits for another warp. m is taken up
-// only when a score passes it by more than 6 (a factor of 64; p stays small enough for float16), and the reference of
-// weights times value scales when one is 64 times it: the common path has two votes and no shuffles. Both are decided for
-// every row alone.
+// item, and computes S^T = K Q^T, P and O^T += V^T P^T on what has arrived. No thread waits for another warp. References are taken
+// up only when a score (16-bit) or a weight times its value scale (codes) is more than 64 times them (p stays small enough
+// for float16): the common path has one vote and no shuffles. It is decided for every row alone.
 // Bound by the cache's bytes where there are many requests (64 of 8192 keys, int8: 209 us, 5.3 TB/s of 6.56 measured; 256 of
 // 1024, e4m3: 119 us, 4.7 TB/s; 16-bit, 4 tokens: 411 us, 5.2 TB/s), and before that by the instructions that make float16
 // of codes and weights of scores; one request of 1000 keys takes 19 us, most of it two launches and first uses of code.
@@ -245,9 +255,11 @@ struct PfCfg {
   static constexpr int ROW = (CODE == CODE_NONE ? 2 : 1) * D;  // bytes of a key
   // 16-key tiles of a block: two where the registers have room for them (256 requests of 1024 keys, e4m3: 119 us, with one 133)
   static constexpr int MK = ROW <= 128 ? 2 : 1;
-  // Warps of a CTA, one CTA per SM: as many as rings of enough blocks fit in shared memory and results in registers (the same
-  // batch: 12 warps 119 us, 8 124, 4 186; 64 requests of 8192 keys, D = 256: 8 warps 207 us, 4 294)
-  static constexpr int NW = ROW <= 128 ? 12 : ROW <= 256 ? 8 : 4;
+  // Warps of a CTA, one CTA per SM: as many as rings of enough blocks fit in shared memory and results in registers. At most 8
+  // rows (NT = 1): the same batch with 12 warps 119 us, 8 124, 4 186; 64 requests of 8192 keys, D = 256: 8 warps 207 us, 4
+  // 294. 16 rows: codes of D = 128 do not fit the registers of 12 warps (64 requests of 8192 keys, e4m3, 4 tokens: 8 warps
+  // 248 us, 10 311, 12 302), of D = 64 they do (8 warps 196 us, 12 164); D = 256: 8 warps 296 us, 6 367 (some spills in both).
+  static constexpr int NW = ROW > 256 ? 4 : ROW > 128 || (NT == 2 && CODE != CODE_NONE && D == 128) ? 8 : 12;
   static constexpr int BLK = 16 * MK;
   using R = PrTile<D, CODE, BLK>;
   static constexpr int STAGE = 2 * R::TILE;
@@ -428,18 +440,20 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
       fac[i] = Q8 ? __shfl_sync(0xffffffffu, qs[i >> 1], (qc + (i & 1)) * 4) * a.scale_log2 : a.scale_log2;
 
     float m[2 * NT], l[2 * NT], o[KT][NT][4];
-    float vref[2 * NT], vinv[2 * NT];  // codes: O is the sum of p vs c over vref; 1 / vref
+    float vtop[2 * NT];  // codes: O is the sum of 2^(x - vtop) vs c
+    bool apart = false;  // of some row m and vtop differ
 #pragma unroll
     for (int i = 0; i < 2 * NT; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.0f;
-      vref[i] = vinv[i] = 0.0f;
+      vtop[i] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
 
+    bool noted = false;
     for (int kb = start; kb < end; kb += BLK) {
       ok = mbar_wait(full_bar + st, phase, EX_DEVERR_WAIT_TMA);
       ok = __all_sync(0xffffffffu, ok);
@@ -497,10 +511,8 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             sc[i][j][2 * e + 1] *= Q8 ? fac[2 * j + 1] * ksc : fac[2 * j + 1];
           }
         }
-      bool odd = false;  // a value that is not finite and that some row may not see
       uint32_t hidden = 0;  // bit ((i NT + j) 4 + e): the row does not see the key
       if (!whole) {
-        uint32_t bad = 0;
 #pragma unroll
         for (int i = 0; i < MK; ++i) {
 #pragma unroll
@@ -532,47 +544,83 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             if (none) {
               *x = make_uint4(0, 0, 0, 0);  // values that may not be read: 0 * NaN would reach O
             } else if constexpr (CODE != CODE_INT8) {
-              bad |= not_finite<CODE, F16>(x->x) | not_finite<CODE, F16>(x->y) | not_finite<CODE, F16>(x->z) | not_finite<CODE, F16>(x->w);
+              // values that are not finite and that some row may not see: taken out, and in the end added to the rows that do
+              if (not_finite<CODE, F16>(x->x) | not_finite<CODE, F16>(x->y) | not_finite<CODE, F16>(x->z) | not_finite<CODE, F16>(x->w)) {
+                *x = make_uint4(only_finite<CODE, F16>(x->x), only_finite<CODE, F16>(x->y), only_finite<CODE, F16>(x->z), only_finite<CODE, F16>(x->w));
+                noted = true;
+              }
             }
           }
         }
         fence_proxy_async_shared();  // the ring slot is written by TMA next
         __syncwarp();
-        if constexpr (CODE != CODE_INT8) odd = __any_sync(0xffffffffu, bad != 0);
       }
-      // references: taken up for the rows that need it
-      float top[2 * NT];
+      // references: taken up for the rows that need it. No product of a lane passes its largest score with its largest value
+      // scale (but for roundings, hence 5.9): so one vote decides for scores and products, before a weight is made. Which other
+      // rows of the warp need it makes no difference to a row.
+      float top[2 * NT], lv = -INFINITY;
       bool need = false;
+      if constexpr (Q8) {
+        float v = fmaxf(vsc[0][0], vsc[0][1]);  // (NaN: left out)
+#pragma unroll
+        for (int i = 1; i < MK; ++i) v = fmaxf(v, fmaxf(vsc[i][0], vsc[i][1]));
+        lv = lg2(v);
+      }
 #pragma unroll
       for (int x = 0; x < 2 * NT; ++x) {
         float v = fmaxf(sc[0][x >> 1][x & 1], sc[0][x >> 1][2 + (x & 1)]);
 #pragma unroll
         for (int i = 1; i < MK; ++i) v = fmaxf(v, fmaxf(sc[i][x >> 1][x & 1], sc[i][x >> 1][2 + (x & 1)]));
         top[x] = v;
-        need |= v > m[x] + 6.0f;
+        need |= Q8 ? v > m[x] + 60.0f || v + lv > vtop[x] + 5.9f : v > m[x] + 6.0f;
       }
-      const bool moved = __any_sync(0xffffffffu, need);
-      if (moved) {
+      if (__any_sync(0xffffffffu, need)) {
+        float be[2 * NT];  // what O is scaled by
+        bool some = false, differ = false;
 #pragma unroll
         for (int x = 0; x < 2 * NT; ++x) {
-          float v = top[x];
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          if (v > m[x] + 6.0f) {  // (for m = -inf as well)
-            const float al = ex2(m[x] - v);
-            m[x] = v;
-            l[x] *= al;
-            if constexpr (Q8) {
-              vref[x] *= al;  // (O stays: it is over the reference)
-            } else {
+          float v = top[x], vb = -INFINITY;  // the row's largest score, and the largest with the value scale in it
+          if constexpr (Q8) {
 #pragma unroll
-              for (int mt = 0; mt < KT; ++mt) {
-                o[mt][x >> 1][x & 1] *= al;
-                o[mt][x >> 1][2 + (x & 1)] *= al;
-              }
-            }
+            for (int i = 0; i < MK; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) vb = fmaxf(vb, sc[i][x >> 1][2 * e + (x & 1)] + lg2(vsc[i][e]));
           }
+#pragma unroll
+          for (int d = 4; d <= 16; d <<= 1) {
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+            if constexpr (Q8) vb = fmaxf(vb, __shfl_xor_sync(0xffffffffu, vb, d));
+          }
+          be[x] = 1.0f;
+          if constexpr (Q8) {
+            if (v > m[x] + 60.0f || vb > vtop[x] + 6.0f) {  // (the row's own: what other rows need does not matter)
+              // Weights are over the products' reference, so that these need no factor, as long as that is not above the largest
+              // score and at most 60 below it (weights and their sum stay far from the largest numbers). The products' is at
+              // least 126 below it: what they lose then (2^-25 times 2^-126 times a code) is below bf16's smallest step.
+              const float most = fmaxf(v, m[x]), high = vb > vtop[x] + 6.0f ? vb : vtop[x];
+              const float mn = fmaxf(m[x], fminf(fmaxf(high, most - 60.0f), most)), to = fmaxf(high, mn - 66.0f);
+              l[x] *= ex2(m[x] - mn);
+              m[x] = mn;
+              be[x] = ex2(vtop[x] - to);
+              vtop[x] = to;
+            }
+            differ |= m[x] != vtop[x];
+          } else if (v > m[x] + 6.0f) {  // (for m = -inf as well)
+            be[x] = ex2(m[x] - v);
+            m[x] = v;
+            l[x] *= be[x];
+          }
+          some |= be[x] != 1.0f;
+        }
+        if constexpr (Q8) apart = __any_sync(0xffffffffu, differ);
+        if (kb > start && __any_sync(0xffffffffu, some)) {  // (the first block's O is 0)
+#pragma unroll
+          for (int x = 0; x < 2 * NT; ++x)
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt) {
+              o[mt][x >> 1][x & 1] *= be[x];
+              o[mt][x >> 1][2 + (x & 1)] *= be[x];
+            }
         }
       }
       // weights; for codes times the keys' value scales (of a key that is not seen it may be anything)
@@ -597,43 +645,15 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
             }
           }
         }
-      if constexpr (Q8) {
-        float high[2 * NT];
-        bool rise = moved;
+      if (Q8 && apart) {
 #pragma unroll
         for (int x = 0; x < 2 * NT; ++x) {
-          float v = fmaxf(sc[0][x >> 1][x & 1], sc[0][x >> 1][2 + (x & 1)]);  // (NaN: left out)
+          const float half = ex2(0.5f * (m[x] - vtop[x])), f = m[x] == vtop[x] ? 1.0f : half * half;  // (may be below the normal numbers)
 #pragma unroll
-          for (int i = 1; i < MK; ++i) v = fmaxf(v, fmaxf(sc[i][x >> 1][x & 1], sc[i][x >> 1][2 + (x & 1)]));
-          high[x] = v;
-          rise |= v > 64.0f * vref[x];
+          for (int i = 0; i < MK; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sc[i][x >> 1][2 * e + (x & 1)] *= f;
         }
-        if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-          for (int x = 0; x < 2 * NT; ++x) {
-            float v = high[x] < INFINITY ? high[x] : 0.0f;
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            // At least 2^-126, so that its reciprocal is a number: products down to 2^-149 are then above 2^-24, and what they
-            // lose (2^-25 times 2^-126 times a code) is below bf16's smallest step.
-            const float to = fmaxf(v > 64.0f * vref[x] ? v : vref[x], 0x1p-126f);
-            vinv[x] = __frcp_rn(to);
-            const float be = to == vref[x] ? 1.0f : vref[x] * vinv[x];
-            vref[x] = to;
-#pragma unroll
-            for (int mt = 0; mt < KT; ++mt) {
-              o[mt][x >> 1][x & 1] *= be;
-              o[mt][x >> 1][2 + (x & 1)] *= be;
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < MK; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[i][j][e] *= vinv[2 * j + (e & 1)];
       }
       uint32_t pb[MK][NT][2];
 #pragma unroll
@@ -643,44 +663,6 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
           pb[i][j][0] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][0], sc[i][j][1]) : pack_bf16(sc[i][j][0], sc[i][j][1]));
           pb[i][j][1] = movmatrix_t(MF16 ? pack2<__half>(sc[i][j][2], sc[i][j][3]) : pack_bf16(sc[i][j][2], sc[i][j][3]));
         }
-      if (CODE != CODE_INT8 && odd) {
-        // Added as they are (their weight is positive, however small) to the rows that see them, then taken out: 0 times one of
-        // them would reach the others. Dims of a lane: 16-bit qr, qr + 8 of every 16, codes 2 qr, 2 qr + 1.
-#pragma unroll 1
-        for (int kk = 0; kk < 16 * MK; ++kk) {
-          const int d = kb + kk - ctx;
-#pragma unroll
-          for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint8_t* at = vs + (Q8 ? pr_at<C::PITCH, C::HALF>(kk, mt) + 2 * qr + u : pr_at<C::PITCH, C::HALF>(kk, 2 * mt + u) + 2 * qr);
-              float v;
-              if constexpr (Q8) {
-                v = (*at & 0x7f) == 0x7f ? NAN : 0.0f;
-              } else {
-                const uint16_t w = *reinterpret_cast<const uint16_t*>(at);
-                v = F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
-              }
-              if (fabsf(v) < INFINITY) continue;
-#pragma unroll
-              for (int x = 0; x < 2 * NT; ++x) {
-                const int r = (x >> 1) * 8 + qc + (x & 1), t = r / a.G;
-                if (r >= R) continue;
-                if (d >= 0 && !(((a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull)) >> d) & 1ull)) continue;
-                o[mt][x >> 1][2 * u + (x & 1)] += v;
-              }
-            }
-        }
-        __syncwarp();
-#pragma unroll 1
-        for (int i = 0; i < 16 * MK; ++i)
-          for (int c = lane; c < C::ROW / 16; c += 32) {
-            uint4* x = reinterpret_cast<uint4*>(vs + pr_at<C::PITCH, C::HALF>(i, c));
-            *x = make_uint4(only_finite<CODE, F16>(x->x), only_finite<CODE, F16>(x->y), only_finite<CODE, F16>(x->z), only_finite<CODE, F16>(x->w));
-          }
-        fence_proxy_async_shared();
-        __syncwarp();
-      }
       const int mi = lane >> 3;
 #pragma unroll
       for (int i = 0; i < MK; ++i) {
@@ -713,6 +695,36 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
       load_block();  // into the slot that was just read
     }
     if (!ok) break;
+    if (CODE != CODE_INT8 && __any_sync(0xffffffffu, noted)) {
+      // Values that are not finite: added as they are (their weight is positive, however small) to the rows that see them; what
+      // blocks that are seen whole have made of them stays. Dims of a lane: 16-bit qr, qr + 8 of every 16, codes 2 qr, 2 qr + 1.
+#pragma unroll 1
+      for (int key = start; key < end; ++key) {
+        const int pg = a.bt[(int64_t)b * a.sbt + key / a.BS], d = key - ctx;
+        if (pg < 0 || pg >= a.blocks) continue;
+        const int64_t at = (int64_t)pg * a.sv_block + (int64_t)(key % a.BS) * a.sv_page + (int64_t)g * a.sv_head;
+#pragma unroll
+        for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float v;
+            if constexpr (Q8) {
+              v = (reinterpret_cast<const uint8_t*>(a.v)[at + mt * 16 + 2 * qr + u] & 0x7f) == 0x7f ? NAN : 0.0f;
+            } else {
+              const uint16_t w = reinterpret_cast<const uint16_t*>(a.v)[at + mt * 16 + qr + 8 * u];
+              v = F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+            }
+            if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+            for (int x = 0; x < 2 * NT; ++x) {
+              const int r = (x >> 1) * 8 + qc + (x & 1), t = r / a.G;
+              if (r >= R) continue;
+              if (d >= 0 && !(((a.mask ? a.mask[first + t] : (t >= 63 ? ~0ull : (2ull << t) - 1ull)) >> d) & 1ull)) continue;
+              o[mt][x >> 1][2 * u + (x & 1)] += v;
+            }
+          }
+      }
+    }
     const bool single = pr_segments(keys) == 1;
 #pragma unroll
     for (int x = 0; x < 2 * NT; ++x) {
@@ -723,7 +735,7 @@ __global__ void __launch_bounds__(32 * PfCfg<D, CODE, NT>::NW, 1)
       const int c = (x >> 1) * 8 + qc + (x & 1);
       if (c >= R) continue;
       const int t = c / a.G, h = g * a.G + c % a.G;
-      const float up = Q8 ? vref[x] : 1.0f;
+      const float half = ex2(0.5f * (vtop[x] - m[x])), up = !Q8 || vtop[x] == m[x] ? 1.0f : half * half;
       // 16 dims a tile: codes 2 qr, 2 qr + 1; 16-bit qr, qr + 8
       if (single) {
         const float inv = lx > 0.0f ? up / lx : (lx == 0.0f ? 0.0f : lx);  // nothing seen: zeros; NaN stays NaN

@@ -166,7 +166,7 @@ constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values t
 template <int D, int CODE, bool F16>
 __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     k_tree_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-              const __grid_constant__ PrArgs a, const void* vcache, int64_t s_block, int64_t s_page, int64_t s_head) {
+              const __grid_constant__ PrArgs a) {
   using C = PtcCfg<D, CODE>;
   constexpr bool Q8 = C::Q8;
   constexpr bool MF16 = Q8 || F16;
@@ -844,8 +844,8 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
 #pragma unroll
                   for (int i = 0; i < 16; ++i) y[i] = o[i];
                   ptc_context_infinities<F16>(y, a.bt + (int64_t)w.b * a.sbt, a.BS, a.blocks,
-                                              reinterpret_cast<const uint16_t*>(vcache) + (int64_t)w.g * s_head + c + k, s_block,
-                                              s_page, w.start, w.jedge * 128, col, W);
+                                              reinterpret_cast<const uint16_t*>(a.v) + (int64_t)w.g * a.sv_head + c + k, a.sv_block,
+                                              a.sv_page, w.start, w.jedge * 128, col, W);
 #pragma unroll
                   for (int i = 0; i < 16; ++i) o[i] = y[i];
                 }
@@ -884,14 +884,14 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
               if (key >= w.end || (d >= 0 && !((rw >> d) & 1ull))) continue;
               const int page = a.bt[(int64_t)w.b * a.sbt + key / a.BS];
               if (page < 0 || page >= a.blocks) continue;
-              const int64_t at = (int64_t)page * s_block + (int64_t)(key % a.BS) * s_page + (int64_t)w.g * s_head + d0;
+              const int64_t at = (int64_t)page * a.sv_block + (int64_t)(key % a.BS) * a.sv_page + (int64_t)w.g * a.sv_head + d0;
               float y[4];
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
                 if constexpr (Q8) {
-                  y[n] = (reinterpret_cast<const uint8_t*>(vcache)[at + n] & 0x7f) == 0x7f ? NAN : 0.0f;
+                  y[n] = (reinterpret_cast<const uint8_t*>(a.v)[at + n] & 0x7f) == 0x7f ? NAN : 0.0f;
                 } else {
-                  const uint16_t e = reinterpret_cast<const uint16_t*>(vcache)[at + n];
+                  const uint16_t e = reinterpret_cast<const uint16_t*>(a.v)[at + n];
                   y[n] = F16 ? __half2float(__ushort_as_half(e)) : __uint_as_float((uint32_t)e << 16);
                   if (fabsf(y[n]) < INFINITY) y[n] = 0.0f;
                 }
