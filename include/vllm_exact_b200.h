@@ -326,7 +326,9 @@ int ex_paged_decode_q8(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, c
  * context, and of the drafted tokens those of its bits: row r sees drafted token j if bit j of tree_mask[r] is set
  * (tree_mask NULL: those up to itself, a chain). A row that sees nothing gives zeros. A request with more than
  * max_tokens rows, or with rows that q (tokens rows) does not have, is left untouched, as are rows of no request.
- * Other conventions as ex_paged_decode_q8; a row's bits depend on its own request alone.
+ * Other conventions as ex_paged_decode_q8; a row's bits depend on its own request alone, and there on its number of drafted
+ * tokens, not on what those hold that the row does not see. Weights are held in 16 bits (the cache's type; codes: float16), where
+ * ex_paged_decode holds them as two bf16 numbers: the two do not give a token the same bits.
  */
 int ex_tree_attention(const void* q, int64_t sq_t, int64_t sq_h, int q_dtype, const void* k_cache, const void* v_cache,
                       int code, int64_t s_block, int64_t s_page, int64_t s_head, const float* k_scale,

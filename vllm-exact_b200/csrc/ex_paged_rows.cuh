@@ -246,9 +246,10 @@ __device__ __forceinline__ void transposed_to_f16(uint32_t w, uint32_t& even, ui
 // item, and computes S^T = K Q^T, P and O^T += V^T P^T on what has arrived. No thread waits for another warp. References are taken
 // up only when a score (16-bit) or a weight times its value scale (codes) is more than 64 times them (p stays small enough
 // for float16): the common path has one vote and no shuffles. It is decided for every row alone.
-// Bound by the cache's bytes where there are many requests (64 of 8192 keys, int8: 209 us, 5.3 TB/s of 6.56 measured; 256 of
-// 1024, e4m3: 119 us, 4.7 TB/s; 16-bit, 4 tokens: 411 us, 5.2 TB/s), and before that by the instructions that make float16
-// of codes and weights of scores; one request of 1000 keys takes 19 us, most of it two launches and first uses of code.
+// Near the cache's bytes where there are many requests (64 of 8192 keys, int8: 207 us, 5.3 TB/s of 6.56 measured; 256 of
+// 768 to 1280, e4m3: 121 us, 4.6 TB/s; 16-bit, 4 tokens: 381 us, 5.6 TB/s). No unit is full (64 of 4096, e4m3: DRAM 80 % of a
+// copy, issue slots 40 %, products 16 %): three warps a scheduler wait on their own chains of load, product, weights, product.
+// One request of 1000 keys takes 19 us: two launches, and four blocks a warp one after another.
 // ------------------------------------------------------------------------------------------------------------------
 template <int D, int CODE, int NT>
 struct PfCfg {

@@ -17,10 +17,15 @@
 //                   another sequence or to nobody, are zeroed, since 0 * NaN would reach O; values that are not finite
 //                   are zeroed and noted, and the rows that see such a key get it added at the end.
 // D = 256: one query tile and two S buffers (tensor memory holds no more), S of the next block issued before P V.
-// Bound by the products and the exponentials together, at the clock that the board's power leaves (1.6 to 1.7 GHz under this
-// load): a prompt of 16384 tokens (32 heads of 128 over 8) takes 1740 to 1890 us, 1.16 to 1.26 PFLOP/s; without its softmax it
-// would take 1554, without its products 1352 us. Steps of 64 keys with two S buffers a tile, so that no softmax waits for its
-// S: 1810 to 1980 us (a product of 64 columns reads Q as often as one of 128). Two threads a row: no faster, and spills.
+// Bound by the products and the exponentials together (busy 50 and 45 % of the cycles, in turn), at the clock that the board's
+// power leaves. Three prompts of 2048 to 8192 tokens (32 heads of 128 over 8) take 710 us, 1.13 PFLOP/s, at 1965 MHz, and called
+// for seconds, at 1657 MHz, 812 us, 0.98 PFLOP/s; one of 16384 tokens 1765 and 2058 us, and without its softmax 1554, without its
+// products 1352 us. Steps of 64 keys with two S buffers a tile, so that no softmax waits for its S: 1810 to 1980 us (a product of
+// 64 columns reads Q as often as one of 128). Two threads a row: no faster, and spills.
+//
+// P has the 16 bits of V, since a product takes both in one type: one rounding of half a step, 2^-8 of a weight over bf16, with
+// the sum of the unrounded weights below it. Relative error of the long prompts against 64 bits 0.0022, of which the
+// outputs' own rounding is 0.0016.
 #pragma once
 #include "ex_paged_rows.cuh"
 
@@ -42,7 +47,7 @@ constexpr int PA_THREADS = 384;
 constexpr int PA_KEYS = 128;
 constexpr int PA_EDGES = 4;  // 256 rows reach over at most 3 blocks that are not visible to all of them
 // Of eight pairs of weights PA_POLY are 2^x by polynomial (ex2_pair): prompts of 2048 to 8192 tokens, D = 128, take 770, 731,
-// 774 and 807 us with 0, 1, 2 and 3.
+// 774 and 807 us with 0, 1, 2 and 3. (Measured at D = 128, used for every head size.)
 constexpr int PA_POLY = 1;
 constexpr int PA_REGS_LAUNCH = 168, PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 static_assert(256 * PA_REGS_SOFTMAX + 128 * PA_REGS_OTHER <= PA_THREADS * PA_REGS_LAUNCH, "register shares");

@@ -1,5 +1,6 @@
 // Attention of many query rows per KV head (more than 16: drafted tokens times grouped heads) over a 16-bit or 8-bit
-// paged cache, on tcgen05. The mathematics and the masks are those of ex_paged_rows.cuh.
+// paged cache, on tcgen05. The mathematics and the masks are those of ex_paged_rows.cuh. Over codes m and the products' reference
+// are both kept: P is 2^(x - m) vs 2^(m - vtop), so that a key's weight is made once for the sum and the product.
 //
 // One CTA per SM takes items (request, segment of its keys, KV head, tile of 128 rows) and walks the segment in blocks
 // of 128 keys: S = Q K^T with both operands in shared memory, O += P V with P in tensor memory over the S it came
@@ -19,12 +20,14 @@
 //   warps 12-15     for codes: codes to float16 tiles (exact; values behind the end to zeros, and in blocks with drafted tokens or
 //                   the end codes that are NaN, noted as 10 and 11 do)
 // 16-bit: bound by reading the cache once (a block of 128 keys is 64 KB for D = 128, 1.5 us of an SM's share of HBM) and by an
-// item's start and end, when only as much is read as the ring holds: queries 600 cycles (their loads run during the last
-// products), first scores 1400, last products 3000, results 8000, of 45000 for 2048 keys. 64 requests of 8192 keys with 16
-// tokens: 455 us, 4.7 TB/s.
-// Codes: bound by shared memory's bandwidth, 1800 cycles a block of 128 keys (S reads both operands, 512; P V 256; the
-// converters 768; TMA 256) of the 2650 that it takes; four converter warps more change nothing. 16 requests of 16384 keys,
-// 7 tokens: 242 us, 2.3 TB/s.
+// item's start and end, when only as much is read as the ring holds (of 45000 cycles for 2048 keys 13000 by clock readings in
+// the kernel: queries 600, first scores 1400, last products 3000, results 8000). 64 requests of 6144 to 10240 keys, 16 tokens:
+// 465 us, 4.6 TB/s, at 1965 MHz; 531 us called for seconds, when the power limit leaves 1650 MHz.
+// Codes: no unit is full (counters of 16 requests of 16384 keys, 7 tokens: shared memory's pipe 53 % with the products' reads,
+// issue slots 45 %, products 32 %, DRAM 36 % of a copy); it is each block's chain of load, conversion, product, softmax. Four
+// converter warps more change nothing. 16 requests of 12288 to 20480 keys, 7 tokens: 240 us, 2.3 TB/s.
+//
+// P has the 16 bits of V (codes: float16), as in ex_paged_rows.cuh: one rounding of half a step, 2^-8 of a weight over bf16.
 #pragma once
 #include "ex_paged_rows.cuh"
 #include "ex_prompt_attn.cuh"

@@ -13,7 +13,7 @@ request, so a request's output bits are the same alone, in any batch, and under 
 
 Beside them, without a counterpart in the reference: ``paged_decode_q8``, the same over an 8-bit cache (kv_cache.py), and
 ``tree_attention``, up to 64 drafted tokens per request over a 16-bit or 8-bit cache under an ancestor mask. Their
-segments depend on the request's own length, not on MAX_LEN, with the same invariance.
+segments depend on the request's own length, not on MAX_LEN, with the same invariance; their bits are not paged_decode's.
 """
 from __future__ import annotations
 
@@ -171,6 +171,11 @@ def tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_s
     the drafted ones); of the drafted tokens row r sees number j if bit j of tree_mask[r] (int64, one word per row of
     query) is set, its own bit included if it is to see itself. tree_mask None: a chain, each row sees the drafted tokens
     up to itself. A row that sees nothing gives zeros.
+
+    Weights are held in the cache's 16 bits (8-bit caches: float16), where paged_decode holds them as two bf16 numbers:
+    over a 16-bit cache a token's bits are not those of paged_decode, and they depend on how many tokens were drafted
+    with it (requests of more than 16 rows a KV head are another kernel's). They do not depend on the other requests, nor on
+    what drafted tokens hold that the row does not see. Over an 8-bit cache one drafted token is paged_decode_q8's.
 
     The cache is 16-bit in query's type, any strides as in paged_decode, or 8-bit with key_scale and value_scale
     (kv_cache.py); block_size a multiple of 8. A request with more rows than max_query_len is left untouched, as are rows
