@@ -449,3 +449,32 @@ def test_tree_lengths_around_the_segments(dtype, T):
         P.tree_attention(q[b * T:b * T + T].to(DEV), c.dk, c.dv, c.dt[b:b + 1], c.dl[b:b + 1], cu([T]), 0.1, one, T,
                          key_scale=c.ds[0], value_scale=c.ds[1], max_seq_len=L)
         assert torch.equal(one, got[b * T:b * T + T]), L
+
+
+@pytest.mark.parametrize("kind", [BF, E4])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tree_notes_of_many_items_in_turn(kind, D):
+    """Thirty short requests a CTA, every third with a value that is not finite: no request hears of another's, however many
+    items lie between."""
+    from vllm_exact import paged_attn as P
+    H, KV, T, lens = 16, 1, 2, [20, 20]
+    c = Cache(lens, 16, KV, D, E4 if kind == E4 else None)
+    q = torch.randn(T, H, D, generator=gen(21)).to(BF).to(DEV)
+    for x in (c.dk, c.dv, *c.ds):  # the same keys and values in both sequences
+        if x is not None:
+            y = x.view(torch.uint8) if x.element_size() == 1 else x
+            y[c.dt[1].long()] = y[c.dt[0].long()]
+    blk = int(c.table[1, 0])
+    if kind == E4:
+        c.dv.view(torch.uint8)[blk, 3, 0, 5] = 0x7f
+    else:
+        c.dv[blk, 3, 0, 5] = float("inf")
+    n = 30 * torch.cuda.get_device_properties(0).multi_processor_count
+    bad = torch.arange(n, device=DEV) % 3 == 0
+    table = c.dt[bad.long()].contiguous()
+    out = torch.empty(n * T, H, D, dtype=BF, device=DEV)
+    P.tree_attention(q.repeat(n, 1, 1), c.dk, c.dv, table, torch.full((n,), 20, dtype=torch.int32, device=DEV), cu([T] * n), 0.1, out, T,
+                     key_scale=c.ds[0], value_scale=c.ds[1])
+    out = out.view(n, T, H, D)
+    assert torch.equal(out[~bad], out[1].expand(n, T, H, D)[~bad]) and bool(torch.isfinite(out[1]).all())
+    assert torch.equal(torch.isfinite(out[bad]), (torch.arange(D, device=DEV) != 5).expand(n, T, H, D)[bad])

@@ -163,8 +163,9 @@ __device__ __noinline__ void ptc_context_infinities(float* o, const int32_t* pag
 }
 
 constexpr int PTC_EDGES = 8;   // edge blocks in flight: each takes a slot of the ring
-constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values that are not finite are kept (the ring, of at most
-                               // 8 slots, runs ahead of the rows)
+constexpr int PTC_POISON = 8;  // items with edge blocks whose notes of values that are not finite are kept (the rings, of at most 8
+                               // tiles or of 6 behind the conversion, and two or more an item, run ahead of the rows, which clear
+                               // the notes that they have read)
 
 template <int D, int CODE, bool F16>
 __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
@@ -205,6 +206,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
   pdl_launch_dependents();
   if (tid == 0) {
     *sfail = 0;
+    for (int i = 0; i < PTC_POISON * 8; ++i) poison[i] = 0;
     for (int i = 0; i < 8; ++i) {
       mbar_init(full_bar + i, Q8 ? 128 : C::LOADED);
       mbar_init(empty_bar + i, 1);
@@ -445,11 +447,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     bool ok = true;
     while (ok && next()) {
       uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
-      if (jedge < nblk) {
-        ++item;
-        if (warp == 10 && lane < 8) mine[lane] = 0;
-        asm volatile("bar.sync 6, 64;" ::: "memory");
-      }
+      if (jedge < nblk) ++item;
       for (int j = jedge; j < nblk && ok; ++j) {
         const int e = j - jedge;
         // the producer's word that the slots are this block's
@@ -477,11 +475,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
       bool ok = true;
       while (ok && next()) {
         uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
-        if (NOTES && jedge < nblk) {
-          ++item;
-          if (t < 8) mine[t] = 0;
-          asm volatile("bar.sync 6, 128;" ::: "memory");
-        }
+        if (jedge < nblk) ++item;
 #pragma unroll 1
         for (int n = 0; n < 2 * nblk && ok; ++n) {
           int j;
@@ -599,7 +593,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
     };
     bool more = next_item();
     while (more) {
-      const uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
+      uint32_t* mine = poison + (item & (PTC_POISON - 1)) * 8;
       if (jedge < nblk) ++item;
       // copies of the rows: each weighs W keys of a block
       const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1, rows = 128 / copies, W = 128 / copies;
@@ -929,6 +923,7 @@ __global__ void __launch_bounds__((PtcCfg<D, CODE>::THREADS), 1)
         a.ws_l[pi] = lall;
       }
       asm volatile("bar.sync 2, 256;" ::: "memory");  // before the queries and sfac are written again
+      if (NOTES && any && tid < 8) mine[tid] = 0;     // for the item PTC_POISON on
     }
     __syncwarp();
     tc_fence_before();
