@@ -13,7 +13,9 @@
 //
 // 8-bit codes become float16 (exact). The key scale multiplies the score; the value scale goes into P: P is p_j vs_j over a
 // reference of the row's own, the largest p_j vs_j of the keys that it sees so far. So float16 P keeps 11 bits of every product
-// that counts, and what a hidden key or one of next to no weight has for a value scale is nothing to the row.
+// that counts, and what a hidden key or one of next to no weight has for a value scale is nothing to the row. (A finite
+// weight under 2^-126 of the largest is 0, as float32's normal numbers end there: with values 2^122 times the others' even such a
+// one would count.)
 //
 // P is rounded to the 16 bits of V (codes: to float16), since one product takes both in one type: half a step, 2^-8 of a weight
 // over bf16, 2^-11 over float16 and codes, with sums of unrounded weights below it. ex_paged_decode holds P as two bf16 numbers,
